@@ -90,6 +90,33 @@ class FabAttentionVarlenParams(ctypes.Structure):
     ]
 
 
+class FabAttentionBwdParams(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("v", _vp), ("o", _vp), ("dout", _vp), ("lse", _vp),
+        ("dq", _vp), ("dk", _vp), ("dv", _vp),
+        *((f"{t}_stride_{d}", _i64) for t in ("q", "k", "v", "o", "dout", "lse", "dq", "dk", "dv") for d in "bhs"),
+        ("cu_seqlens_q", _vp), ("cu_seqlens_k", _vp),
+        ("batch", _i32), ("heads_q", _i32), ("heads_kv", _i32), ("seqlen_q", _i32), ("seqlen_k", _i32),
+        ("total_q", _i32), ("total_k", _i32), ("head_dim", _i32), ("dtype", _i32), ("sm_scale", _f32),
+        ("causal", _i32), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+MAX_ROPE_AXES = 4
+
+
+class FabRopeAxesParams(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("q_out", _vp), ("k_out", _vp), ("positions", _vp), ("cos", _vp), ("sin", _vp),
+        ("q_stride_t", _i64), ("q_stride_h", _i64), ("k_stride_t", _i64), ("k_stride_h", _i64),
+        ("q_out_stride_t", _i64), ("q_out_stride_h", _i64), ("k_out_stride_t", _i64), ("k_out_stride_h", _i64),
+        ("positions_stride_axis", _i64), ("positions_stride_t", _i64),
+        ("tokens", _i32), ("heads_q", _i32), ("heads_k", _i32), ("head_dim", _i32), ("axes", _i32),
+        ("sections", _i32 * MAX_ROPE_AXES), ("table_rows", _i32), ("positions_64bit", _i32), ("inverse", _i32),
+        ("dtype", _i32),
+    ]
+
+
 MAX_TP_RANKS = 8
 
 
@@ -133,6 +160,8 @@ PROTOTYPES = {
     "fab_flash_attn_fwd_block_d_nomask_contiguous": (_i32, [_vp] * 4 + [_i32] * 5 + [_f32, _i32, _vp]),
     "fab_attention_fwd": (_i32, [ctypes.POINTER(FabAttentionParams), _vp]),
     "fab_attention_fwd_varlen": (_i32, [ctypes.POINTER(FabAttentionVarlenParams), _vp]),
+    "fab_attention_bwd_workspace": (_i32, [ctypes.POINTER(FabAttentionBwdParams), ctypes.POINTER(ctypes.c_size_t)]),
+    "fab_attention_bwd": (_i32, [ctypes.POINTER(FabAttentionBwdParams), _vp]),
     "fab_attention_fwd_variant": (_i32, [ctypes.POINTER(FabAttentionParams), _i32, _vp]),
     "fab_flash_attn_config_variant": (_i32, [_i32, _i32, _i32, ctypes.POINTER(FabFaConfig)]),
     "fab_attention_fwd_plan": (_i32, [ctypes.POINTER(FabAttentionParams), _i32, ctypes.POINTER(FabFaPlan)]),
@@ -158,6 +187,10 @@ PROTOTYPES = {
     "fab_rmsnorm_rstd": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i64, _i64, _i64, _f32, _i32, _vp]),
     "fab_bias_rope": (_i32, [_vp] * 4 + [_i32] * 4 + [_i64, _i32, _vp]),
     "fab_silu_mul": (_i32, [_vp, _vp, _i32, _i32, _i64, _i64, _i32, _i32, _vp]),
+    "fab_layernorm": (_i32, [_vp] * 8 + [_i64, _i32] + [_i64] * 4 + [_f32, _i32, _i32, _vp]),
+    "fab_layernorm_bwd_workspace": (_i32, [_i64, _i32, ctypes.POINTER(ctypes.c_size_t)]),
+    "fab_layernorm_bwd": (_i32, [_vp] * 10 + [ctypes.c_size_t, _i64, _i32] + [_i64] * 4 + [_i32, _i32, _vp]),
+    "fab_rope_axes": (_i32, [ctypes.POINTER(FabRopeAxesParams), _vp]),
     "fab_flash_attn_config": (_i32, [_i32, _i32, ctypes.POINTER(FabFaConfig)]),
     "fab_kernel_attrs_query": (_i32, [_i32, _i32, _i32, ctypes.POINTER(FabKernelAttrs)]),
     "fab_device_limits_query": (_i32, [_i32, ctypes.POINTER(FabDeviceLimits)]),

@@ -938,8 +938,9 @@ int fab_device_limits_query(int device, fab_device_limits* out) {
 
 int fab_get_device_error(int* code) {
   if (code == nullptr) return kErrInvalidArg;
-  // This unit's status word (attention, decoder ops), then the GEMM unit's;
-  // both are cleared, the first code recorded is reported.
+  // This unit's status word (attention, decoder ops), then the GEMM unit's
+  // and the attention backward's; all are cleared, the first code found is
+  // reported.
   int v = 0;
   if (cudaMemcpyFromSymbol(&v, g_fab_device_error, sizeof(int)) != cudaSuccess) return kErrCuda;
   if (v != 0) {
@@ -947,9 +948,12 @@ int fab_get_device_error(int* code) {
     if (cudaMemcpyToSymbol(g_fab_device_error, &zero, sizeof(int)) != cudaSuccess) return kErrCuda;
   }
   int g = 0;
-  const int rc = gemm_take_device_error(&g);
+  int rc = gemm_take_device_error(&g);
   if (rc) return rc;
-  *code = v != 0 ? v : g;
+  int w = 0;
+  rc = fa_bwd_take_device_error(&w);
+  if (rc) return rc;
+  *code = v != 0 ? v : g != 0 ? g : w;
   return kOk;
 }
 

@@ -92,6 +92,40 @@ struct FaLaunch {
   int total_k;
 };
 
+// What the attention backward kernels read (fa_bwd_kernel.cuh).
+struct FaBwdParams {
+  const void* o;
+  const void* dout;
+  const float* lse;
+  void* dq;
+  void* dk;
+  void* dv;
+  int64_t o_sb, o_sh, o_ss;
+  int64_t g_sb, g_sh, g_ss;  // dout
+  int64_t l_sb, l_sh, l_ss;
+  int64_t dq_sb, dq_sh, dq_ss;
+  int64_t dk_sb, dk_sh, dk_ss;
+  int64_t dv_sb, dv_sh, dv_ss;
+  // Workspace.  Per streamed-tile-sized tile of query rows, [2][rows]:
+  // -lse * log2(e) and -delta; for fp16 each row's scale exponent and each
+  // tile's largest |dout| too.
+  float* stats;
+  float* row_exp;
+  float* tile_max;
+  int stat_tiles;  // tiles of one head (dense: of one batch entry's head)
+  int B, Hq, Hkv, M, N, D;  // M, N: longest lengths of a packed batch
+  int group;
+  float scale;
+  float scale_log2;
+  int causal;
+  int q_tiles, k_tiles;  // 128-row tiles of the longest sequence
+  int num_dkv;           // CTAs below this index form dK and dV, the others dQ
+  const int* cu_q;       // packed batches, as in FaKernelParams
+  const int* cu_k;
+  int total_q;
+  int total_k;
+};
+
 // Plan of a split-KV launch: the tile config it runs and the workspace it needs.
 struct FaSplitPlan {
   int num_splits;
@@ -225,6 +259,8 @@ int gemm_allreduce(const GemmLaunch& L, const GemmArParams& ar, cudaStream_t str
 int gemm_kernel_attrs(int in_dtype, int* regs, int* smem, int* threads);
 // Reads and clears the GEMM translation unit's device status word.
 int gemm_take_device_error(int* code);
+// The same for the attention backward's unit.
+int fa_bwd_take_device_error(int* code);
 
 // Helpers implemented in capi.cu.
 int ensure_smem_attr(const void* kernel, int bytes);

@@ -1,0 +1,223 @@
+// Translation unit of the training operators around the attention: layer
+// norm and multi-axis rotary embedding (train_ops.cuh), with their C entry
+// points.  Their kernels have no device-side waits.
+#include <cmath>
+#include <cstdint>
+
+#include "fa_b200.h"
+#include "fa_internal.h"
+#include "train_ops.cuh"
+
+namespace fab {
+namespace {
+
+bool aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+int elt_bytes(int dtype) { return dtype == kDtypeF32 ? 4 : 2; }
+
+// Lines of partial dw/db sums: a fixed count, so that the order of the sums
+// does not depend on the device.
+constexpr int kMaxPartLines = 592;
+
+int launched() { return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch; }
+
+// Threads of a CTA whose every thread holds nv vectors of v columns.
+int row_threads(int cols, int v, int nv) { return static_cast<int>(ceil_div(ceil_div(cols, v * nv), 32) * 32); }
+
+template <typename T, typename W, int V, int NV, int kMaxThreads>
+int run_fwd(const LayerNormParams& p, cudaStream_t st) {
+  layernorm_fwd_kernel<T, W, V, NV, kMaxThreads><<<static_cast<unsigned>(p.rows), row_threads(p.cols, V, NV), 0, st>>>(p);
+  return launched();
+}
+
+template <typename T, typename W>
+int fwd(const LayerNormParams& p, cudaStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  const bool vec = p.cols % V == 0 && aligned(p.x, 16) && aligned(p.residual, 16) && aligned(p.w, 16) &&
+                   aligned(p.bias, 16) && aligned(p.y, 16) && aligned(p.x_out, 16) && p.ld_x % V == 0 &&
+                   p.ld_y % V == 0 && (p.residual == nullptr || (p.ld_res % V == 0 && p.ld_xo % V == 0));
+  if (vec) {
+    // The fewest vectors per thread that keep the CTA within 256 threads,
+    // else within 1024.
+    if (p.cols <= 256 * V) return run_fwd<T, W, V, 1, 256>(p, st);
+    if (p.cols <= 512 * V) return run_fwd<T, W, V, 2, 256>(p, st);
+    if (p.cols <= 4096 * V) return run_fwd<T, W, V, 4, 1024>(p, st);
+  } else {
+    if (p.cols <= 1024) return run_fwd<T, W, 1, 4, 256>(p, st);
+    if (p.cols <= 16384) return run_fwd<T, W, 1, 16, 1024>(p, st);
+  }
+  layernorm_fwd_long_kernel<T, W><<<static_cast<unsigned>(p.rows), 1024, 0, st>>>(p);
+  return launched();
+}
+
+template <typename T, typename W, int V, int NV, int kMaxThreads>
+int run_bwd(const LayerNormBwdParams& p, int lines, cudaStream_t st) {
+  layernorm_bwd_kernel<T, W, V, NV, kMaxThreads><<<lines, row_threads(p.cols, V, NV), 0, st>>>(p);
+  return launched();
+}
+
+template <typename T, typename W>
+int bwd(const LayerNormBwdParams& p, void* dw, void* db, int lines, cudaStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  const bool vec = p.cols % V == 0 && aligned(p.x, 16) && aligned(p.dy, 16) && aligned(p.w, 16) &&
+                   aligned(p.dres, 16) && aligned(p.dx, 16) && p.ld_x % V == 0 && p.ld_dy % V == 0 && p.ld_dx % V == 0 &&
+                   (p.dres == nullptr || p.ld_dres % V == 0);
+  int rc;
+  if (vec && p.cols <= 256 * V) {
+    rc = run_bwd<T, W, V, 1, 256>(p, lines, st);
+  } else if (vec && p.cols <= 1024 * V) {
+    rc = run_bwd<T, W, V, 2, 512>(p, lines, st);
+  } else if (!vec && p.cols <= 1024) {
+    rc = run_bwd<T, W, 1, 4, 256>(p, lines, st);
+  } else if (!vec && p.cols <= 8192) {
+    rc = run_bwd<T, W, 1, 16, 512>(p, lines, st);
+  } else {
+    layernorm_bwd_long_kernel<T, W><<<static_cast<unsigned>(p.rows), 1024, 0, st>>>(p);
+    if (p.part != nullptr)
+      layernorm_bwd_long_cols_kernel<T>
+          <<<dim3(static_cast<unsigned>(ceil_div(p.cols, 1024)), static_cast<unsigned>(lines)), 1024, 0, st>>>(p);
+    rc = launched();
+  }
+  if (rc || p.part == nullptr) return rc;
+  layernorm_bwd_finish_kernel<W><<<static_cast<unsigned>(ceil_div(2 * int64_t(p.cols), 32)), 256, 0, st>>>(
+      p.part, lines, p.cols, static_cast<W*>(dw), static_cast<W*>(db));
+  return launched();
+}
+
+// The (T, W) pairs: weights in the activations' type or fp32.
+template <typename F>
+int by_types(int dtype, int w_dtype, F f) {
+  if (dtype == kDtypeF32 && w_dtype == kDtypeF32) return f(float{}, float{});
+  if (dtype == kDtypeBF16 && w_dtype == kDtypeBF16) return f(__nv_bfloat16{}, __nv_bfloat16{});
+  if (dtype == kDtypeBF16 && w_dtype == kDtypeF32) return f(__nv_bfloat16{}, float{});
+  if (dtype == kDtypeF16 && w_dtype == kDtypeF16) return f(__half{}, __half{});
+  if (dtype == kDtypeF16 && w_dtype == kDtypeF32) return f(__half{}, float{});
+  return kErrUnsupported;
+}
+
+int bwd_lines(int64_t rows) { return static_cast<int>(rows < kMaxPartLines ? rows : kMaxPartLines); }
+
+template <typename T, int V>
+int run_rope(const RopeParams& p, cudaStream_t st) {
+  const int nvec = p.half / V + (p.head_dim - 2 * p.half) / V;
+  if (nvec > 256) return kErrUnsupported;
+  rope_axes_kernel<T, V><<<dim3(static_cast<unsigned>(p.tokens), 1), 256, 0, st>>>(p);
+  return launched();
+}
+
+template <typename T>
+int rope(const RopeParams& p, cudaStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  auto even = [&](const void* ptr, int64_t a, int64_t b) { return aligned(ptr, 16) && a % V == 0 && b % V == 0; };
+  const bool vec = p.half % V == 0 && p.head_dim % V == 0 && even(p.q, p.q_st, p.q_sh) && even(p.q_out, p.qo_st, p.qo_sh) &&
+                   (p.heads_k == 0 || (even(p.k, p.k_st, p.k_sh) && even(p.k_out, p.ko_st, p.ko_sh)));
+  return vec ? run_rope<T, V>(p, st) : run_rope<T, 1>(p, st);
+}
+
+}  // namespace
+}  // namespace fab
+
+using namespace fab;
+
+extern "C" {
+
+int fab_layernorm(const void* x, const void* residual, const void* w, const void* bias, void* y, void* x_out,
+                  float* mean, float* rstd, int64_t rows, int cols, int64_t ld_x, int64_t ld_res, int64_t ld_y,
+                  int64_t ld_xo, float eps, int dtype, int w_dtype, void* stream) {
+  if (rows < 0 || cols <= 0 || rows > 0x7fffffffLL) return kErrInvalidArg;
+  if (!(eps >= 0.f) || !std::isfinite(eps)) return kErrInvalidArg;
+  if (rows == 0) return kOk;
+  if (!x || !w || !y || (residual != nullptr && x_out == nullptr) || (mean == nullptr) != (rstd == nullptr))
+    return kErrInvalidArg;
+  const uintptr_t e = elt_bytes(dtype), we = elt_bytes(w_dtype);
+  if (!aligned(x, e) || !aligned(residual, e) || !aligned(y, e) || !aligned(x_out, e) || !aligned(w, we) ||
+      !aligned(bias, we) || !aligned(mean, 4) || !aligned(rstd, 4))
+    return kErrInvalidArg;
+  LayerNormParams p{x, residual, w, bias, y, x_out, mean, rstd, ld_x, ld_res, ld_y, ld_xo, rows, cols, eps};
+  auto st = static_cast<cudaStream_t>(stream);
+  return by_types(dtype, w_dtype, [&](auto t, auto wt) { return fwd<decltype(t), decltype(wt)>(p, st); });
+}
+
+int fab_layernorm_bwd_workspace(int64_t rows, int cols, size_t* bytes) {
+  if (bytes == nullptr || rows < 0 || cols <= 0) return kErrInvalidArg;
+  *bytes = size_t(bwd_lines(rows)) * 2 * size_t(cols) * sizeof(float);
+  return kOk;
+}
+
+int fab_layernorm_bwd(const void* dy, const void* x, const void* w, const float* mean, const float* rstd,
+                      const void* dresidual, void* dx, void* dw, void* db, void* workspace, size_t workspace_bytes,
+                      int64_t rows, int cols, int64_t ld_dy, int64_t ld_x, int64_t ld_dres, int64_t ld_dx, int dtype,
+                      int w_dtype, void* stream) {
+  if (rows < 0 || cols <= 0 || rows > 0x7fffffffLL) return kErrInvalidArg;
+  const uintptr_t e = elt_bytes(dtype), we = elt_bytes(w_dtype);
+  if (!aligned(dw, we) || !aligned(db, we)) return kErrInvalidArg;
+  auto st = static_cast<cudaStream_t>(stream);
+  if (rows == 0) {
+    // Sums over no rows.
+    if (dw != nullptr && cudaMemsetAsync(dw, 0, size_t(cols) * we, st) != cudaSuccess) return kErrCuda;
+    if (db != nullptr && cudaMemsetAsync(db, 0, size_t(cols) * we, st) != cudaSuccess) return kErrCuda;
+    return kOk;
+  }
+  if (!dy || !x || !w || !mean || !rstd || !dx) return kErrInvalidArg;
+  if (!aligned(dy, e) || !aligned(x, e) || !aligned(dresidual, e) || !aligned(dx, e) || !aligned(w, we) ||
+      !aligned(mean, 4) || !aligned(rstd, 4))
+    return kErrInvalidArg;
+  const int lines = bwd_lines(rows);
+  const bool sums = dw != nullptr || db != nullptr;
+  if (sums && (workspace == nullptr || !aligned(workspace, 16) ||
+               workspace_bytes < size_t(lines) * 2 * size_t(cols) * sizeof(float)))
+    return kErrWorkspace;
+  LayerNormBwdParams p{dy, x, w, mean, rstd, dresidual, dx, sums ? static_cast<float*>(workspace) : nullptr,
+                       ld_dy, ld_x, ld_dres, ld_dx, rows, cols};
+  return by_types(dtype, w_dtype,
+                  [&](auto t, auto wt) { return bwd<decltype(t), decltype(wt)>(p, dw, db, lines, st); });
+}
+
+int fab_rope_axes(const fab_rope_axes_params* a, void* stream) {
+  if (a == nullptr) return kErrInvalidArg;
+  if (a->tokens < 0 || a->heads_q < 0 || a->heads_k < 0 || a->head_dim <= 0 || a->table_rows < 0) return kErrInvalidArg;
+  if (a->axes < 1 || a->axes > kMaxRopeAxes) return kErrInvalidArg;
+  if (a->dtype != kDtypeF16 && a->dtype != kDtypeBF16 && a->dtype != kDtypeF32) return kErrInvalidArg;
+  RopeParams p{};
+  int64_t half = 0;
+  for (int i = 0; i < a->axes; ++i) {
+    if (a->sections[i] < 0) return kErrInvalidArg;
+    half += a->sections[i];
+    if (2 * half > a->head_dim) return kErrInvalidArg;
+    p.ends[i] = static_cast<int>(half);
+  }
+  if (half == 0) return kErrInvalidArg;
+  if (a->tokens == 0 || a->heads_q + a->heads_k == 0) return kOk;
+  const uintptr_t e = elt_bytes(a->dtype);
+  if (!a->positions || !aligned(a->positions, a->positions_64bit ? 8 : 4)) return kErrInvalidArg;
+  if (a->table_rows > 0 && (!a->cos || !a->sin || !aligned(a->cos, 4) || !aligned(a->sin, 4))) return kErrInvalidArg;
+  if (a->heads_q > 0 && (!a->q || !a->q_out || !aligned(a->q, e) || !aligned(a->q_out, e))) return kErrInvalidArg;
+  if (a->heads_k > 0 && (!a->k || !a->k_out || !aligned(a->k, e) || !aligned(a->k_out, e))) return kErrInvalidArg;
+  p.q = a->q;
+  p.k = a->k;
+  p.q_out = a->q_out;
+  p.k_out = a->k_out;
+  p.pos = a->positions;
+  p.cos = a->cos;
+  p.sin = a->sin;
+  p.q_st = a->q_stride_t, p.q_sh = a->q_stride_h;
+  p.k_st = a->k_stride_t, p.k_sh = a->k_stride_h;
+  p.qo_st = a->q_out_stride_t, p.qo_sh = a->q_out_stride_h;
+  p.ko_st = a->k_out_stride_t, p.ko_sh = a->k_out_stride_h;
+  p.pos_sa = a->positions_stride_axis, p.pos_st = a->positions_stride_t;
+  p.tokens = a->tokens;
+  p.heads_q = a->heads_q;
+  p.heads_k = a->heads_k;
+  p.head_dim = a->head_dim;
+  p.half = static_cast<int>(half);
+  p.axes = a->axes;
+  p.table_rows = a->table_rows;
+  p.sin_sign = a->inverse ? -1.f : 1.f;
+  p.pos64 = a->positions_64bit ? 1 : 0;
+  auto st = static_cast<cudaStream_t>(stream);
+  if (a->dtype == kDtypeBF16) return rope<__nv_bfloat16>(p, st);
+  if (a->dtype == kDtypeF16) return rope<__half>(p, st);
+  return rope<float>(p, st);
+}
+
+}  // extern "C"

@@ -514,6 +514,168 @@ def attention_forward_varlen(
     return (o, lse) if return_lse else o
 
 
+def _conform_operand(t: torch.Tensor) -> torch.Tensor:
+    """`_conform`, and a copy of broadcast (stride 0) dims, which a tensor map cannot describe."""
+    if any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+        t = t.contiguous()
+    return _conform(t)
+
+
+def _launch_attention_backward(what, dout, q, k, v, out, lse, causal, sm_scale, workspace, cu_q=None, cu_k=None,
+                               max_q=0, max_k=0):
+    """Validate, conform and launch one attention backward; all tensors as [B, H, S, D] views (B = 1 when packed)."""
+    named = (("dout", dout), ("q", q), ("k", k), ("v", v), ("out", out), ("lse", lse))
+    for name, t in named:
+        _require_cuda_tensor(name, t)
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"{what}: gradients are computed in float16 or bfloat16, got {q.dtype}")
+    if any(t.dtype != q.dtype for t in (dout, k, v, out)):
+        raise ValueError(f"{what}: dout, q, k, v and out must share one dtype")
+    if any(t.device != q.device for _, t in named):
+        raise ValueError(f"{what}: all tensors must be on one device")
+    B, Hq, M, D = q.shape
+    Bk, Hkv, N, Dk = k.shape
+    if v.shape != k.shape or Bk != B or Dk != D or out.shape != q.shape or dout.shape != q.shape:
+        raise ValueError(f"{what}: inconsistent shapes dout={tuple(dout.shape)} q={tuple(q.shape)} "
+                         f"k={tuple(k.shape)} v={tuple(v.shape)} out={tuple(out.shape)}")
+    if Hkv == 0 or Hq == 0 or Hq % Hkv:
+        raise ValueError(f"{what}: query heads ({Hq}) must be a multiple of key/value heads ({Hkv})")
+    if lse.dtype != torch.float32 or tuple(lse.shape) != (B, Hq, M):
+        raise ValueError(f"{what}: lse must be float32, one value per query row and head")
+    if D < 1 or D > 256:
+        raise ValueError(f"{what}: head_dim must be between 1 and 256, got {D}")
+    dq, dk, dv = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
+    if B == 0 or (M == 0 and N == 0):
+        return dq, dk, dv
+    # Head dims off the 16-byte grid are written to padded rows first.
+    padded = D * q.element_size() % 16 != 0
+    outs = tuple(_padded_like(t) if padded else t for t in (dq, dk, dv))
+    ins = tuple(_conform_operand(t) if t.numel() else t for t in (q, k, v, out, dout))
+    p = _native.FabAttentionBwdParams()
+    for name, t in zip(("q", "k", "v", "o", "dout", "lse", "dq", "dk", "dv"), (*ins, lse, *outs)):
+        setattr(p, name, t.data_ptr())
+        for d, s in zip("bhs", t.stride()):
+            setattr(p, f"{name}_stride_{d}", s)
+    p.batch, p.heads_q, p.heads_kv, p.seqlen_q, p.seqlen_k, p.head_dim = B, Hq, Hkv, M, N, D
+    if cu_q is not None:
+        p.cu_seqlens_q, p.cu_seqlens_k = cu_q.data_ptr(), cu_k.data_ptr()
+        p.batch, p.total_q, p.total_k, p.seqlen_q, p.seqlen_k = cu_q.numel() - 1, M, N, int(max_q), int(max_k)
+    p.dtype, p.sm_scale, p.causal = _native.dtype_code(q.dtype), float(sm_scale), 1 if causal else 0
+    need = ctypes.c_size_t(0)
+    with torch.cuda.device(q.device):
+        _native.check(_native.lib.fab_attention_bwd_workspace(ctypes.byref(p), ctypes.byref(need)), what)
+        ws = workspace
+        if need.value and ws is None:
+            ws = torch.empty(need.value, device=q.device, dtype=torch.uint8)
+        if ws is not None:
+            _require_cuda_tensor("workspace", ws)
+            p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel() * ws.element_size()
+        stream = ctypes.c_void_p(_native.current_stream_handle(q.device))
+        _native.check(_native.lib.fab_attention_bwd(ctypes.byref(p), stream), what)
+    if padded:
+        for t, buf in zip((dq, dk, dv), outs):
+            t.copy_(buf)
+    return dq, dk, dv
+
+
+def attention_backward(
+    dout: torch.Tensor,
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    out: torch.Tensor,
+    lse: torch.Tensor,
+    *,
+    causal: bool = False,
+    sm_scale: float | None = None,
+    workspace: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dq, dk, dv) of attention_forward(q, k, v) for the output gradient `dout`.
+
+    `out` and `lse` are what attention_forward(..., return_lse=True) gave for
+    the same q, k, v, causal and sm_scale; the probabilities are recomputed
+    from q, k and lse.  float16 or bfloat16; grouped-query gradients are summed
+    over each group's query heads in fp32 inside the kernel, and the same
+    inputs give the same bits on every call.  `workspace` (CUDA, at least
+    attention_backward_workspace_bytes bytes, 256-byte aligned) must not be
+    used by another call until this one has completed; by default one is
+    allocated.  No counterpart in the reference (forward only).
+    """
+    for name, t in (("dout", dout), ("q", q), ("k", k), ("v", v), ("out", out)):
+        if not isinstance(t, torch.Tensor) or t.ndim != 4:
+            raise ValueError(f"attention_backward expects {name} with shape [batch, heads, seq, head_dim]")
+    if sm_scale is None:
+        sm_scale = q.shape[-1] ** -0.5
+    return _launch_attention_backward("attention_backward", dout, q, k, v, out, lse, causal, sm_scale, workspace)
+
+
+def attention_backward_varlen(
+    dout: torch.Tensor,
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    out: torch.Tensor,
+    lse: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    cu_seqlens_k: torch.Tensor,
+    max_seqlen_q: int,
+    max_seqlen_k: int,
+    *,
+    causal: bool = False,
+    sm_scale: float | None = None,
+    workspace: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """attention_backward for attention_forward_varlen: packed [total, heads, D] tensors, lse [heads, total_q].
+
+    Rows of queries without a key get dq = 0 (their `out` is ignored), keys
+    without a query dk = dv = 0, and rows outside every sequence 0.  No
+    sequence's gradients depend on another sequence's values, infinite or NaN
+    ones included.
+    """
+    what = "attention_backward_varlen"
+    for name, t in (("dout", dout), ("q", q), ("k", k), ("v", v), ("out", out)):
+        if not isinstance(t, torch.Tensor) or t.ndim != 3:
+            raise ValueError(f"{what} expects {name} with shape [total_tokens, heads, head_dim]")
+    for name, t in (("cu_seqlens_q", cu_seqlens_q), ("cu_seqlens_k", cu_seqlens_k)):
+        _require_cuda_tensor(name, t)
+    if cu_seqlens_q.dtype != torch.int32 or cu_seqlens_k.dtype != torch.int32:
+        raise ValueError(f"{what}: cu_seqlens_q / cu_seqlens_k must be int32")
+    if cu_seqlens_q.ndim != 1 or cu_seqlens_q.shape != cu_seqlens_k.shape or cu_seqlens_q.numel() < 1:
+        raise ValueError(f"{what}: cu_seqlens_q and cu_seqlens_k must both have batch + 1 entries")
+    if max_seqlen_q < 0 or max_seqlen_k < 0:
+        raise ValueError(f"{what}: max_seqlen_q and max_seqlen_k must not be negative")
+    if not isinstance(lse, torch.Tensor) or lse.ndim != 2:
+        raise ValueError(f"{what} expects lse with shape [heads, total_q]")
+    if cu_seqlens_q.numel() == 1:
+        return torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)
+    if sm_scale is None:
+        sm_scale = q.shape[-1] ** -0.5
+    dense = (t.unsqueeze(0).transpose(1, 2) for t in (dout, q, k, v, out))
+    grads = _launch_attention_backward(what, *dense, lse.unsqueeze(0), causal, sm_scale, workspace,
+                                       cu_seqlens_q.contiguous(), cu_seqlens_k.contiguous(), max_seqlen_q, max_seqlen_k)
+    return tuple(t.transpose(1, 2).squeeze(0) for t in grads)
+
+
+def attention_backward_workspace_bytes(q_shape, k_shape, dtype, *, packed_batch: int | None = None) -> int:
+    """Workspace bytes attention_backward needs for [B, H, S, D] shapes; with `packed_batch` sequences,
+    attention_backward_varlen for [total, H, D] shapes."""
+    p = _native.FabAttentionBwdParams()
+    if packed_batch is None:
+        p.batch, p.heads_q, p.seqlen_q, p.head_dim = q_shape
+        _, p.heads_kv, p.seqlen_k, _ = k_shape
+    else:
+        p.batch, (p.total_q, p.heads_q, p.head_dim), (p.total_k, p.heads_kv, _) = packed_batch, q_shape, k_shape
+        p.seqlen_q, p.seqlen_k = p.total_q, p.total_k
+        p.cu_seqlens_q = p.cu_seqlens_k = 256
+    for name in ("q", "k", "v", "o", "dout", "lse", "dq", "dk", "dv"):
+        setattr(p, name, 256)  # only shapes and the type are read
+    p.dtype, p.sm_scale = _native.dtype_code(dtype), 1.0
+    need = ctypes.c_size_t(0)
+    _native.check(_native.lib.fab_attention_bwd_workspace(ctypes.byref(p), ctypes.byref(need)),
+                  "attention_backward_workspace_bytes")
+    return need.value
+
+
 def _host_pieces(batch: int, kv_heads: int, chunks: int) -> list[tuple[int, int, int]]:
     """How attention_forward_host cuts a call: (batch entry, first kv head, end kv head) per piece.
 
@@ -630,6 +792,9 @@ __all__ = [
     "attention_forward_splitkv",
     "attention_forward_varlen",
     "attention_forward_host",
+    "attention_backward",
+    "attention_backward_varlen",
+    "attention_backward_workspace_bytes",
     "splitkv_workspace_bytes",
     "_flash_attn_fwd_kernel_basic",
     "_flash_attn_fwd_kernel_optimize_shared_mem",

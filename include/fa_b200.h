@@ -154,6 +154,70 @@ typedef struct fab_attention_varlen_params {
 int fab_attention_fwd_varlen(const fab_attention_varlen_params* params, void* stream);
 
 /*
+ * Attention backward: the gradients of fab_attention_fwd's o (or
+ * fab_attention_fwd_varlen's, when the cu_seqlens are given) with respect to
+ * q, k and v, from the forward's inputs, its o and lse, and dout = dL/do:
+ *   P = exp(sm_scale q k^T - lse), dP = dout v^T, dS = P * (dP - rowsum(dout * o)),
+ *   dq = sm_scale dS k, dk = sm_scale sum dS^T q, dv = sum P^T dout,
+ * the sums over the query heads that share a key/value head.  The
+ * probabilities are recomputed; P and dS are rounded to the input type as
+ * tensor-core operands, all sums are fp32 in a fixed order (the same bits on
+ * every call).  fp16 operands are scaled by powers of two inside, so small
+ * gradients do not underflow.  Masks as in the forward.  Query rows that see no key (lse -inf; their o
+ * is ignored) get dq 0, keys that no query sees dk = dv = 0, and rows of a
+ * packed tensor outside [cu[0], cu[batch]) zero gradients.  No counterpart in
+ * the reference, which has no backward pass.
+ *
+ * f16 or bf16 (FAB_ERR_UNSUPPORTED for f32: the forward's f32 runs as tf32),
+ * head_dim <= 256, any finite sm_scale.  Tensors as in the forward: element
+ * strides, stride 1 along head_dim, 16-byte aligned bases and outer strides;
+ * packed tensors use stride_s / stride_h (stride_b is ignored) and lse
+ * [head, token] through lse_stride_h / lse_stride_s.  seqlen_q / seqlen_k are
+ * the longest lengths of a packed batch.  Gradients may not alias inputs.
+ *
+ * The workspace (fab_attention_bwd_workspace bytes, 256-byte aligned, not
+ * initialised) belongs to the call until it completes on its stream.
+ */
+typedef struct fab_attention_bwd_params {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* o;
+  const void* dout;
+  const float* lse;
+  void* dq;
+  void* dk;
+  void* dv;
+  int64_t q_stride_b, q_stride_h, q_stride_s;
+  int64_t k_stride_b, k_stride_h, k_stride_s;
+  int64_t v_stride_b, v_stride_h, v_stride_s;
+  int64_t o_stride_b, o_stride_h, o_stride_s;
+  int64_t dout_stride_b, dout_stride_h, dout_stride_s;
+  int64_t lse_stride_b, lse_stride_h, lse_stride_s;
+  int64_t dq_stride_b, dq_stride_h, dq_stride_s;
+  int64_t dk_stride_b, dk_stride_h, dk_stride_s;
+  int64_t dv_stride_b, dv_stride_h, dv_stride_s;
+  const int32_t* cu_seqlens_q; /* both NULL for a dense batch */
+  const int32_t* cu_seqlens_k;
+  int batch;
+  int heads_q;
+  int heads_kv;
+  int seqlen_q;
+  int seqlen_k;
+  int total_q; /* packed batches only */
+  int total_k;
+  int head_dim;
+  int dtype;
+  float sm_scale;
+  int causal;
+  void* workspace;
+  size_t workspace_bytes;
+} fab_attention_bwd_params;
+
+int fab_attention_bwd_workspace(const fab_attention_bwd_params* params, size_t* bytes);
+int fab_attention_bwd(const fab_attention_bwd_params* params, void* stream);
+
+/*
  * Split-KV ("flash-decoding") form of fab_attention_fwd for short query blocks
  * against long key ranges, where (batch x heads x query tiles) alone would
  * leave most SMs idle.  No counterpart in the reference: it is the split-KV
@@ -385,6 +449,78 @@ int fab_bias_rope(void* y, const void* bias, const void* cos, const void* sin, i
                   int head_dim, int64_t ld, int dtype, void* stream);
 int fab_silu_mul(const void* gu, void* a, int rows, int m, int64_t ld_gu, int64_t ld_a, int interleave, int dtype,
                  void* stream);
+
+/*
+ * Layer norm over rows of `cols` elements, forward and backward (training
+ * companions of the decoder ops above; no counterpart in the reference).
+ * f16, bf16 or f32 rows; weights and bias in the rows' type or f32; fp32
+ * arithmetic, one rounding per stored value.  Leading dims in elements, any
+ * alignment of whole elements (16-byte aligned rows of whole 16-byte units
+ * are read in 16-byte accesses), any cols >= 1.
+ *
+ * fab_layernorm: y = (x' - mean) * rstd * w + bias with x' = x, or
+ *   round(x + residual) (written to x_out, which may alias x) when residual
+ *   is not NULL, and rstd = 1 / sqrt(var + eps); bias, mean and rstd may be
+ *   NULL (mean and rstd together).
+ * fab_layernorm_bwd: x is x' of the forward, mean / rstd its saved values.
+ *   With g = dy * w and xhat = (x - mean) * rstd:
+ *   dx = rstd * (g - mean(g) - xhat * mean(g * xhat)) + dresidual (may be
+ *   NULL; dx may alias dy or dresidual), dw = sum_rows dy * xhat,
+ *   db = sum_rows dy (either may be NULL).  The column sums are formed in a
+ *   fixed order through the workspace (fab_layernorm_bwd_workspace bytes,
+ *   16-byte aligned, not initialised, the call's own until it completes).
+ */
+int fab_layernorm(const void* x, const void* residual, const void* w, const void* bias, void* y, void* x_out,
+                  float* mean, float* rstd, int64_t rows, int cols, int64_t ld_x, int64_t ld_res, int64_t ld_y,
+                  int64_t ld_xo, float eps, int dtype, int w_dtype, void* stream);
+int fab_layernorm_bwd_workspace(int64_t rows, int cols, size_t* bytes);
+int fab_layernorm_bwd(const void* dy, const void* x, const void* w, const float* mean, const float* rstd,
+                      const void* dresidual, void* dx, void* dw, void* db, void* workspace, size_t workspace_bytes,
+                      int64_t rows, int cols, int64_t ld_dy, int64_t ld_x, int64_t ld_dres, int64_t ld_dx, int dtype,
+                      int w_dtype, void* stream);
+
+/*
+ * Rotate-half rotary embedding with several position axes (time, height,
+ * width, ...), out of place or in place, on the query and key heads of every
+ * token in one launch.  The first 2 * half columns of a head are half pairs
+ * (i, half + i), half = the sum of sections[0 .. axes); the first sections[0]
+ * pairs follow axis 0, the next sections[1] axis 1, and so on.  Pair i of
+ * token t turns by the angle whose cosine and sine are row
+ * positions[axis(i)][t], column i of the f32 tables [table_rows][half]:
+ *   lo' = lo * cos - hi * sin,  hi' = hi * cos + lo * sin
+ * (inverse: by minus that angle, which is also the backward pass).  Later
+ * columns are copied.  fp32 arithmetic, one rounding.  A position outside
+ * [0, table_rows) makes its pairs NaN.  f16, bf16 or f32; strides in
+ * elements, stride 1 along the head; k may have no heads.  No counterpart in
+ * the reference.
+ */
+#define FAB_MAX_ROPE_AXES 4
+typedef struct fab_rope_axes_params {
+  const void* q; /* [tokens, heads_q, head_dim] */
+  const void* k;
+  void* q_out; /* may equal q */
+  void* k_out;
+  const void* positions; /* [axes, tokens], int32 or int64 */
+  const float* cos;
+  const float* sin;
+  int64_t q_stride_t, q_stride_h;
+  int64_t k_stride_t, k_stride_h;
+  int64_t q_out_stride_t, q_out_stride_h;
+  int64_t k_out_stride_t, k_out_stride_h;
+  int64_t positions_stride_axis, positions_stride_t;
+  int tokens;
+  int heads_q;
+  int heads_k;
+  int head_dim;
+  int axes;
+  int sections[FAB_MAX_ROPE_AXES];
+  int table_rows;
+  int positions_64bit;
+  int inverse;
+  int dtype;
+} fab_rope_axes_params;
+
+int fab_rope_axes(const fab_rope_axes_params* params, void* stream);
 
 /*
  * Static sm_100a tile table that replaces the reference tuner's compile-and-rank
