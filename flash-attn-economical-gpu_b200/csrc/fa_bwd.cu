@@ -130,6 +130,13 @@ int launch(const fab_attention_bwd_params* p, FaBwdParams& kp, cudaStream_t stre
   auto kern = fa_bwd_kernel<T, kDP>;
   int rc = ensure_smem_attr(reinterpret_cast<const void*>(kern), C::kSmemBytes);
   if (rc) return rc;
+  // The kernel's register split was sized for this launch allocation; a build
+  // compiled to another one is refused.
+  static const int regs = [&] {
+    cudaFuncAttributes a{};
+    return cudaFuncGetAttributes(&a, reinterpret_cast<const void*>(kern)) == cudaSuccess ? a.numRegs : -1;
+  }();
+  if (regs != C::kLaunchRegs) return regs < 0 ? kErrLaunch : kErrUnsupported;
   const bool packed = kp.cu_q != nullptr;
   const int64_t q_rows = packed ? kp.total_q : kp.M, k_rows = packed ? kp.total_k : kp.N;
   const CUtensorMapDataType dt =

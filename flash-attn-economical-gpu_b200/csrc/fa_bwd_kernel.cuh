@@ -38,6 +38,7 @@
 
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "fa_internal.h"
 #include "ptx.cuh"
@@ -91,11 +92,19 @@ struct BwdCfg {
   static constexpr int kABytes = kAAtomBytes * kAtoms;
   static constexpr int kBAtomBytes = kBS * 128;
   static constexpr int kBBytes = kBAtomBytes * kAtoms;
+  // Statistics of the streamed query tiles: one buffer per resident one.
+  static constexpr int kStatBufs = (kRing + 1) / 2;
+  static constexpr int kStatBytes = 2 * kBS * 4;
   static constexpr int kOutDkv = kDP == 256 ? 128 : kDP;                 // output columns of one dK/dV CTA
   static constexpr int kDSplit = kDP / kOutDkv;
   static constexpr int kNumBars = 2 * kRing + 2 + 4 + 2;
-  static constexpr int kSmemBytes = 1024 + 2 * kABytes + kRing * kBBytes + kNumBars * 8 + 16;
+  static constexpr int kSmemBytes = 1024 + 2 * kABytes + kRing * kBBytes + kStatBufs * kStatBytes + kNumBars * 8 + 16;
   static constexpr int kThreads = 384;
+  // Launched with 168 registers a thread; the load/MMA warpgroup hands some
+  // to the two softmax warpgroups, which hold a 64-column row of P across
+  // the wait for dP.
+  static constexpr int kLaunchRegs = 168, kLoadRegs = 72, kSoftmaxRegs = 216;
+  static_assert(128 * kLoadRegs + 256 * kSoftmaxRegs <= kThreads * kLaunchRegs, "register split");
   static constexpr int kTmemS = 0, kTmemP = kBS, kTmemAcc = 2 * kBS;
   static_assert(2 * kBS + kDP <= 512 && 2 * kBS + 2 * kOutDkv <= 512, "TMEM budget");
   static_assert(kSmemBytes <= 232448, "shared memory budget");
@@ -283,7 +292,8 @@ __device__ __forceinline__ void fa_bwd_body(const FaBwdParams& p, const CUtensor
   uint8_t* sA0 = smem;
   uint8_t* sA1 = sA0 + C::kABytes;
   uint8_t* sB = sA1 + C::kABytes;
-  uint64_t* bar_full = reinterpret_cast<uint64_t*>(sB + kRing * C::kBBytes);
+  float* sStat = reinterpret_cast<float*>(sB + kRing * C::kBBytes);
+  uint64_t* bar_full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(sStat) + C::kStatBufs * C::kStatBytes);
   uint64_t* bar_empty = bar_full + kRing;
   uint64_t* bar_a = bar_empty + kRing;  // [2]
   uint64_t* bar_s = bar_a + 2;          // S(i) complete
@@ -322,6 +332,9 @@ __device__ __forceinline__ void fa_bwd_body(const FaBwdParams& p, const CUtensor
   const uint32_t tmem = *tmem_slot;
   const bool skip = *abort_flag != 0;
 
+  // Each warpgroup re-splits its registers first, whatever it does after.
+  if (warp < 4) {
+    setmaxnreg_dec<C::kLoadRegs>();
   if (warp == 0 && !skip && nt > 0) {
     // ------------------------------------------------------------ producer
     // The whole warp runs this; lane 0 issues the copies.
@@ -352,7 +365,13 @@ __device__ __forceinline__ void fa_bwd_body(const FaBwdParams& p, const CUtensor
       const bool fix = packed && rows_left < kBS && (kDkv || !second);
       uint64_t* bar = fix ? bar_fix : bar_full + s;
       if (lane == 0) {
-        mbar_arrive_expect_tx(bar, C::kBBytes);
+        // A query tile brings its rows' statistics along (same barrier; its
+        // buffer is free when its slot is: both were last used for dK).
+        const bool stat = kDkv && !second;
+        mbar_arrive_expect_tx(bar, C::kBBytes + (stat ? C::kStatBytes : 0));
+        if (stat)
+          bulk_load_g2s(sStat + (t / 2) % C::kStatBufs * (2 * kBS),
+                        p.stats + (bwd_stat_tile0(p, b, h_stream0 + g, q_row0, kBS) + ti) * (2 * kBS), C::kStatBytes, bar);
         uint8_t* dst = sB + s * C::kBBytes;
         const CUtensorMap* map = second ? b1 : b0;
         for (int a = 0; a < C::kAtoms; ++a)
@@ -477,7 +496,10 @@ __device__ __forceinline__ void fa_bwd_body(const FaBwdParams& p, const CUtensor
     commit(bar_done);
     volatile int no_abort = 0;
     mbar_wait_warp(bar_done, 0, &no_abort, kDevTimeoutTeardown);
-  } else if (warp >= 4 && !skip) {
+  }
+  } else {
+    setmaxnreg_inc<C::kSoftmaxRegs>();
+  if (!skip) {
     // ------------------------------------------------------------- softmax
     const int half = (warp - 4) >> 2;
     const int wq = warp & 3;
@@ -511,38 +533,29 @@ __device__ __forceinline__ void fa_bwd_body(const FaBwdParams& p, const CUtensor
       cta_scale = exp2f(-e - BwdElem<T>::kPExp);
       unscale = exp2f(e);
     }
-    bool ok = true;
-    int g = 0, ti = first;
-    for (int i = 0; i < nt; ++i) {
-      // Streamed rows of this tile: query positions (dK/dV) or key positions.
-      const int pos0 = ti * kBS + half * kCols;
-      const float* st = nullptr;
-      if constexpr (kDkv)
-        st = p.stats + (bwd_stat_tile0(p, b, h_stream0 + g, q_row0, kBS) + ti) * (2 * kBS) + half * kCols;
-      bool need_mask;
-      if constexpr (kDkv)
-        need_mask = p.causal && pos0 < row0 + 127;
-      else
-        need_mask = pos0 + kCols > N || (p.causal && pos0 + kCols - 1 > row0);
-      // Valid columns [lo, hi) of this lane.
-      int lo = 0, hi = kCols;
-      if (need_mask) {
-        if constexpr (kDkv) {
-          lo = my - pos0;
-        } else {
-          hi = (p.causal ? min(N, my + 1) : N) - pos0;
-        }
+    // One streamed tile.  `masked`: some pair of this warpgroup's columns is
+    // not visible; `pos0` is the position of its first column.
+    auto step = [&](auto masked, int i, int pos0) -> bool {
+      constexpr bool kMasked = decltype(masked)::value;
+      [[maybe_unused]] const float* st = sStat + i % C::kStatBufs * (2 * kBS) + half * kCols;
+      // Visible columns [lo, hi) of this lane.
+      const int lo = kMasked && kDkv ? my - pos0 : 0;
+      const int hi = kMasked && !kDkv ? (p.causal ? min(N, my + 1) : N) - pos0 : kCols;
+      if constexpr (kDkv) {
+        // The statistics land with the query tile; S(i) implies it, but only
+        // this wait orders the copy before this thread's reads.
+        if (!mbar_wait_warp(bar_full + (2 * i) % kRing, ((2 * i) / kRing) & 1, abort_flag, kDevTimeoutKV)) return false;
       }
-      if (!(ok = mbar_wait_warp(bar_s, i & 1, abort_flag, kDevTimeoutS))) break;
+      if (!mbar_wait_warp(bar_s, i & 1, abort_flag, kDevTimeoutS)) return false;
       tc_fence_after();
       float pr[kCols];
+      {
+        uint32_t rr[kCols / 32][32];
 #pragma unroll
-      for (int cc = 0; cc < kCols / 32; ++cc) {
-        uint32_t rr[32];
-        tmem_ld32(tS + cc * 32, rr);
+        for (int cc = 0; cc < kCols / 32; ++cc) tmem_ld32(tS + cc * 32, rr[cc]);
         tmem_wait_ld();
 #pragma unroll
-        for (int e = 0; e < 32; ++e) pr[cc * 32 + e] = __uint_as_float(rr[e]);
+        for (int x = 0; x < kCols; ++x) pr[x] = __uint_as_float(rr[x / 32][x % 32]);
       }
       if constexpr (!kDkv) {
         tc_fence_before();
@@ -551,20 +564,27 @@ __device__ __forceinline__ void fa_bwd_body(const FaBwdParams& p, const CUtensor
       }
 #pragma unroll
       for (int cc = 0; cc < kCols / 32; ++cc) {
-        uint32_t pk[16];
+        [[maybe_unused]] uint32_t pk[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int x = cc * 32 + 2 * e;
-          float2 nl = make_float2(row_nl, row_nl);
-          if constexpr (kDkv) nl = __ldg(reinterpret_cast<const float2*>(st + x));
-          const float2 a = __ffma2_rn(make_float2(pr[x], pr[x + 1]), c2, nl);
+        for (int e = 0; e < 32; e += 4) {
+          const int x = cc * 32 + e;
+          float4 nl = make_float4(row_nl, row_nl, row_nl, row_nl);
+          if constexpr (kDkv) nl = *reinterpret_cast<const float4*>(st + x);
+          const float2 a = __ffma2_rn(make_float2(pr[x], pr[x + 1]), c2, make_float2(nl.x, nl.y));
+          const float2 d = __ffma2_rn(make_float2(pr[x + 2], pr[x + 3]), c2, make_float2(nl.z, nl.w));
           pr[x] = ex2_approx(a.x);
           pr[x + 1] = ex2_approx(a.y);
-          if (need_mask) {
-            if (x < lo || x >= hi) pr[x] = 0.f;
-            if (x + 1 < lo || x + 1 >= hi) pr[x + 1] = 0.f;
+          pr[x + 2] = ex2_approx(d.x);
+          pr[x + 3] = ex2_approx(d.y);
+          if constexpr (kMasked) {
+#pragma unroll
+            for (int y = x; y < x + 4; ++y)
+              if (y < lo || y >= hi) pr[y] = 0.f;
           }
-          pk[e] = BwdElem<T>::pack2(pr[x], pr[x + 1]);
+          if constexpr (kDkv) {
+            pk[e / 2] = BwdElem<T>::pack2(pr[x], pr[x + 1]);
+            pk[e / 2 + 1] = BwdElem<T>::pack2(pr[x + 2], pr[x + 3]);
+          }
         }
         if constexpr (kDkv) tmem_st16(tS + cc * 16, pk);
       }
@@ -574,45 +594,60 @@ __device__ __forceinline__ void fa_bwd_body(const FaBwdParams& p, const CUtensor
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_p);
       }
-      if (!(ok = mbar_wait_warp(bar_dp, i & 1, abort_flag, kDevTimeoutS))) break;
+      if (!mbar_wait_warp(bar_dp, i & 1, abort_flag, kDevTimeoutS)) return false;
       tc_fence_after();
-      uint32_t ds[kCols / 2];
+      uint32_t rr[kCols / 32][32];
+#pragma unroll
+      for (int cc = 0; cc < kCols / 32; ++cc) tmem_ld32(tP + cc * 32, rr[cc]);
+      tmem_wait_ld();
 #pragma unroll
       for (int cc = 0; cc < kCols / 32; ++cc) {
-        uint32_t rr[32];
-        tmem_ld32(tP + cc * 32, rr);
-        tmem_wait_ld();
+        [[maybe_unused]] uint32_t pk[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int x = cc * 32 + 2 * e;
-          float2 nd = make_float2(row_nd, row_nd);
-          if constexpr (kDkv) nd = __ldg(reinterpret_cast<const float2*>(st + kBS + x));
-          float2 d = __fadd2_rn(make_float2(__uint_as_float(rr[2 * e]), __uint_as_float(rr[2 * e + 1])), nd);
-          d = __fmul2_rn(make_float2(pr[x], pr[x + 1]), d);
-          if constexpr (kDkv && BwdElem<T>::kScaled) d = __fmul2_rn(d, make_float2(cta_scale, cta_scale));
-          if (need_mask) {
-            // P is 0 there, but dP may be infinite or NaN.
-            if (x < lo || x >= hi) d.x = 0.f;
-            if (x + 1 < lo || x + 1 >= hi) d.y = 0.f;
+        for (int e = 0; e < 32; e += 4) {
+          const int x = cc * 32 + e;
+          float4 nd = make_float4(row_nd, row_nd, row_nd, row_nd);
+          if constexpr (kDkv) nd = *reinterpret_cast<const float4*>(st + kBS + x);
+          float2 d0 = __fadd2_rn(make_float2(__uint_as_float(rr[cc][e]), __uint_as_float(rr[cc][e + 1])),
+                                 make_float2(nd.x, nd.y));
+          float2 d1 = __fadd2_rn(make_float2(__uint_as_float(rr[cc][e + 2]), __uint_as_float(rr[cc][e + 3])),
+                                 make_float2(nd.z, nd.w));
+          d0 = __fmul2_rn(make_float2(pr[x], pr[x + 1]), d0);
+          d1 = __fmul2_rn(make_float2(pr[x + 2], pr[x + 3]), d1);
+          if constexpr (kDkv && BwdElem<T>::kScaled) {
+            d0 = __fmul2_rn(d0, make_float2(cta_scale, cta_scale));
+            d1 = __fmul2_rn(d1, make_float2(cta_scale, cta_scale));
           }
-          ds[cc * 16 + e] = BwdElem<T>::pack2(d.x, d.y);
+          if constexpr (kMasked) {
+            // P is 0 there, but dP may be infinite or NaN.
+            if (x < lo || x >= hi) d0.x = 0.f;
+            if (x + 1 < lo || x + 1 >= hi) d0.y = 0.f;
+            if (x + 2 < lo || x + 2 >= hi) d1.x = 0.f;
+            if (x + 3 < lo || x + 3 >= hi) d1.y = 0.f;
+          }
+          pk[e / 2] = BwdElem<T>::pack2(d0.x, d0.y);
+          pk[e / 2 + 1] = BwdElem<T>::pack2(d1.x, d1.y);
         }
-      }
-#pragma unroll
-      for (int cc = 0; cc < kCols / 32; ++cc) {
-        uint32_t pk[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) pk[e] = ds[cc * 16 + e];
         tmem_st16(tP + cc * 16, pk);
       }
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_ds);
-      if (++ti == last) {
-        ti = first;
-        ++g;
-      }
+      return true;
+    };
+    bool ok = true;
+    int ti = first;
+    for (int i = 0; ok && i < nt; ++i) {
+      // Streamed rows of this tile: query positions (dK/dV) or key positions.
+      const int pos0 = ti * kBS + half * kCols;
+      bool need_mask;
+      if constexpr (kDkv)
+        need_mask = p.causal && pos0 < row0 + 127;
+      else
+        need_mask = pos0 + kCols > N || (p.causal && pos0 + kCols - 1 > row0);
+      ok = need_mask ? step(std::true_type{}, i, pos0) : step(std::false_type{}, i, pos0);
+      if (++ti == last) ti = first;
     }
 
     // ------------------------------------------------------------ epilogue
@@ -659,6 +694,7 @@ __device__ __forceinline__ void fa_bwd_body(const FaBwdParams& p, const CUtensor
         if (row_ok && left > 0) bwd_store32<T>(out + col0 + cc * 32, v, left);
       }
     }
+  }
   }
 
   tc_fence_before();
