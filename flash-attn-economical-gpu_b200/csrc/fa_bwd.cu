@@ -4,6 +4,7 @@
 // unit it has its own copy of the device status word.
 #include <cudaTypedefs.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 
@@ -32,28 +33,80 @@ int stat_rows(int D) { return D <= 128 ? 128 : 64; }  // BwdCfg::kBS
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 size_t round256(size_t x) { return (x + 255) / 256 * 256; }
 
-struct BwdWorkspace {
-  int64_t tiles_per_head;
-  size_t row_exp, tile_max, bytes;  // byte offsets behind the statistics
+// A slice no shorter than this is worth its own read-out (see choose_slices).
+constexpr int64_t kMinSliceTiles = 4;
+constexpr int kSms = 148;  // plans depend on sizes only, so that results do not depend on the device at hand
+
+// What a call launches and how its workspace is laid out (byte offsets).
+struct BwdPlan {
+  int bs;  // rows of a streamed tile
+  int q_tiles, k_tiles;
+  int64_t stat_tiles;
+  int dkv_slice_len, dkv_slices, dq_slice_len, dq_slices;
+  int64_t part_k_tiles, part_q_tiles;
+  size_t row_exp, tile_max, dkv_part, dq_part, bytes;
 };
 
-BwdWorkspace workspace_plan(const fab_attention_bwd_params* p) {
-  BwdWorkspace w{};
-  const int bs = stat_rows(p->head_dim);
-  int64_t tiles;
-  if (p->cu_seqlens_q != nullptr) {
-    w.tiles_per_head = p->total_q / bs + int64_t(p->batch) + 1;
-    tiles = w.tiles_per_head * p->heads_q;
-  } else {
-    w.tiles_per_head = ceil_div(p->seqlen_q, bs);
-    tiles = w.tiles_per_head * p->heads_q * p->batch;
+// Streamed tiles a tile works through, summed over the tiles of one head (of
+// the longest sequence).
+int64_t streamed_tiles(int64_t tiles, int64_t other_rows, int bs, bool causal, bool dkv) {
+  const int64_t all = ceil_div(other_rows, bs);
+  if (!causal) return tiles * all;
+  int64_t sum = 0;
+  for (int64_t t = 0; t < tiles; ++t) {
+    const int64_t n = dkv ? all - t * 128 / bs : ceil_div(std::min(other_rows, (t + 1) * 128), bs);
+    sum += n > 0 ? n : 0;
   }
-  w.row_exp = round256(size_t(tiles) * 2 * bs * sizeof(float));
-  w.tile_max = w.bytes = w.row_exp;
-  if (p->dtype == kDtypeF16) {
-    w.tile_max = w.row_exp + round256(size_t(tiles) * bs * sizeof(float));
-    w.bytes = w.tile_max + round256(size_t(tiles) * sizeof(float));
-  }
+  return sum;
+}
+
+// Slices of the longest tile's `longest` streamed tiles when an SM's share of
+// the whole work is `share` of them.  Measured on B200: FILL IN.
+void choose_slices(int64_t longest, double share, int* len, int* slices) {
+  const int64_t want = std::max<int64_t>(kMinSliceTiles, static_cast<int64_t>(share / 2 + 0.5));
+  *len = static_cast<int>(std::min<int64_t>(longest < 1 ? 1 : longest, want));
+  *slices = 1;
+  if (longest * 2 >= want * 3) *slices = static_cast<int>(std::min<int64_t>(ceil_div(longest, want), 1 << 15));
+  if (*slices == 1) *len = 0x7fffffff;
+}
+
+BwdPlan make_plan(const fab_attention_bwd_params* p) {
+  BwdPlan w{};
+  const bool packed = p->cu_seqlens_q != nullptr;
+  const int bs = w.bs = stat_rows(p->head_dim);
+  const int dsplit = p->head_dim > 128 ? 2 : 1;
+  const int group = p->heads_q / p->heads_kv;
+  const int64_t M = packed ? std::min(p->seqlen_q, p->total_q) : p->seqlen_q;
+  const int64_t N = packed ? std::min(p->seqlen_k, p->total_k) : p->seqlen_k;
+  w.q_tiles = static_cast<int>(ceil_div(M, 128));
+  w.k_tiles = static_cast<int>(ceil_div(N, 128));
+  // Tiles of one head in the numbering of the statistics and partial sums.
+  w.stat_tiles = packed ? p->total_q / bs + int64_t(p->batch) + 1 : ceil_div(M, bs);
+  w.part_q_tiles = packed ? p->total_q / 128 + int64_t(p->batch) + 1 : w.q_tiles;
+  w.part_k_tiles = packed ? p->total_k / 128 + int64_t(p->batch) + 1 : w.k_tiles;
+  const int64_t per_q = int64_t(p->heads_q) * (packed ? 1 : p->batch), per_kv = int64_t(p->heads_kv) * (packed ? 1 : p->batch);
+  // The work in products of 128 x bs x 128: a streamed tile costs a dK/dV item
+  // four (S, dP, dV, dK) and a dQ item three.  A packed batch's lengths are
+  // not known here; its tiles are taken to be as long as the longest.
+  const bool causal = p->causal != 0;
+  double dkv = 0, dq = 0;
+  if (w.k_tiles > 0) dkv = double(streamed_tiles(w.k_tiles, M, bs, causal, true)) / w.k_tiles * group * dsplit * per_kv * w.part_k_tiles;
+  if (w.q_tiles > 0) dq = double(streamed_tiles(w.q_tiles, N, bs, causal, false)) / w.q_tiles * per_q * w.part_q_tiles;
+  const double share = (4 * dkv + 3 * dq) / kSms;
+  choose_slices(ceil_div(M, bs) * group, share / 4, &w.dkv_slice_len, &w.dkv_slices);
+  choose_slices(ceil_div(N, bs), share / 3, &w.dq_slice_len, &w.dq_slices);
+  const int64_t tiles = w.stat_tiles * per_q;
+  size_t at = round256(size_t(tiles) * 2 * bs * sizeof(float));
+  w.row_exp = at;
+  if (p->dtype == kDtypeF16) at += round256(size_t(tiles) * bs * sizeof(float));
+  w.tile_max = at;
+  if (p->dtype == kDtypeF16) at += round256(size_t(tiles) * sizeof(float));
+  const int dp = padded_head_dim(p->head_dim);
+  w.dkv_part = at;
+  if (w.dkv_slices > 1) at += size_t(w.part_k_tiles) * per_kv * w.dkv_slices * 2 * dp * 128 * sizeof(float);
+  w.dq_part = at;
+  if (w.dq_slices > 1) at += size_t(w.part_q_tiles) * per_q * w.dq_slices * dp * 128 * sizeof(float);
+  w.bytes = at;
   return w;
 }
 
@@ -112,7 +165,8 @@ int validate(const fab_attention_bwd_params* p, bool* empty) {
 
 template <typename T, int kBS>
 void launch_stats(const FaBwdParams& kp, cudaStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(ceil_div(kp.M, kBS)), static_cast<unsigned>(kp.B * kp.Hq));
+  const dim3 grid(static_cast<unsigned>(ceil_div(kp.M, kBS)),
+                  static_cast<unsigned>(kp.B * kp.Hq + (kp.cu_q != nullptr ? 3 : 0)));
   // Lanes per row: eight columns each.
   if constexpr (kBS == 64) {
     fa_bwd_stats_kernel<T, 64, 32><<<grid, 256, 0, stream>>>(kp);
@@ -161,19 +215,44 @@ int launch(const fab_attention_bwd_params* p, FaBwdParams& kp, cudaStream_t stre
       if ((rc = map(&kb, p->k, k_rows, kp.Hkv, p->k_stride_s, p->k_stride_h, p->k_stride_b, C::kBS))) return rc;
       if ((rc = map(&vb, p->v, k_rows, kp.Hkv, p->v_stride_s, p->v_stride_h, p->v_stride_b, C::kBS))) return rc;
     }
-    if (static_cast<int64_t>(kp.B) * kp.Hq > 65535) return kErrUnsupported;
-    if (kp.M > 0) launch_stats<T, C::kBS>(kp, stream);
+    if (static_cast<int64_t>(kp.B) * kp.Hq > 65000) return kErrUnsupported;
   } else {
-    // Nothing attends to anything: the CTAs write zeros and read no map.
+    // Nothing attends to anything: the items write zeros and read no map.
     qa = ga = ka = va = qb = gb = kb = vb = CUtensorMap{};
   }
-  if (packed) fa_bwd_zero_rest_kernel<T><<<dim3(8, 3), 256, 0, stream>>>(kp);
-  const int64_t dkv = static_cast<int64_t>(kp.B) * kp.Hkv * kp.k_tiles * C::kDSplit;
-  const int64_t grid = dkv + static_cast<int64_t>(kp.B) * kp.Hq * kp.q_tiles;
+  const int64_t dkv_tiles = static_cast<int64_t>(kp.B) * kp.Hkv * kp.k_tiles * C::kDSplit;
+  const int64_t dq_tiles = static_cast<int64_t>(kp.B) * kp.Hq * kp.q_tiles;
+  const int64_t dkv = dkv_tiles * kp.dkv_slices, grid = dkv + dq_tiles * kp.dq_slices;
   if (grid > 0x7fffffffLL) return kErrUnsupported;
   kp.num_dkv = static_cast<int>(dkv);
-  if (grid > 0)
-    kern<<<static_cast<unsigned>(grid), C::kThreads, C::kSmemBytes, stream>>>(kp, ka, va, qb, gb, qa, ga, kb, vb);
+  const bool stats = q_rows > 0 && k_rows > 0 && kp.M > 0;
+  if (stats)
+    launch_stats<T, C::kBS>(kp, stream);
+  else if (packed)
+    fa_bwd_zero_rest_kernel<T><<<dim3(8, 3), 256, 0, stream>>>(kp);
+  if (grid > 0) {
+    // Set up while the statistics kernel still runs.
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(grid));
+    cfg.blockDim = dim3(C::kThreads);
+    cfg.dynamicSmemBytes = C::kSmemBytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = stats ? 1 : 0;
+    if (cudaLaunchKernelEx(&cfg, kern, kp, ka, va, qb, gb, qa, ga, kb, vb) != cudaSuccess) {
+      cudaGetLastError();
+      return kErrLaunch;
+    }
+    if (kp.dkv_slices > 1)
+      fa_bwd_join_kernel<T, kDP, true>
+          <<<dim3(static_cast<unsigned>(dkv_tiles), BwdOut<T, kDP, true>::kCols / 32), 256, 0, stream>>>(kp);
+    if (kp.dq_slices > 1)
+      fa_bwd_join_kernel<T, kDP, false>
+          <<<dim3(static_cast<unsigned>(dq_tiles), BwdOut<T, kDP, false>::kCols / 32), 256, 0, stream>>>(kp);
+  }
   return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
 }
 
@@ -202,7 +281,7 @@ int fab_attention_bwd_workspace(const fab_attention_bwd_params* p, size_t* bytes
   bool empty = false;
   const int rc = validate(p, &empty);
   if (rc || empty) return rc;
-  *bytes = workspace_plan(p).bytes;
+  *bytes = make_plan(p).bytes;
   return kOk;
 }
 
@@ -210,11 +289,11 @@ int fab_attention_bwd(const fab_attention_bwd_params* p, void* stream) {
   bool empty = false;
   const int rc = validate(p, &empty);
   if (rc || empty) return rc;
-  const BwdWorkspace w = workspace_plan(p);
+  const BwdPlan w = make_plan(p);
   if (w.bytes > 0 && (p->workspace == nullptr || (reinterpret_cast<uintptr_t>(p->workspace) & 255u) != 0 ||
                       p->workspace_bytes < w.bytes))
     return kErrWorkspace;
-  if (w.tiles_per_head > 0x7fffffffLL) return kErrUnsupported;
+  if (w.stat_tiles > 0x7fffffffLL) return kErrUnsupported;
   uint8_t* ws = static_cast<uint8_t*>(p->workspace);
   FaBwdParams kp{};
   kp.o = p->o;
@@ -244,7 +323,7 @@ int fab_attention_bwd(const fab_attention_bwd_params* p, void* stream) {
   kp.stats = reinterpret_cast<float*>(ws);
   kp.row_exp = reinterpret_cast<float*>(ws + w.row_exp);
   kp.tile_max = reinterpret_cast<float*>(ws + w.tile_max);
-  kp.stat_tiles = static_cast<int>(w.tiles_per_head);
+  kp.stat_tiles = static_cast<int>(w.stat_tiles);
   kp.B = p->batch;
   kp.Hq = p->heads_q;
   kp.Hkv = p->heads_kv;
@@ -263,8 +342,16 @@ int fab_attention_bwd(const fab_attention_bwd_params* p, void* stream) {
     kp.M = kp.M < kp.total_q ? kp.M : kp.total_q;
     kp.N = kp.N < kp.total_k ? kp.N : kp.total_k;
   }
-  kp.q_tiles = static_cast<int>(ceil_div(kp.M, 128));
-  kp.k_tiles = static_cast<int>(ceil_div(kp.N, 128));
+  kp.q_tiles = w.q_tiles;
+  kp.k_tiles = w.k_tiles;
+  kp.dkv_slice_len = w.dkv_slice_len;
+  kp.dkv_slices = w.dkv_slices;
+  kp.dq_slice_len = w.dq_slice_len;
+  kp.dq_slices = w.dq_slices;
+  kp.part_k_tiles = static_cast<int>(w.part_k_tiles);
+  kp.part_q_tiles = static_cast<int>(w.part_q_tiles);
+  kp.dkv_part = reinterpret_cast<float*>(ws + w.dkv_part);
+  kp.dq_part = reinterpret_cast<float*>(ws + w.dq_part);
   auto st = static_cast<cudaStream_t>(stream);
   return p->dtype == kDtypeBF16 ? launch_dim<__nv_bfloat16>(p, kp, st) : launch_dim<__half>(p, kp, st);
 }

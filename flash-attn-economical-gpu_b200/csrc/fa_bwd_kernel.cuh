@@ -6,27 +6,28 @@
 // (sum_g over the query heads that share a key/value head).  P is recomputed
 // from Q, K and LSE instead of being stored.
 //
-// Two launches.  fa_bwd_stats_kernel (memory-bound) reads O and dO once and
+// fa_bwd_stats_kernel (memory-bound) reads O and dO once and
 // leaves -lse*log2(e) and -delta per query row.  fa_bwd_kernel then runs two
-// kinds of CTAs, both one 128-row stationary tile against a stream of tiles:
-//   * dK/dV CTAs (blockIdx.x < num_dkv): K and V tiles stationary, every
+// kinds of work items, both one 128-row stationary tile against a stream of tiles:
+//   * dK/dV items: K and V tiles stationary, every
 //     (query head of the group, query tile) streamed.  The products are taken
 //     transposed, S^T = K Q^T and dP^T = V dO^T, so that P^T and dS^T come out
 //     with keys in the TMEM lanes and are, converted in place, the A operands
 //     (from TMEM) of dV += P^T dO and dK += dS^T Q: neither goes through
 //     shared memory.
-//   * dQ CTAs: Q and dO tiles stationary, K and V tiles streamed,
+//   * dQ items: Q and dO tiles stationary, K and V tiles streamed,
 //     S = Q K^T, dP = dO V^T, dQ += dS K.
 // S and dP are formed twice (7 products instead of 5), and in return every
 // output element is summed in one accumulator in a fixed order: no fp32 dQ
 // traffic through L2, no atomics, the same bits from call to call, and shared
 // heads need no second reduction.
 //
-// Warp 0 loads (TMA), warp 1 issues tcgen05.mma, warps 4-11 are two softmax
-// warpgroups: each covers the 128 lanes and one half of the streamed tile's
-// columns.  Per streamed tile i the issue order is
+// A CTA stays on its SM and takes item after item (a tile, or a slice of one
+// when there are few).  Warp 0 loads (TMA), warp 1 issues tcgen05.mma, warps
+// 4-11 are two softmax warpgroups: each covers the 128 lanes and one half of
+// the streamed tile's columns.  Per streamed tile i the issue order is
 //   [dV(i)] S(i+1)  |  dK/dQ(i) dP(i+1)
-// where the first group waits for P(i) (or, in dQ CTAs, for S(i) to have been
+// where the first group waits for P(i) (or, in dQ items, for S(i) to have been
 // read) and the second for dS(i): while the softmax warps turn S(i+1) into P
 // the tensor core runs dK(i) and dP(i+1), and while they turn dP into dS it
 // runs dV(i) and S(i+1).  P overwrites its own half of S, dS its own half of
@@ -64,7 +65,7 @@ struct BwdElem<__half> {
   // dS = P * (dP - delta) is rounded to fp16 as an operand, and P is about
   // 1/keys: with the small dO of real training it would fall below fp16's
   // normal range although dQ and dK do not.  dS is therefore formed times a
-  // power of two that brings the largest |dO| of its row (dQ) or of the CTA's
+  // power of two that brings the largest |dO| of its row (dQ) or of the item's
   // rows (dK) to [1, 2); the epilogue divides it out.
   static constexpr bool kScaled = true;
   // P itself is an operand of dV: as P * 2^12 it keeps its precision down to
@@ -80,8 +81,8 @@ struct BwdElem<__half> {
 // Tile shapes by padded head dim.  Streamed tiles have 128 rows up to head
 // dim 128; at 256 shared memory holds the two stationary tiles (128 KB) and
 // three 64-row ones.  dK and dV together exceed TMEM at 256, so there a dK/dV
-// CTA forms S and dP over the whole head dim but 128 columns of each output,
-// and two CTAs cover a key tile.
+// item forms S and dP over the whole head dim but 128 columns of each output,
+// and two items cover a key tile.
 template <int kDP_>
 struct BwdCfg {
   static constexpr int kDP = kDP_;
@@ -95,10 +96,12 @@ struct BwdCfg {
   // Statistics of the streamed query tiles: one buffer per resident one.
   static constexpr int kStatBufs = (kRing + 1) / 2;
   static constexpr int kStatBytes = 2 * kBS * 4;
-  static constexpr int kOutDkv = kDP == 256 ? 128 : kDP;                 // output columns of one dK/dV CTA
+  static constexpr int kOutDkv = kDP == 256 ? 128 : kDP;                 // output columns of one dK/dV item
   static constexpr int kDSplit = kDP / kOutDkv;
-  static constexpr int kNumBars = 2 * kRing + 2 + 4 + 2;
-  static constexpr int kSmemBytes = 1024 + 2 * kABytes + kRing * kBBytes + kStatBufs * kStatBytes + kNumBars * 8 + 16;
+  // full/empty per slot; stationary full/empty x 2; S, P, dP, dS; accumulators
+  // final and read; ragged tile; next item full/empty x 2; its request; teardown.
+  static constexpr int kNumBars = 2 * kRing + 4 + 4 + 2 + 1 + 4 + 2;
+  static constexpr int kSmemBytes = 1024 + 2 * kABytes + kRing * kBBytes + kStatBufs * kStatBytes + kNumBars * 8 + 48;
   static constexpr int kThreads = 384;
   // Launched with 168 registers a thread; the load/MMA warpgroup hands some
   // to the two softmax warpgroups, which hold a 64-column row of P across
@@ -131,6 +134,33 @@ __device__ __forceinline__ void bwd_seq(const int* cu, int b, int total, int lon
   len = min(min(max(cu[b + 1], row0), total) - row0, longest);
 }
 
+// Rows of a packed tensor that belong to no sequence (before cu[0], after
+// cu[B]) get zero gradients.  which: 0 dq, 1 dk, 2 dv.
+template <typename T>
+__device__ __forceinline__ void bwd_zero_rest(const FaBwdParams& p, int which) {
+  const bool is_q = which == 0;
+  const int* cu = is_q ? p.cu_q : p.cu_k;
+  const int total = is_q ? p.total_q : p.total_k, heads = is_q ? p.Hq : p.Hkv;
+  const int head = min(max(cu[0], 0), total);
+  const int tail = max(min(max(cu[p.B], 0), total), head);
+  T* out = reinterpret_cast<T*>(is_q ? p.dq : which == 1 ? p.dk : p.dv);
+  const int64_t ss = is_q ? p.dq_ss : which == 1 ? p.dk_ss : p.dv_ss;
+  const int64_t sh = is_q ? p.dq_sh : which == 1 ? p.dk_sh : p.dv_sh;
+  const int rest = head + total - tail;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < static_cast<int64_t>(rest) * heads * p.D; i += gridDim.x * 256ll) {
+    const int d = static_cast<int>(i % p.D);
+    const int h = static_cast<int>(i / p.D % heads);
+    int row = static_cast<int>(i / p.D / heads);
+    if (row >= head) row += tail - head;
+    out[row * ss + h * sh + d] = static_cast<T>(0.f);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) fa_bwd_zero_rest_kernel(const FaBwdParams p) {
+  bwd_zero_rest<T>(p, blockIdx.y);
+}
+
 // Per query row: -lse * log2(e), plus kPExp, (-inf for rows that saw no key and for the
 // padding rows of the last tile, so that P is 0 there) and -delta, as
 // [tile][2][kBS]; for fp16 also the row's scale exponent and the tile's
@@ -138,7 +168,13 @@ __device__ __forceinline__ void bwd_seq(const int* cu, int b, int total, int lon
 // columns each, so a warp reads whole 128-byte lines.
 template <typename T, int kBS, int kLanes>
 __global__ void __launch_bounds__(256) fa_bwd_stats_kernel(const FaBwdParams p) {
+  // The main kernel may be set up meanwhile; it waits before it reads.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int bh = blockIdx.y;
+  if (bh >= p.B * p.Hq) {  // three more rows of CTAs, for packed batches
+    bwd_zero_rest<T>(p, bh - p.B * p.Hq);
+    return;
+  }
   const int b = bh / p.Hq, h = bh % p.Hq;
   int q0, M;
   bwd_seq(p.cu_q, b, p.total_q, p.M, q0, M);
@@ -209,28 +245,6 @@ __global__ void __launch_bounds__(256) fa_bwd_stats_kernel(const FaBwdParams p) 
   }
 }
 
-// Rows of a packed tensor that belong to no sequence (before cu[0], after
-// cu[B]) get zero gradients.  blockIdx.y: dq, dk, dv.
-template <typename T>
-__global__ void __launch_bounds__(256) fa_bwd_zero_rest_kernel(const FaBwdParams p) {
-  const bool is_q = blockIdx.y == 0;
-  const int* cu = is_q ? p.cu_q : p.cu_k;
-  const int total = is_q ? p.total_q : p.total_k, heads = is_q ? p.Hq : p.Hkv;
-  const int head = min(max(cu[0], 0), total);
-  const int tail = max(min(max(cu[p.B], 0), total), head);
-  T* out = reinterpret_cast<T*>(is_q ? p.dq : blockIdx.y == 1 ? p.dk : p.dv);
-  const int64_t ss = is_q ? p.dq_ss : blockIdx.y == 1 ? p.dk_ss : p.dv_ss;
-  const int64_t sh = is_q ? p.dq_sh : blockIdx.y == 1 ? p.dk_sh : p.dv_sh;
-  const int rest = head + total - tail;
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < static_cast<int64_t>(rest) * heads * p.D; i += gridDim.x * 256ll) {
-    const int d = static_cast<int>(i % p.D);
-    const int h = static_cast<int>(i / p.D % heads);
-    int row = static_cast<int>(i / p.D / heads);
-    if (row >= head) row += tail - head;
-    out[row * ss + h * sh + d] = static_cast<T>(0.f);
-  }
-}
-
 // 32 fp32 values as part of an output row (16-byte aligned).
 template <typename T>
 __device__ __forceinline__ void bwd_store32(T* dst, const float (&v)[32], int ncols) {
@@ -249,452 +263,662 @@ __device__ __forceinline__ void bwd_store32(T* dst, const float (&v)[32], int nc
   }
 }
 
-// One CTA's work.  kDkv: a key tile against its query tiles, else a query
-// tile against its key tiles.  a0/a1 are the maps of the stationary operands
-// (K and V, or Q and dO), b0/b1 of the streamed ones (Q and dO, or K and V).
+// A work item: one stationary tile (and, at head dim 256, one half of the
+// output columns) against a slice of its streamed tiles.
+struct BwdItem {
+  int b, h, tile;          // batch entry, head (of the stationary tile), 128-row tile
+  int dcol0;               // first output column
+  int q_row0, k_row0;      // the sequence's first rows in a packed tensor
+  int M, N;                // its lengths
+  int row0;                // first stationary row within the sequence
+  int first, per_head;     // streamed tiles [first, first + per_head) of each head
+  int begin, nt;           // this slice: streamed tiles begin .. begin + nt of all heads'
+  int slice, slices;
+};
+
+// Streamed tiles of a stationary tile are cut into slices when there are too
+// few stationary tiles to fill the GPU; slice s of `slices` takes an even
+// share, and with more than one each leaves fp32 sums that
+// fa_bwd_join_kernel adds in slice order.
+__device__ __forceinline__ void bwd_slices(int total, int slice_len, int max_slices, int& slices, int& share) {
+  slices = min(max_slices, max(1, (total + slice_len - 1) / slice_len));
+  share = (total + slices - 1) / slices;
+}
+
+// False: nothing to do (a tile or slice that this sequence does not have).
+template <int kDP, bool kDkv>
+__device__ __forceinline__ bool bwd_item(const FaBwdParams& p, int index, BwdItem& w) {
+  using C = BwdCfg<kDP>;
+  constexpr int kDSplit = kDkv ? C::kDSplit : 1;
+  const int tiles = kDkv ? p.k_tiles : p.q_tiles;
+  const int heads = kDkv ? p.Hkv : p.Hq;
+  const int max_slices = kDkv ? p.dkv_slices : p.dq_slices;
+  w.slice = index % max_slices;
+  index /= max_slices;
+  w.dcol0 = kDSplit > 1 ? index % kDSplit * C::kOutDkv : 0;
+  index /= kDSplit;
+  // The tile is the fast index, so that CTAs at work together share a head's
+  // operands in L2; longest (causal) first.
+  w.tile = kDkv ? index % tiles : tiles - 1 - index % tiles;
+  w.b = index / tiles / heads;
+  w.h = index / tiles % heads;
+  bwd_seq(p.cu_q, w.b, p.total_q, p.M, w.q_row0, w.M);
+  bwd_seq(p.cu_k, w.b, p.total_k, p.N, w.k_row0, w.N);
+  w.row0 = w.tile * 128;
+  if (w.row0 >= (kDkv ? w.N : w.M)) return false;
+  int last;
+  if constexpr (kDkv) {
+    w.first = p.causal ? w.row0 / C::kBS : 0;  // query m sees key n iff m >= n
+    last = (w.M + C::kBS - 1) / C::kBS;
+  } else {
+    w.first = 0;
+    last = ((p.causal ? min(w.N, w.row0 + 128) : w.N) + C::kBS - 1) / C::kBS;
+  }
+  w.per_head = max(0, last - w.first);
+  const int total = w.per_head * (kDkv ? p.group : 1);
+  int share;
+  bwd_slices(total, kDkv ? p.dkv_slice_len : p.dq_slice_len, max_slices, w.slices, share);
+  if (w.slice >= w.slices) return false;
+  w.begin = w.slice * share;
+  w.nt = max(0, min(share, total - w.begin));
+  return true;
+}
+
+// fp32 sums of a slice: [slot][accumulator][column][row].
+template <int kDP, bool kDkv>
+__device__ __forceinline__ int64_t bwd_part_slot(const FaBwdParams& p, const BwdItem& w) {
+  using C = BwdCfg<kDP>;
+  int64_t tile;
+  if constexpr (kDkv) {
+    tile = p.cu_k != nullptr ? static_cast<int64_t>(w.h) * p.part_k_tiles + w.k_row0 / 128 + w.b + w.tile
+                             : (static_cast<int64_t>(w.b) * p.Hkv + w.h) * p.part_k_tiles + w.tile;
+    return (tile * C::kDSplit + w.dcol0 / C::kOutDkv) * p.dkv_slices + w.slice;
+  } else {
+    tile = p.cu_q != nullptr ? static_cast<int64_t>(w.h) * p.part_q_tiles + w.q_row0 / 128 + w.b + w.tile
+                             : (static_cast<int64_t>(w.b) * p.Hq + w.h) * p.part_q_tiles + w.tile;
+    return tile * p.dq_slices + w.slice;
+  }
+}
+
+// Where thread (half, row r) writes: dK/dV items: warpgroup 0 dK, 1 dV; dQ
+// items: each half of the columns.
 template <typename T, int kDP, bool kDkv>
-__device__ __forceinline__ void fa_bwd_body(const FaBwdParams& p, const CUtensorMap* a0, const CUtensorMap* a1,
-                                            const CUtensorMap* b0, const CUtensorMap* b1, int index,
-                                            uint8_t* smem_raw) {
+struct BwdOut {
+  static constexpr int kOut = kDkv ? BwdCfg<kDP>::kOutDkv : kDP;
+  static constexpr int kCols = kDkv ? kOut : kOut / 2;  // columns of one thread
+  T* row;     // the output row
+  float* part;  // this thread's column 0 of the slice's sums
+  int col0;   // its first column
+  bool row_ok;
+  __device__ __forceinline__ BwdOut(const FaBwdParams& p, const BwdItem& w, int half, int r) {
+    const int my = w.row0 + r;
+    row_ok = my < (kDkv ? w.N : w.M);
+    if constexpr (kDkv) {
+      const bool is_v = half == 1;
+      const int64_t ss = is_v ? p.dv_ss : p.dk_ss, sh = is_v ? p.dv_sh : p.dk_sh, sb = is_v ? p.dv_sb : p.dk_sb;
+      row = reinterpret_cast<T*>(is_v ? p.dv : p.dk) + (p.cu_k ? w.k_row0 * ss : w.b * sb) + w.h * sh + my * ss;
+      col0 = w.dcol0;
+      part = p.dkv_part + (bwd_part_slot<kDP, true>(p, w) * 2 + half) * (kOut * 128) + r;
+    } else {
+      row = reinterpret_cast<T*>(p.dq) + (p.cu_q ? w.q_row0 * p.dq_ss : w.b * p.dq_sb) + w.h * p.dq_sh + my * p.dq_ss;
+      col0 = half * kCols;
+      part = p.dq_part + bwd_part_slot<kDP, false>(p, w) * (kOut * 128) + col0 * 128 + r;
+    }
+  }
+};
+
+// Shared memory, barriers and running counters of a CTA.  Every role keeps
+// its own copy of the counters, advanced alike.
+template <int kDP>
+struct BwdCta {
+  using C = BwdCfg<kDP>;
+  uint8_t *sA0, *sA1, *sB;
+  float* sStat;
+  uint64_t *full, *empty, *a_full, *a_empty, *s, *pr, *dp, *ds, *done, *acc_free, *fix, *sched_full, *sched_empty, *clc, *drained;
+  uint32_t* tmem_slot;
+  volatile int* abort_flag;
+  volatile int* next;  // [2]
+  uint32_t clc_resp;
+  __device__ __forceinline__ explicit BwdCta(uint8_t* smem) {
+    sA0 = smem;
+    sA1 = sA0 + C::kABytes;
+    sB = sA1 + C::kABytes;
+    sStat = reinterpret_cast<float*>(sB + C::kRing * C::kBBytes);
+    full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(sStat) + C::kStatBufs * C::kStatBytes);
+    empty = full + C::kRing;
+    a_full = empty + C::kRing;
+    a_empty = a_full + 2;
+    s = a_empty + 2;    // S(i) complete
+    pr = s + 1;         // P(i) stored (dK/dV), S(i) read (dQ)
+    dp = pr + 1;        // dP(i) complete
+    ds = dp + 1;        // dS(i) stored
+    done = ds + 1;      // accumulators final
+    acc_free = done + 1;  // accumulators read
+    fix = acc_free + 1;   // ragged tile landed, before its rows are cleared
+    sched_full = fix + 1;
+    sched_empty = sched_full + 2;
+    clc = sched_empty + 2;
+    drained = clc + 1;
+    tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
+    abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    next = reinterpret_cast<volatile int*>(tmem_slot + 2);
+    clc_resp = (smem_u32(tmem_slot + 4) + 15u) & ~15u;
+  }
+};
+
+struct BwdCount {
+  int t = 0;      // streamed tiles put into (taken from) the ring
+  int i = 0;      // pairs of them
+  int items = 0;  // items with work
+};
+
+// ---------------------------------------------------------------- producer
+// The whole warp 0 runs this; lane 0 issues the copies.  a0/a1 are the maps
+// of the stationary operands (K and V, or Q and dO), b0/b1 of the streamed
+// ones (Q and dO, or K and V).
+template <typename T, int kDP, bool kDkv>
+__device__ __forceinline__ bool bwd_produce(const FaBwdParams& p, const BwdCta<kDP>& c, const CUtensorMap* a0,
+                                            const CUtensorMap* a1, const CUtensorMap* b0, const CUtensorMap* b1,
+                                            int index, BwdCount& n) {
+  using C = BwdCfg<kDP>;
+  constexpr int kBS = C::kBS, kRing = C::kRing;
+  BwdItem w;
+  if (!bwd_item<kDP, kDkv>(p, index, w) || w.nt == 0) return true;
+  const int lane = threadIdx.x & 31;
+  const bool packed = p.cu_q != nullptr;
+  const int map_b = packed ? 0 : w.b;
+  const int a_row = (kDkv ? w.k_row0 : w.q_row0) + w.row0;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    if (!mbar_wait_warp(c.a_empty + x, (n.items & 1) ^ 1, c.abort_flag, kDevTimeoutEmpty)) return false;
+    if (lane == 0) {
+      mbar_arrive_expect_tx(c.a_full + x, C::kABytes);
+      for (int a = 0; a < C::kAtoms; ++a)
+        tma_load_4d((x ? c.sA1 : c.sA0) + a * C::kAAtomBytes, x ? a1 : a0, c.a_full + x, a * 64, a_row, w.h, map_b);
+    }
+  }
+  // What follows reads the statistics kernel's output.
+  if (n.items == 0) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    fence_proxy_async_global();
+  }
+  ++n.items;
+  const int stat_len = kDkv ? w.M : w.N;  // valid streamed rows of the sequence
+  const int row_base = kDkv ? w.q_row0 : w.k_row0;
+  const int h0 = kDkv ? w.h * p.group : w.h / p.group;
+  int g = w.begin / w.per_head, ti = w.begin % w.per_head;
+  for (int x = 0; x < 2 * w.nt; ++x, ++n.t) {
+    const int slot = n.t % kRing;
+    const bool second = (x & 1) != 0;
+    if (!mbar_wait_warp(c.empty + slot, ((n.t / kRing) & 1) ^ 1, c.abort_flag, kDevTimeoutEmpty)) return false;
+    const int tile = w.first + ti;
+    const int rows_left = stat_len - tile * kBS;
+    // A packed sequence's last tile runs into the next sequence's rows.  Rows
+    // of the summed dimension must be zero there (0 x NaN is NaN), so such a
+    // tile is cleared past the end before it is handed on.  V tiles of dQ
+    // items are exempt: they only feed dP columns that are masked.
+    const bool fix = packed && rows_left < kBS && (kDkv || !second);
+    uint8_t* dst = c.sB + slot * C::kBBytes;
+    if (lane == 0) {
+      // A query tile brings its rows' statistics along (same barrier; its
+      // buffer is free when its slot is: both were last used for dK).
+      uint64_t* bar = fix ? c.fix : c.full + slot;
+      const bool stat = kDkv && !second;
+      mbar_arrive_expect_tx(bar, C::kBBytes + (stat ? C::kStatBytes : 0));
+      if (stat)
+        bulk_load_g2s(c.sStat + (n.t / 2) % C::kStatBufs * (2 * kBS),
+                      p.stats + (bwd_stat_tile0(p, w.b, h0 + g, w.q_row0, kBS) + tile) * (2 * kBS), C::kStatBytes, bar);
+      const CUtensorMap* map = second ? b1 : b0;
+      for (int a = 0; a < C::kAtoms; ++a)
+        tma_load_4d(dst + a * C::kBAtomBytes, map, bar, a * 64, row_base + tile * kBS, h0 + g, map_b);
+    }
+    if (fix) {
+      if (!mbar_wait_warp(c.fix, n.i & 1, c.abort_flag, kDevTimeoutKV)) return false;
+      ++n.i;  // the producer counts cleared tiles here
+      const int chunks = (kBS - rows_left) * 8;  // 16-byte pieces of one atom's rows past the end
+      for (int a = 0; a < C::kAtoms; ++a)
+        for (int k = lane; k < chunks; k += 32)
+          *reinterpret_cast<uint4*>(dst + a * C::kBAtomBytes + rows_left * 128 + k * 16) = make_uint4(0, 0, 0, 0);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(c.full + slot);
+    }
+    if (second && ++ti == w.per_head) {
+      ti = 0;
+      ++g;
+    }
+  }
+  return true;
+}
+
+// -------------------------------------------------------------- MMA issuer
+template <typename T, int kDP, bool kDkv>
+__device__ __forceinline__ bool bwd_issue(const FaBwdParams& p, const BwdCta<kDP>& c, uint32_t tmem, bool leader,
+                                          int index, BwdCount& n) {
   using C = BwdCfg<kDP>;
   constexpr int kBS = C::kBS, kRing = C::kRing;
   constexpr int kOut = kDkv ? C::kOutDkv : kDP;  // columns of each accumulator
-  constexpr int kDSplit = kDkv ? C::kDSplit : 1;
+  BwdItem w;
+  if (!bwd_item<kDP, kDkv>(p, index, w) || w.nt == 0) return true;
+  const int nt = w.nt;
+  constexpr uint32_t kFmt = BwdElem<T>::kFmt;
+  constexpr uint32_t idesc_s = umma_idesc(kFmt, 128, kBS, 0, 0);
+  constexpr uint32_t idesc_o = umma_idesc(kFmt, 128, kOut, 0, 1);
+  constexpr uint32_t kHi = umma_desc_hi(1024, kLayoutSw128);
+  const uint32_t a0_lo = umma_desc_lo(smem_u32(c.sA0), 16);
+  const uint32_t a1_lo = umma_desc_lo(smem_u32(c.sA1), 16);
+  const uint32_t b_lo = umma_desc_lo(smem_u32(c.sB), 16);
+  // The same tiles as MN-major operands, from this item's first output column.
+  const uint32_t bn_lo = umma_desc_lo(smem_u32(c.sB) + (w.dcol0 / 64) * C::kBAtomBytes, C::kBAtomBytes);
+  auto wait = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
+    return mbar_wait_warp(bar, parity, c.abort_flag, code);
+  };
+  // D[128 x kBS] = A (stationary) x B(slot)^T over the head dim.
+  auto issue_s = [&](uint32_t d, uint32_t alo, int s) {
+    uint32_t qa = alo, kb = b_lo + s * (C::kBBytes >> 4);
+    asm volatile("" : "+r"(qa), "+r"(kb));
+#pragma unroll
+    for (int kk = 0; kk < kDP / 16; ++kk) {
+      const int a = kk >> 2;
+      const uint32_t off = (kk & 3) * 32;
+      const uint64_t ad = umma_desc_join(qa + ((a * C::kAAtomBytes + off) >> 4), kHi);
+      const uint64_t bd = umma_desc_join(kb + ((a * C::kBAtomBytes + off) >> 4), kHi);
+      if (leader) mma_ss_f16(d, ad, bd, idesc_s, kk > 0 ? 1u : 0u);
+    }
+  };
+  // D[128 x kOut] += A (TMEM, kBS wide) x B(slot).  Each softmax warpgroup's
+  // half of A starts at its half of the fp32 columns.
+  auto issue_o = [&](uint32_t d, uint32_t a, int s, bool acc) {
+    uint32_t vb = bn_lo + s * (C::kBBytes >> 4);
+    asm volatile("" : "+r"(vb));
+#pragma unroll
+    for (int kk = 0; kk < kBS / 16; ++kk) {
+      constexpr int kHalf = kBS / 32;
+      const uint32_t at = a + (kk / kHalf) * (kBS / 2) + (kk % kHalf) * 8;
+      const uint64_t bd = umma_desc_join(vb + ((kk * 16 * 128) >> 4), kHi);
+      if (leader) mma_ts_f16(d, at, bd, idesc_o, (acc || kk > 0) ? 1u : 0u);
+    }
+  };
+  auto commit = [&](uint64_t* bar) {
+    if (leader) mma_commit(bar);
+  };
+  const uint32_t tS = tmem + C::kTmemS, tP = tmem + C::kTmemP;
+  const uint32_t tAcc0 = tmem + C::kTmemAcc, tAcc1 = tAcc0 + kOut;
+  auto slot = [](int t) { return t % kRing; };
+  auto par = [](int t) { return static_cast<uint32_t>((t / kRing) & 1); };
+  const uint32_t turn = n.items & 1;
+  ++n.items;
 
-  // ---- work item: the tile is the fast index, longest (causal) first
-  const int tiles = kDkv ? p.k_tiles : p.q_tiles;
-  const int heads = kDkv ? p.Hkv : p.Hq;
-  const int dcol0 = kDSplit > 1 ? index % kDSplit * kOut : 0;
-  index /= kDSplit;
-  const int tile = kDkv ? index % tiles : tiles - 1 - index % tiles;
-  const int b = index / tiles / heads, h = index / tiles % heads;
-  int q_row0, k_row0, M, N;
-  bwd_seq(p.cu_q, b, p.total_q, p.M, q_row0, M);
-  bwd_seq(p.cu_k, b, p.total_k, p.N, k_row0, N);
-  const int map_b = p.cu_q != nullptr ? 0 : b;
-  const int row0 = tile * 128;  // first stationary row within the sequence
-  if (row0 >= (kDkv ? N : M)) return;
-  // Streamed tiles [first, first + per_head) of each of `group` heads.
-  int first = 0, last;
-  if constexpr (kDkv) {
-    if (p.causal) first = row0 / kBS;  // query m sees key n iff m >= n
-    last = (M + kBS - 1) / kBS;
-  } else {
-    const int seen = p.causal ? min(N, row0 + 128) : N;
-    last = (seen + kBS - 1) / kBS;
+  // The previous item's last products are queued ahead: S and dP of this one
+  // overwrite buffers whose contents those read, in issue order.
+  if (!wait(c.a_full, turn, kDevTimeoutQ) || !wait(c.full + slot(n.t), par(n.t), kDevTimeoutKV)) return false;
+  tc_fence_after();
+  issue_s(tS, a0_lo, slot(n.t));
+  commit(c.s);
+  if (nt == 1) commit(c.a_empty);
+  if (!wait(c.a_full + 1, turn, kDevTimeoutQ) || !wait(c.full + slot(n.t + 1), par(n.t + 1), kDevTimeoutKV)) return false;
+  tc_fence_after();
+  issue_s(tP, a1_lo, slot(n.t + 1));
+  commit(c.dp);
+  if (nt == 1) commit(c.a_empty + 1);
+  if constexpr (!kDkv) commit(c.empty + slot(n.t + 1));
+  for (int i = 0; i < nt; ++i, ++n.i, n.t += 2) {
+    const int t0 = n.t, t1 = n.t + 1;
+    if (!wait(c.pr, n.i & 1, kDevTimeoutP)) return false;
+    // The first product into the accumulators waits until the previous item's
+    // sums have been read.
+    if (i == 0 && !wait(c.acc_free, turn ^ 1, kDevTimeoutAcc)) return false;
+    tc_fence_after();
+    if constexpr (kDkv) {
+      issue_o(tAcc1, tS, slot(t1), i > 0);
+      commit(c.empty + slot(t1));
+    }
+    if (i + 1 < nt) {
+      if (!wait(c.full + slot(t0 + 2), par(t0 + 2), kDevTimeoutKV)) return false;
+      tc_fence_after();
+      issue_s(tS, a0_lo, slot(t0 + 2));
+      commit(c.s);
+      if (i + 2 == nt) commit(c.a_empty);
+    }
+    if (!wait(c.ds, n.i & 1, kDevTimeoutP)) return false;
+    tc_fence_after();
+    issue_o(tAcc0, tP, slot(t0), i > 0);
+    commit(c.empty + slot(t0));
+    if (i + 1 < nt) {
+      if (!wait(c.full + slot(t1 + 2), par(t1 + 2), kDevTimeoutKV)) return false;
+      tc_fence_after();
+      issue_s(tP, a1_lo, slot(t1 + 2));
+      commit(c.dp);
+      if (i + 2 == nt) commit(c.a_empty + 1);
+      if constexpr (!kDkv) commit(c.empty + slot(t1 + 2));
+    }
   }
-  const int per_head = max(0, last - first);
-  const int nt = per_head * (kDkv ? p.group : 1);
-  const int h_stream0 = kDkv ? h * p.group : h / p.group;
+  commit(c.done);
+  return true;
+}
 
+// ----------------------------------------------------------------- softmax
+template <typename T, int kDP, bool kDkv>
+__device__ __forceinline__ bool bwd_softmax(const FaBwdParams& p, const BwdCta<kDP>& c, uint32_t tmem, int index,
+                                            BwdCount& n) {
+  using C = BwdCfg<kDP>;
+  constexpr int kBS = C::kBS, kRing = C::kRing;
+  using Out = BwdOut<T, kDP, kDkv>;
+  BwdItem w;
+  if (!bwd_item<kDP, kDkv>(p, index, w)) return true;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int half = (warp - 4) >> 2;
+  const int wq = warp & 3;
+  const int r = wq * 32 + lane;  // TMEM lane: stationary row
+  const uint32_t lane_base = static_cast<uint32_t>(wq * 32) << 16;
+  constexpr int kCols = kBS / 2;  // columns of one warpgroup
+  const uint32_t tS = tmem + lane_base + C::kTmemS + half * kCols;
+  const uint32_t tP = tmem + lane_base + C::kTmemP + half * kCols;
+  const int my = w.row0 + r;  // position of this lane's row in the sequence
+  const int M = w.M, N = w.N, row0 = w.row0, nt = w.nt;
+  const float2 c2 = make_float2(p.scale_log2, p.scale_log2);
+  [[maybe_unused]] float row_nl = 0.f, row_nd = 0.f, cta_scale = 1.f;
+  float unscale = 1.f;
+  if constexpr (!kDkv) {
+    if (nt > 0 && my < M) {
+      const int64_t st_tile = bwd_stat_tile0(p, w.b, w.h, w.q_row0, kBS) + my / kBS;
+      row_nl = p.stats[st_tile * (2 * kBS) + my % kBS];
+      row_nd = p.stats[st_tile * (2 * kBS) + kBS + my % kBS];
+      if constexpr (BwdElem<T>::kScaled) {
+        const float e = p.row_exp[st_tile * kBS + my % kBS];
+        row_nl += e - BwdElem<T>::kPExp;  // P, hence dS, times 2^e
+        unscale = exp2f(-e);
+      }
+    }
+  } else if constexpr (BwdElem<T>::kScaled) {
+    // Largest |dO| over every row this item sums.
+    float big = 0.f;
+    for (int x = lane; x < nt; x += 32) {
+      const int j = w.begin + x;
+      big = fmaxf(big, p.tile_max[bwd_stat_tile0(p, w.b, w.h * p.group + j / w.per_head, w.q_row0, kBS) + w.first +
+                                  j % w.per_head]);
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
+    const float e = big > 0.f ? floorf(log2f(big)) : 0.f;
+    cta_scale = exp2f(-e - BwdElem<T>::kPExp);
+    unscale = exp2f(e);
+  }
+
+  // One streamed tile.  `masked`: some pair of this warpgroup's columns is
+  // not visible; `pos0` is the position of its first column.
+  auto step = [&](auto masked, int pos0) -> bool {
+    constexpr bool kMasked = decltype(masked)::value;
+    [[maybe_unused]] const float* st = c.sStat + n.i % C::kStatBufs * (2 * kBS) + half * kCols;
+    // Visible columns [lo, hi) of this lane.
+    const int lo = kMasked && kDkv ? my - pos0 : 0;
+    const int hi = kMasked && !kDkv ? (p.causal ? min(N, my + 1) : N) - pos0 : kCols;
+    if constexpr (kDkv) {
+      // The statistics land with the query tile; S(i) implies it, but only
+      // this wait orders the copy before this thread's reads.
+      if (!mbar_wait_warp(c.full + (2 * n.i) % kRing, ((2 * n.i) / kRing) & 1, c.abort_flag, kDevTimeoutKV)) return false;
+    }
+    if (!mbar_wait_warp(c.s, n.i & 1, c.abort_flag, kDevTimeoutS)) return false;
+    tc_fence_after();
+    float pr[kCols];
+    {
+      uint32_t rr[kCols / 32][32];
+#pragma unroll
+      for (int cc = 0; cc < kCols / 32; ++cc) tmem_ld32(tS + cc * 32, rr[cc]);
+      tmem_wait_ld();
+#pragma unroll
+      for (int x = 0; x < kCols; ++x) pr[x] = __uint_as_float(rr[x / 32][x % 32]);
+    }
+    if constexpr (!kDkv) {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(c.pr);
+    }
+#pragma unroll
+    for (int cc = 0; cc < kCols / 32; ++cc) {
+      [[maybe_unused]] uint32_t pk[16];
+#pragma unroll
+      for (int e = 0; e < 32; e += 4) {
+        const int x = cc * 32 + e;
+        float4 nl = make_float4(row_nl, row_nl, row_nl, row_nl);
+        if constexpr (kDkv) nl = *reinterpret_cast<const float4*>(st + x);
+        const float2 a = __ffma2_rn(make_float2(pr[x], pr[x + 1]), c2, make_float2(nl.x, nl.y));
+        const float2 d = __ffma2_rn(make_float2(pr[x + 2], pr[x + 3]), c2, make_float2(nl.z, nl.w));
+        pr[x] = ex2_approx(a.x);
+        pr[x + 1] = ex2_approx(a.y);
+        pr[x + 2] = ex2_approx(d.x);
+        pr[x + 3] = ex2_approx(d.y);
+        if constexpr (kMasked) {
+#pragma unroll
+          for (int y = x; y < x + 4; ++y)
+            if (y < lo || y >= hi) pr[y] = 0.f;
+        }
+        if constexpr (kDkv) {
+          pk[e / 2] = BwdElem<T>::pack2(pr[x], pr[x + 1]);
+          pk[e / 2 + 1] = BwdElem<T>::pack2(pr[x + 2], pr[x + 3]);
+        }
+      }
+      if constexpr (kDkv) tmem_st16(tS + cc * 16, pk);
+    }
+    if constexpr (kDkv) {
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(c.pr);
+    }
+    if (!mbar_wait_warp(c.dp, n.i & 1, c.abort_flag, kDevTimeoutS)) return false;
+    tc_fence_after();
+    uint32_t rr[kCols / 32][32];
+#pragma unroll
+    for (int cc = 0; cc < kCols / 32; ++cc) tmem_ld32(tP + cc * 32, rr[cc]);
+    tmem_wait_ld();
+#pragma unroll
+    for (int cc = 0; cc < kCols / 32; ++cc) {
+      [[maybe_unused]] uint32_t pk[16];
+#pragma unroll
+      for (int e = 0; e < 32; e += 4) {
+        const int x = cc * 32 + e;
+        float4 nd = make_float4(row_nd, row_nd, row_nd, row_nd);
+        if constexpr (kDkv) nd = *reinterpret_cast<const float4*>(st + kBS + x);
+        float2 d0 = __fadd2_rn(make_float2(__uint_as_float(rr[cc][e]), __uint_as_float(rr[cc][e + 1])),
+                               make_float2(nd.x, nd.y));
+        float2 d1 = __fadd2_rn(make_float2(__uint_as_float(rr[cc][e + 2]), __uint_as_float(rr[cc][e + 3])),
+                               make_float2(nd.z, nd.w));
+        d0 = __fmul2_rn(make_float2(pr[x], pr[x + 1]), d0);
+        d1 = __fmul2_rn(make_float2(pr[x + 2], pr[x + 3]), d1);
+        if constexpr (kDkv && BwdElem<T>::kScaled) {
+          d0 = __fmul2_rn(d0, make_float2(cta_scale, cta_scale));
+          d1 = __fmul2_rn(d1, make_float2(cta_scale, cta_scale));
+        }
+        if constexpr (kMasked) {
+          // P is 0 there, but dP may be infinite or NaN.
+          if (x < lo || x >= hi) d0.x = 0.f;
+          if (x + 1 < lo || x + 1 >= hi) d0.y = 0.f;
+          if (x + 2 < lo || x + 2 >= hi) d1.x = 0.f;
+          if (x + 3 < lo || x + 3 >= hi) d1.y = 0.f;
+        }
+        pk[e / 2] = BwdElem<T>::pack2(d0.x, d0.y);
+        pk[e / 2 + 1] = BwdElem<T>::pack2(d1.x, d1.y);
+      }
+      tmem_st16(tP + cc * 16, pk);
+    }
+    tmem_wait_st();
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(c.ds);
+    return true;
+  };
+  int ti = w.nt > 0 ? w.begin % w.per_head : 0;
+  for (int i = 0; i < nt; ++i) {
+    // Streamed rows of this tile: query positions (dK/dV) or key positions.
+    const int pos0 = (w.first + ti) * kBS + half * kCols;
+    bool need_mask;
+    if constexpr (kDkv)
+      need_mask = p.causal && pos0 < row0 + 127;
+    else
+      need_mask = pos0 + kCols > N || (p.causal && pos0 + kCols - 1 > row0);
+    if (!(need_mask ? step(std::true_type{}, pos0) : step(std::false_type{}, pos0))) return false;
+    ++n.i;
+    if (++ti == w.per_head) ti = 0;
+  }
+
+  // -------------------------------------------------------------- epilogue
+  if (nt > 0) {
+    if (!mbar_wait_warp(c.done, n.items & 1, c.abort_flag, kDevTimeoutO)) return false;
+    tc_fence_after();
+    ++n.items;
+  }
+  const Out out(p, w, half, r);
+  const bool is_v = kDkv && half == 1;
+  const float mul = is_v ? exp2f(-BwdElem<T>::kPExp) : p.scale * unscale;
+  const uint32_t t_acc = tmem + lane_base + C::kTmemAcc + (kDkv ? (is_v ? Out::kOut : 0) : out.col0);
+  const bool sliced = w.slices > 1;
+#pragma unroll 1
+  for (int cc = 0; cc < Out::kCols / 32; ++cc) {
+    float v[32];
+    if (nt > 0) {
+      uint32_t rr[32];
+      tmem_ld32(t_acc + cc * 32, rr);
+      tmem_wait_ld();
+#pragma unroll
+      for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(rr[e]) * mul;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) v[e] = 0.f;  // no pair is visible
+    }
+    if (sliced) {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) out.part[(cc * 32 + e) * 128] = v[e];
+    } else {
+      const int left = p.D - out.col0 - cc * 32;
+      if (out.row_ok && left > 0) bwd_store32<T>(out.row + out.col0 + cc * 32, v, left);
+    }
+  }
+  if (nt > 0) {
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(c.acc_free);
+  }
+  return true;
+}
+
+// One CTA per SM works through items: its own block index, then those of
+// blocks that have not started, which it takes from the hardware scheduler
+// (cluster launch control).  Loads, products and softmax run ahead into the
+// next item, so only the accumulators' read-out separates two items.
+template <typename T, int kDP>
+__global__ void __launch_bounds__(384, 1)
+    fa_bwd_kernel(const __grid_constant__ FaBwdParams p, const __grid_constant__ CUtensorMap k_a,
+                  const __grid_constant__ CUtensorMap v_a, const __grid_constant__ CUtensorMap q_b,
+                  const __grid_constant__ CUtensorMap g_b, const __grid_constant__ CUtensorMap q_a,
+                  const __grid_constant__ CUtensorMap g_a, const __grid_constant__ CUtensorMap k_b,
+                  const __grid_constant__ CUtensorMap v_b) {
+  using C = BwdCfg<kDP>;
+  extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
-  uint8_t* smem = smem_raw + ((1024u - (raw & 1023u)) & 1023u);
-  uint8_t* sA0 = smem;
-  uint8_t* sA1 = sA0 + C::kABytes;
-  uint8_t* sB = sA1 + C::kABytes;
-  float* sStat = reinterpret_cast<float*>(sB + kRing * C::kBBytes);
-  uint64_t* bar_full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(sStat) + C::kStatBufs * C::kStatBytes);
-  uint64_t* bar_empty = bar_full + kRing;
-  uint64_t* bar_a = bar_empty + kRing;  // [2]
-  uint64_t* bar_s = bar_a + 2;          // S(i) complete
-  uint64_t* bar_p = bar_s + 1;          // P(i) stored (dK/dV), S(i) read (dQ)
-  uint64_t* bar_dp = bar_p + 1;         // dP(i) complete
-  uint64_t* bar_ds = bar_dp + 1;        // dS(i) stored
-  uint64_t* bar_done = bar_ds + 1;      // accumulators final
-  uint64_t* bar_fix = bar_done + 1;     // ragged tile landed, before its rows are cleared
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_fix + 1);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-
+  const BwdCta<kDP> c(smem_raw + ((1024u - (raw & 1023u)) & 1023u));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kRing; ++s) {
-      mbar_init(bar_full + s, 1);
-      mbar_init(bar_empty + s, 1);
+    for (int s = 0; s < C::kRing; ++s) {
+      mbar_init(c.full + s, 1);
+      mbar_init(c.empty + s, 1);
     }
-    mbar_init(bar_a, 1);
-    mbar_init(bar_a + 1, 1);
-    mbar_init(bar_s, 1);
-    mbar_init(bar_p, 8);  // one arrival per softmax warp
-    mbar_init(bar_dp, 1);
-    mbar_init(bar_ds, 8);
-    mbar_init(bar_done, 1);
-    mbar_init(bar_fix, 1);
-    *abort_flag = *reinterpret_cast<volatile int*>(&g_fab_device_error) != 0 ? 1 : 0;
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(c.a_full + x, 1);
+      mbar_init(c.a_empty + x, 1);
+      mbar_init(c.sched_full + x, 1);
+      mbar_init(c.sched_empty + x, 9);  // the issuer and the eight softmax warps
+    }
+    mbar_init(c.s, 1);
+    mbar_init(c.pr, 8);  // one arrival per softmax warp
+    mbar_init(c.dp, 1);
+    mbar_init(c.ds, 8);
+    mbar_init(c.done, 1);
+    mbar_init(c.acc_free, 8);
+    mbar_init(c.fix, 1);
+    mbar_init(c.clc, 1);
+    mbar_init(c.drained, 1);
+    *c.abort_flag = *reinterpret_cast<volatile int*>(&g_fab_device_error) != 0 ? 1 : 0;
     mbar_fence_init();
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, 512);
+    tmem_alloc(c.tmem_slot, 512);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
-  const bool skip = *abort_flag != 0;
+  const uint32_t tmem = *c.tmem_slot;
+  const bool skip = *c.abort_flag != 0;
+  // The item after the q-th, for the issuer and the softmax warps; -1: none.
+  auto next_item = [&](int q) -> int {
+    if (!mbar_wait_warp(c.sched_full + (q & 1), (q >> 1) & 1, c.abort_flag, kDevTimeoutSched)) return -1;
+    const int x = c.next[q & 1];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(c.sched_empty + (q & 1));
+    return x;
+  };
 
   // Each warpgroup re-splits its registers first, whatever it does after.
   if (warp < 4) {
     setmaxnreg_dec<C::kLoadRegs>();
-  if (warp == 0 && !skip && nt > 0) {
-    // ------------------------------------------------------------ producer
-    // The whole warp runs this; lane 0 issues the copies.
-    const bool packed = p.cu_q != nullptr;
-    const int stat_len = kDkv ? M : N;  // valid streamed rows of the sequence
-    const int row_base = kDkv ? q_row0 : k_row0;
-    if (lane == 0) {
-      const int a_row = (kDkv ? k_row0 : q_row0) + row0;
-      mbar_arrive_expect_tx(bar_a, C::kABytes);
-      for (int a = 0; a < C::kAtoms; ++a) tma_load_4d(sA0 + a * C::kAAtomBytes, a0, bar_a, a * 64, a_row, h, map_b);
-      mbar_arrive_expect_tx(bar_a + 1, C::kABytes);
-      for (int a = 0; a < C::kAtoms; ++a)
-        tma_load_4d(sA1 + a * C::kAAtomBytes, a1, bar_a + 1, a * 64, a_row, h, map_b);
-    }
-    bool ok = true;
-    uint32_t fixes = 0;
-    int issued = 0;
-    int g = 0, ti = first;  // head of the group and tile of streamed pair t / 2
-    for (int t = 0; t < 2 * nt; ++t) {
-      const int s = t % kRing;
-      const bool second = (t & 1) != 0;
-      if (!(ok = mbar_wait_warp(bar_empty + s, ((t / kRing) & 1) ^ 1, abort_flag, kDevTimeoutEmpty))) break;
-      const int rows_left = stat_len - ti * kBS;
-      // A packed sequence's last tile runs into the next sequence's rows.
-      // Rows of the summed dimension must be zero there (0 x NaN is NaN), so
-      // such a tile is cleared past the end before it is handed on.  V tiles
-      // of dQ CTAs are exempt: they only feed dP columns that are masked.
-      const bool fix = packed && rows_left < kBS && (kDkv || !second);
-      uint64_t* bar = fix ? bar_fix : bar_full + s;
+    if (warp == 0 && !skip) {
+      BwdCount n;
+      volatile int no_abort = 0;
+      int index = static_cast<int>(blockIdx.x);
+      for (int q = 0; index >= 0; ++q) {
+        const bool ok = index < p.num_dkv
+                            ? bwd_produce<T, kDP, true>(p, c, &k_a, &v_a, &q_b, &g_b, index, n)
+                            : bwd_produce<T, kDP, false>(p, c, &q_a, &g_a, &k_b, &v_b, index - p.num_dkv, n);
+        if (!ok) break;
+        // All of this item's loads are under way: ask for the next one.
+        if (q >= 2 && !mbar_wait_warp(c.sched_empty + (q & 1), ((q - 2) >> 1) & 1, c.abort_flag, kDevTimeoutSched)) break;
+        int x = -1;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(c.clc, 16);
+          clc_try_cancel(c.clc_resp, c.clc);
+          if (mbar_wait(c.clc, q & 1, &no_abort, kDevTimeoutSched)) x = clc_first_cta_x(c.clc_resp);
+          c.next[q & 1] = x;
+          mbar_arrive(c.sched_full + (q & 1));
+        }
+        index = __shfl_sync(0xffffffffu, x, 0);
+      }
+      // No copy may still be landing when the CTA leaves.
       if (lane == 0) {
-        // A query tile brings its rows' statistics along (same barrier; its
-        // buffer is free when its slot is: both were last used for dK).
-        const bool stat = kDkv && !second;
-        mbar_arrive_expect_tx(bar, C::kBBytes + (stat ? C::kStatBytes : 0));
-        if (stat)
-          bulk_load_g2s(sStat + (t / 2) % C::kStatBufs * (2 * kBS),
-                        p.stats + (bwd_stat_tile0(p, b, h_stream0 + g, q_row0, kBS) + ti) * (2 * kBS), C::kStatBytes, bar);
-        uint8_t* dst = sB + s * C::kBBytes;
-        const CUtensorMap* map = second ? b1 : b0;
-        for (int a = 0; a < C::kAtoms; ++a)
-          tma_load_4d(dst + a * C::kBAtomBytes, map, bar, a * 64, row_base + ti * kBS, h_stream0 + g, map_b);
+        for (int x = 0; x < 2; ++x)
+          if (n.items > 0) mbar_wait(c.a_full + x, (n.items - 1) & 1, &no_abort, kDevTimeoutTeardown);
+        for (int x = max(0, n.t - C::kRing); x < n.t; ++x)
+          mbar_wait(c.full + (x % C::kRing), (x / C::kRing) & 1, &no_abort, kDevTimeoutTeardown);
       }
-      issued = t + 1;
-      if (fix) {
-        if (!(ok = mbar_wait_warp(bar_fix, fixes & 1, abort_flag, kDevTimeoutKV))) break;
-        ++fixes;
-        uint8_t* dst = sB + s * C::kBBytes;
-        const int chunks = (kBS - rows_left) * 8;  // 16-byte pieces of one atom's rows past the end
-        for (int a = 0; a < C::kAtoms; ++a)
-          for (int c = lane; c < chunks; c += 32)
-            *reinterpret_cast<uint4*>(dst + a * C::kBAtomBytes + rows_left * 128 + c * 16) = make_uint4(0, 0, 0, 0);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar_full + s);
+      __syncwarp();
+    } else if (warp == 1 && !skip) {
+      const bool leader = elect_one();
+      BwdCount n;
+      int index = static_cast<int>(blockIdx.x);
+      for (int q = 0; index >= 0; ++q) {
+        const bool ok = index < p.num_dkv ? bwd_issue<T, kDP, true>(p, c, tmem, leader, index, n)
+                                          : bwd_issue<T, kDP, false>(p, c, tmem, leader, index - p.num_dkv, n);
+        if (!ok) break;
+        index = next_item(q);
       }
-      if (second && ++ti == last) {
-        ti = first;
-        ++g;
-      }
+      // Drain the tensor pipe before TMEM is released.
+      if (leader) mma_commit(c.drained);
+      volatile int no_abort = 0;
+      mbar_wait_warp(c.drained, 0, &no_abort, kDevTimeoutTeardown);
     }
-    // No copy may still be landing when the CTA leaves.
-    volatile int no_abort = 0;
-    if (lane == 0) {
-      mbar_wait(bar_a, 0, &no_abort, kDevTimeoutTeardown);
-      mbar_wait(bar_a + 1, 0, &no_abort, kDevTimeoutTeardown);
-      for (int x = max(0, issued - kRing); x < issued; ++x)
-        mbar_wait(bar_full + (x % kRing), (x / kRing) & 1, &no_abort, kDevTimeoutTeardown);
-    }
-    __syncwarp();
-  } else if (warp == 1 && !skip && nt > 0) {
-    // ---------------------------------------------------------- MMA issuer
-    const bool leader = elect_one();
-    constexpr uint32_t kFmt = BwdElem<T>::kFmt;
-    constexpr uint32_t idesc_s = umma_idesc(kFmt, 128, kBS, 0, 0);
-    constexpr uint32_t idesc_o = umma_idesc(kFmt, 128, kOut, 0, 1);
-    constexpr uint32_t kHi = umma_desc_hi(1024, kLayoutSw128);
-    const uint32_t a0_lo = umma_desc_lo(smem_u32(sA0), 16);
-    const uint32_t a1_lo = umma_desc_lo(smem_u32(sA1), 16);
-    const uint32_t b_lo = umma_desc_lo(smem_u32(sB), 16);
-    // The same tiles as MN-major operands, from this CTA's first output column.
-    const uint32_t bn_lo = umma_desc_lo(smem_u32(sB) + (dcol0 / 64) * C::kBAtomBytes, C::kBAtomBytes);
-    auto wait = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
-      return mbar_wait_warp(bar, parity, abort_flag, code);
-    };
-    // D[128 x kBS] = A (stationary) x B(slot)^T over the head dim.
-    auto issue_s = [&](uint32_t d, uint32_t alo, int s) {
-      uint32_t qa = alo, kb = b_lo + s * (C::kBBytes >> 4);
-      asm volatile("" : "+r"(qa), "+r"(kb));
-#pragma unroll
-      for (int kk = 0; kk < kDP / 16; ++kk) {
-        const int a = kk >> 2;
-        const uint32_t off = (kk & 3) * 32;
-        const uint64_t ad = umma_desc_join(qa + ((a * C::kAAtomBytes + off) >> 4), kHi);
-        const uint64_t bd = umma_desc_join(kb + ((a * C::kBAtomBytes + off) >> 4), kHi);
-        if (leader) mma_ss_f16(d, ad, bd, idesc_s, kk > 0 ? 1u : 0u);
-      }
-    };
-    // D[128 x kOut] += A (TMEM, kBS wide) x B(slot).  Each softmax warpgroup's
-    // half of A starts at its half of the fp32 columns.
-    auto issue_o = [&](uint32_t d, uint32_t a, int s, bool acc) {
-      uint32_t vb = bn_lo + s * (C::kBBytes >> 4);
-      asm volatile("" : "+r"(vb));
-#pragma unroll
-      for (int kk = 0; kk < kBS / 16; ++kk) {
-        constexpr int kHalf = kBS / 32;
-        const uint32_t at = a + (kk / kHalf) * (kBS / 2) + (kk % kHalf) * 8;
-        const uint64_t bd = umma_desc_join(vb + ((kk * 16 * 128) >> 4), kHi);
-        if (leader) mma_ts_f16(d, at, bd, idesc_o, (acc || kk > 0) ? 1u : 0u);
-      }
-    };
-    auto commit = [&](uint64_t* bar) {
-      if (leader) mma_commit(bar);
-    };
-    const uint32_t tS = tmem + C::kTmemS, tP = tmem + C::kTmemP;
-    const uint32_t tAcc0 = tmem + C::kTmemAcc, tAcc1 = tAcc0 + kOut;
-    auto slot = [](int t) { return t % kRing; };
-    auto par = [](int t) { return static_cast<uint32_t>((t / kRing) & 1); };
-
-    bool ok = wait(bar_a, 0, kDevTimeoutQ) && wait(bar_full + slot(0), par(0), kDevTimeoutKV);
-    if (ok) {
-      tc_fence_after();
-      issue_s(tS, a0_lo, slot(0));
-      commit(bar_s);
-      ok = wait(bar_a + 1, 0, kDevTimeoutQ) && wait(bar_full + slot(1), par(1), kDevTimeoutKV);
-    }
-    if (ok) {
-      tc_fence_after();
-      issue_s(tP, a1_lo, slot(1));
-      commit(bar_dp);
-      if constexpr (!kDkv) commit(bar_empty + slot(1));
-    }
-    for (int i = 0; ok && i < nt; ++i) {
-      const int t0 = 2 * i, t1 = 2 * i + 1;
-      if (!(ok = wait(bar_p, i & 1, kDevTimeoutP))) break;
-      tc_fence_after();
-      if constexpr (kDkv) {
-        issue_o(tAcc1, tS, slot(t1), i > 0);
-        commit(bar_empty + slot(t1));
-      }
-      if (i + 1 < nt) {
-        if (!(ok = wait(bar_full + slot(t0 + 2), par(t0 + 2), kDevTimeoutKV))) break;
-        tc_fence_after();
-        issue_s(tS, a0_lo, slot(t0 + 2));
-        commit(bar_s);
-      }
-      if (!(ok = wait(bar_ds, i & 1, kDevTimeoutP))) break;
-      tc_fence_after();
-      issue_o(tAcc0, tP, slot(t0), i > 0);
-      commit(bar_empty + slot(t0));
-      if (i + 1 < nt) {
-        if (!(ok = wait(bar_full + slot(t1 + 2), par(t1 + 2), kDevTimeoutKV))) break;
-        tc_fence_after();
-        issue_s(tP, a1_lo, slot(t1 + 2));
-        commit(bar_dp);
-        if constexpr (!kDkv) commit(bar_empty + slot(t1 + 2));
-      }
-    }
-    // Drain the tensor pipe; the softmax warps read the accumulators after this.
-    commit(bar_done);
-    volatile int no_abort = 0;
-    mbar_wait_warp(bar_done, 0, &no_abort, kDevTimeoutTeardown);
-  }
   } else {
     setmaxnreg_inc<C::kSoftmaxRegs>();
-  if (!skip) {
-    // ------------------------------------------------------------- softmax
-    const int half = (warp - 4) >> 2;
-    const int wq = warp & 3;
-    const int r = wq * 32 + lane;  // TMEM lane: stationary row
-    const uint32_t lane_base = static_cast<uint32_t>(wq * 32) << 16;
-    constexpr int kCols = kBS / 2;  // columns of one warpgroup
-    const uint32_t tS = tmem + lane_base + C::kTmemS + half * kCols;
-    const uint32_t tP = tmem + lane_base + C::kTmemP + half * kCols;
-    const int my = row0 + r;  // position of this lane's row in the sequence
-    const float2 c2 = make_float2(p.scale_log2, p.scale_log2);
-    float row_nl = 0.f, row_nd = 0.f, unscale = 1.f, cta_scale = 1.f;
-    if constexpr (!kDkv) {
-      if (nt > 0 && my < M) {
-        const int64_t st_tile = bwd_stat_tile0(p, b, h, q_row0, kBS) + my / kBS;
-        row_nl = p.stats[st_tile * (2 * kBS) + my % kBS];
-        row_nd = p.stats[st_tile * (2 * kBS) + kBS + my % kBS];
-        if constexpr (BwdElem<T>::kScaled) {
-          const float e = p.row_exp[st_tile * kBS + my % kBS];
-          row_nl += e - BwdElem<T>::kPExp;  // P, hence dS, times 2^e
-          unscale = exp2f(-e);
-        }
-      }
-    } else if constexpr (BwdElem<T>::kScaled) {
-      // Largest |dO| over every row this CTA sums.
-      float big = 0.f;
-      for (int x = lane; x < nt; x += 32)
-        big = fmaxf(big, p.tile_max[bwd_stat_tile0(p, b, h_stream0 + x / per_head, q_row0, kBS) + first + x % per_head]);
-#pragma unroll
-      for (int off = 16; off > 0; off >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
-      const float e = big > 0.f ? floorf(log2f(big)) : 0.f;
-      cta_scale = exp2f(-e - BwdElem<T>::kPExp);
-      unscale = exp2f(e);
-    }
-    // One streamed tile.  `masked`: some pair of this warpgroup's columns is
-    // not visible; `pos0` is the position of its first column.
-    auto step = [&](auto masked, int i, int pos0) -> bool {
-      constexpr bool kMasked = decltype(masked)::value;
-      [[maybe_unused]] const float* st = sStat + i % C::kStatBufs * (2 * kBS) + half * kCols;
-      // Visible columns [lo, hi) of this lane.
-      const int lo = kMasked && kDkv ? my - pos0 : 0;
-      const int hi = kMasked && !kDkv ? (p.causal ? min(N, my + 1) : N) - pos0 : kCols;
-      if constexpr (kDkv) {
-        // The statistics land with the query tile; S(i) implies it, but only
-        // this wait orders the copy before this thread's reads.
-        if (!mbar_wait_warp(bar_full + (2 * i) % kRing, ((2 * i) / kRing) & 1, abort_flag, kDevTimeoutKV)) return false;
-      }
-      if (!mbar_wait_warp(bar_s, i & 1, abort_flag, kDevTimeoutS)) return false;
-      tc_fence_after();
-      float pr[kCols];
-      {
-        uint32_t rr[kCols / 32][32];
-#pragma unroll
-        for (int cc = 0; cc < kCols / 32; ++cc) tmem_ld32(tS + cc * 32, rr[cc]);
-        tmem_wait_ld();
-#pragma unroll
-        for (int x = 0; x < kCols; ++x) pr[x] = __uint_as_float(rr[x / 32][x % 32]);
-      }
-      if constexpr (!kDkv) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar_p);
-      }
-#pragma unroll
-      for (int cc = 0; cc < kCols / 32; ++cc) {
-        [[maybe_unused]] uint32_t pk[16];
-#pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          const int x = cc * 32 + e;
-          float4 nl = make_float4(row_nl, row_nl, row_nl, row_nl);
-          if constexpr (kDkv) nl = *reinterpret_cast<const float4*>(st + x);
-          const float2 a = __ffma2_rn(make_float2(pr[x], pr[x + 1]), c2, make_float2(nl.x, nl.y));
-          const float2 d = __ffma2_rn(make_float2(pr[x + 2], pr[x + 3]), c2, make_float2(nl.z, nl.w));
-          pr[x] = ex2_approx(a.x);
-          pr[x + 1] = ex2_approx(a.y);
-          pr[x + 2] = ex2_approx(d.x);
-          pr[x + 3] = ex2_approx(d.y);
-          if constexpr (kMasked) {
-#pragma unroll
-            for (int y = x; y < x + 4; ++y)
-              if (y < lo || y >= hi) pr[y] = 0.f;
-          }
-          if constexpr (kDkv) {
-            pk[e / 2] = BwdElem<T>::pack2(pr[x], pr[x + 1]);
-            pk[e / 2 + 1] = BwdElem<T>::pack2(pr[x + 2], pr[x + 3]);
-          }
-        }
-        if constexpr (kDkv) tmem_st16(tS + cc * 16, pk);
-      }
-      if constexpr (kDkv) {
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar_p);
-      }
-      if (!mbar_wait_warp(bar_dp, i & 1, abort_flag, kDevTimeoutS)) return false;
-      tc_fence_after();
-      uint32_t rr[kCols / 32][32];
-#pragma unroll
-      for (int cc = 0; cc < kCols / 32; ++cc) tmem_ld32(tP + cc * 32, rr[cc]);
-      tmem_wait_ld();
-#pragma unroll
-      for (int cc = 0; cc < kCols / 32; ++cc) {
-        [[maybe_unused]] uint32_t pk[16];
-#pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          const int x = cc * 32 + e;
-          float4 nd = make_float4(row_nd, row_nd, row_nd, row_nd);
-          if constexpr (kDkv) nd = *reinterpret_cast<const float4*>(st + kBS + x);
-          float2 d0 = __fadd2_rn(make_float2(__uint_as_float(rr[cc][e]), __uint_as_float(rr[cc][e + 1])),
-                                 make_float2(nd.x, nd.y));
-          float2 d1 = __fadd2_rn(make_float2(__uint_as_float(rr[cc][e + 2]), __uint_as_float(rr[cc][e + 3])),
-                                 make_float2(nd.z, nd.w));
-          d0 = __fmul2_rn(make_float2(pr[x], pr[x + 1]), d0);
-          d1 = __fmul2_rn(make_float2(pr[x + 2], pr[x + 3]), d1);
-          if constexpr (kDkv && BwdElem<T>::kScaled) {
-            d0 = __fmul2_rn(d0, make_float2(cta_scale, cta_scale));
-            d1 = __fmul2_rn(d1, make_float2(cta_scale, cta_scale));
-          }
-          if constexpr (kMasked) {
-            // P is 0 there, but dP may be infinite or NaN.
-            if (x < lo || x >= hi) d0.x = 0.f;
-            if (x + 1 < lo || x + 1 >= hi) d0.y = 0.f;
-            if (x + 2 < lo || x + 2 >= hi) d1.x = 0.f;
-            if (x + 3 < lo || x + 3 >= hi) d1.y = 0.f;
-          }
-          pk[e / 2] = BwdElem<T>::pack2(d0.x, d0.y);
-          pk[e / 2 + 1] = BwdElem<T>::pack2(d1.x, d1.y);
-        }
-        tmem_st16(tP + cc * 16, pk);
-      }
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar_ds);
-      return true;
-    };
-    bool ok = true;
-    int ti = first;
-    for (int i = 0; ok && i < nt; ++i) {
-      // Streamed rows of this tile: query positions (dK/dV) or key positions.
-      const int pos0 = ti * kBS + half * kCols;
-      bool need_mask;
-      if constexpr (kDkv)
-        need_mask = p.causal && pos0 < row0 + 127;
-      else
-        need_mask = pos0 + kCols > N || (p.causal && pos0 + kCols - 1 > row0);
-      ok = need_mask ? step(std::true_type{}, i, pos0) : step(std::false_type{}, i, pos0);
-      if (++ti == last) ti = first;
-    }
-
-    // ------------------------------------------------------------ epilogue
-    // dK/dV: warpgroup 0 writes dK (acc 0), warpgroup 1 dV (acc 1); dQ: each
-    // warpgroup half of the columns.
-    if (nt > 0 && ok) ok = mbar_wait_warp(bar_done, 0, abort_flag, kDevTimeoutO);
-    tc_fence_after();
-    const bool row_ok = my < (kDkv ? N : M);
-    T* out;
-    float mul;
-    int col0, ncol;
-    uint32_t t_acc;
-    if constexpr (kDkv) {
-      const bool is_v = half == 1;
-      out = reinterpret_cast<T*>(is_v ? p.dv : p.dk);
-      const int64_t ss = is_v ? p.dv_ss : p.dk_ss, sh = is_v ? p.dv_sh : p.dk_sh, sb = is_v ? p.dv_sb : p.dk_sb;
-      out += (p.cu_k ? k_row0 * ss : b * sb) + h * sh + my * ss;
-      mul = is_v ? exp2f(-BwdElem<T>::kPExp) : p.scale * unscale;
-      col0 = dcol0;
-      ncol = kOut;
-      t_acc = tmem + lane_base + C::kTmemAcc + (is_v ? kOut : 0);
-    } else {
-      out = reinterpret_cast<T*>(p.dq) + (p.cu_q ? q_row0 * p.dq_ss : b * p.dq_sb) + h * p.dq_sh + my * p.dq_ss;
-      mul = p.scale * unscale;
-      col0 = half * (kOut / 2);
-      ncol = kOut / 2;
-      t_acc = tmem + lane_base + C::kTmemAcc + col0;
-    }
-    if (ok) {
-#pragma unroll 1
-      for (int cc = 0; cc < ncol / 32; ++cc) {
-        float v[32];
-        if (nt > 0) {
-          uint32_t rr[32];
-          tmem_ld32(t_acc + cc * 32, rr);
-          tmem_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(rr[e]) * mul;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = 0.f;  // no pair is visible
-        }
-        const int left = p.D - col0 - cc * 32;
-        if (row_ok && left > 0) bwd_store32<T>(out + col0 + cc * 32, v, left);
+    if (!skip) {
+      asm volatile("griddepcontrol.wait;" ::: "memory");  // the statistics
+      BwdCount n;
+      int index = static_cast<int>(blockIdx.x);
+      for (int q = 0; index >= 0; ++q) {
+        const bool ok = index < p.num_dkv ? bwd_softmax<T, kDP, true>(p, c, tmem, index, n)
+                                          : bwd_softmax<T, kDP, false>(p, c, tmem, index - p.num_dkv, n);
+        if (!ok) break;
+        index = next_item(q);
       }
     }
-  }
   }
 
   tc_fence_before();
@@ -705,19 +929,30 @@ __device__ __forceinline__ void fa_bwd_body(const FaBwdParams& p, const CUtensor
   }
 }
 
-template <typename T, int kDP>
-__global__ void __launch_bounds__(384, 1)
-    fa_bwd_kernel(const __grid_constant__ FaBwdParams p, const __grid_constant__ CUtensorMap k_a,
-                  const __grid_constant__ CUtensorMap v_a, const __grid_constant__ CUtensorMap q_b,
-                  const __grid_constant__ CUtensorMap g_b, const __grid_constant__ CUtensorMap q_a,
-                  const __grid_constant__ CUtensorMap g_a, const __grid_constant__ CUtensorMap k_b,
-                  const __grid_constant__ CUtensorMap v_b) {
-  extern __shared__ uint8_t smem_raw[];
-  const int x = static_cast<int>(blockIdx.x);
-  if (x < p.num_dkv)
-    fa_bwd_body<T, kDP, true>(p, &k_a, &v_a, &q_b, &g_b, x, smem_raw);
-  else
-    fa_bwd_body<T, kDP, false>(p, &q_a, &g_a, &k_b, &v_b, x - p.num_dkv, smem_raw);
+// Adds the slices of every tile that has more than one, in slice order, and
+// stores the result.  blockIdx.x: tile (as an item without its slice),
+// blockIdx.y: 32-column chunk of a thread's columns.
+template <typename T, int kDP, bool kDkv>
+__global__ void __launch_bounds__(256) fa_bwd_join_kernel(const FaBwdParams p) {
+  using Out = BwdOut<T, kDP, kDkv>;
+  const int max_slices = kDkv ? p.dkv_slices : p.dq_slices;
+  BwdItem w;
+  if (!bwd_item<kDP, kDkv>(p, static_cast<int>(blockIdx.x) * max_slices, w) || w.slices <= 1) return;
+  const Out out(p, w, threadIdx.x >> 7, threadIdx.x & 127);
+  const int cc = blockIdx.y;
+  const int left = p.D - out.col0 - cc * 32;
+  if (!out.row_ok || left <= 0) return;
+  constexpr int64_t kSlot = static_cast<int64_t>(kDkv ? 2 : 1) * Out::kOut * 128;
+  const float* src = out.part + cc * 32 * 128;
+  float v[32];
+#pragma unroll
+  for (int e = 0; e < 32; ++e) v[e] = src[e * 128];
+  for (int s = 1; s < w.slices; ++s) {
+    src += kSlot;
+#pragma unroll
+    for (int e = 0; e < 32; ++e) v[e] += src[e * 128];
+  }
+  bwd_store32<T>(out.row + out.col0 + cc * 32, v, left);
 }
 
 }  // namespace fab

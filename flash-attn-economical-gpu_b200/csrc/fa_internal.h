@@ -119,7 +119,14 @@ struct FaBwdParams {
   float scale_log2;
   int causal;
   int q_tiles, k_tiles;  // 128-row tiles of the longest sequence
-  int num_dkv;           // CTAs below this index form dK and dV, the others dQ
+  int num_dkv;           // items below this index form dK and dV, the others dQ
+  // Slices of a tile's work (see bwd_slices): their length in streamed tiles
+  // and the most of them a tile has; fp32 sums of tiles with more than one.
+  int dkv_slice_len, dkv_slices;
+  int dq_slice_len, dq_slices;
+  int part_k_tiles, part_q_tiles;  // tiles of one head, numbered like stat_tiles
+  float* dkv_part;
+  float* dq_part;
   const int* cu_q;       // packed batches, as in FaKernelParams
   const int* cu_k;
   int total_q;
