@@ -23,15 +23,20 @@
 // heads need no second reduction.
 //
 // A CTA stays on its SM and takes item after item (a tile, or a slice of one
-// when there are few).  Warp 0 loads (TMA), warp 1 issues tcgen05.mma, warps
-// 4-11 are two softmax warpgroups: each covers the 128 lanes and one half of
-// the streamed tile's columns.  Per streamed tile i the issue order is
-//   [dV(i)] S(i+1)  |  dK/dQ(i) dP(i+1)
-// where the first group waits for P(i) (or, in dQ items, for S(i) to have been
-// read) and the second for dS(i): while the softmax warps turn S(i+1) into P
-// the tensor core runs dK(i) and dP(i+1), and while they turn dP into dS it
-// runs dV(i) and S(i+1).  P overwrites its own half of S, dS its own half of
-// dP, so no warp writes columns another still has to read.
+// when there are few).  Warps 0 and 3 load (TMA; one operand each), warps 1
+// and 2 issue tcgen05.mma, warps 4-11 are two softmax warpgroups: each covers the 128 lanes and one half of
+// the streamed tile's columns.  Per streamed tile i
+//   warp 1 issues  [dV(i)] S(i+1)      once P(i) is stored (dQ: S(i) read)
+//   warp 2 issues  dK(i)/dQ(i) dP(i+1) once dS(i) is stored
+// Each pair shares one TMEM buffer (P overwrites S, dS overwrites dP), whose
+// products its warp keeps in order; the two pairs touch different buffers and
+// need no order between them.  One issuing warp for all four left the tensor
+// core idle for the few hundred cycles that a warp's first wait after a burst
+// of products takes (measured: twice per tile, of some 3300 cycles); with two,
+// the other's products run meanwhile.  While the softmax warps turn S(i+1)
+// into P the tensor core runs dK(i) and dP(i+1), and while they turn dP into
+// dS it runs dV(i) and S(i+1).  P overwrites its own half of S, dS its own
+// half of dP, so no warp writes columns another still has to read.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -83,25 +88,44 @@ struct BwdElem<__half> {
 // three 64-row ones.  dK and dV together exceed TMEM at 256, so there a dK/dV
 // item forms S and dP over the whole head dim but 128 columns of each output,
 // and two items cover a key tile.
+//
+// The two streamed operands have a ring each.  The first (Q, or K) is read by
+// S(i) and again by dK(i) or dQ(i), a whole tile's time later, and its next
+// load has only until S two tiles on to land; the second (dO, or V) is done
+// with half a tile after it is first read.  So the first ring is the longer.
+#ifndef FAB_BWD_HALVES
+#define FAB_BWD_HALVES 1
+#endif
+#ifndef FAB_BWD_TURNS
+#define FAB_BWD_TURNS 1
+#endif
+#ifndef FAB_BWD_PASS
+#define FAB_BWD_PASS (kDP / 32)
+#endif
 template <int kDP_>
 struct BwdCfg {
   static constexpr int kDP = kDP_;
-  static constexpr int kBS = kDP == 256 ? 64 : 128;                      // streamed rows
-  static constexpr int kRing = kDP == 256 ? 3 : kDP == 128 ? 4 : 8;      // streamed tiles in shared memory
-  static constexpr int kAtoms = kDP / 64;                                // 128-byte column atoms
+  static constexpr int kBS = kDP == 256 ? 64 : 128;  // streamed rows
+  static constexpr int kRing0 = kDP == 256 ? 2 : kDP == 128 ? 3 : 4;
+  static constexpr int kRing1 = kDP == 256 ? 1 : kDP == 128 ? 2 : 3;
+  static constexpr int kAtoms = kDP / 64;  // 128-byte column atoms
   static constexpr int kAAtomBytes = 128 * 128;
   static constexpr int kABytes = kAAtomBytes * kAtoms;
   static constexpr int kBAtomBytes = kBS * 128;
   static constexpr int kBBytes = kBAtomBytes * kAtoms;
-  // Statistics of the streamed query tiles: one buffer per resident one.
-  static constexpr int kStatBufs = (kRing + 1) / 2;
-  static constexpr int kStatBytes = 2 * kBS * 4;
-  static constexpr int kOutDkv = kDP == 256 ? 128 : kDP;                 // output columns of one dK/dV item
+  static constexpr int kStatBytes = 2 * kBS * 4;  // statistics of a streamed query tile, two buffers
+  static constexpr int kOutDkv = kDP == 256 ? 128 : kDP;  // output columns of one dK/dV item
   static constexpr int kDSplit = kDP / kOutDkv;
-  // full/empty per slot; stationary full/empty x 2; S, P, dP, dS; accumulators
-  // final and read; ragged tile; next item full/empty x 2; its request; teardown.
-  static constexpr int kNumBars = 2 * kRing + 4 + 4 + 2 + 1 + 4 + 2;
-  static constexpr int kSmemBytes = 1024 + 2 * kABytes + kRing * kBBytes + kStatBufs * kStatBytes + kNumBars * 8 + 48;
+  // full/empty per slot; statistics full/empty x 2; stationary full/empty x 2;
+  // S, P x 2, dP, dS x 2; issue order x 2; accumulators final x 2 and read; ragged tile x 2; next item
+  // full/empty x 2; its request; teardown x 2.
+  static constexpr int kNumBars = 2 * (kRing0 + kRing1) + 4 + 4 + 6 + 3 + 2 + 4 + 3 + 2;
+  static constexpr int kTailBytes = 208;  // TMEM address, abort flag, two items, the scheduler's response
+  static constexpr int kSmemBytes =
+      2 * kABytes + (kRing0 + kRing1) * kBBytes + 2 * kStatBytes + kNumBars * 8 + kTailBytes;
+  // P and dS are handed to the tensor core in two halves where a warp works
+  // through two 32-column chunks.
+  static constexpr bool kHalves = kBS == 128 && FAB_BWD_HALVES;
   static constexpr int kThreads = 384;
   // Launched with 168 registers a thread; the load/MMA warpgroup hands some
   // to the two softmax warpgroups, which hold a 64-column row of P across
@@ -263,9 +287,39 @@ __device__ __forceinline__ void bwd_store32(T* dst, const float (&v)[32], int nc
   }
 }
 
+// Warp-collective bounded wait for a phase, in few instructions: these kernels
+// hold some sixty waits, and with the general one (ptx.cuh) inlined at each
+// they outgrew the instruction cache.  Each try suspends for a microsecond at
+// most; after kWaitTries, or once another warp of the CTA has given up, the
+// warp leaves its code in the abort flag and unwinds.
+constexpr uint32_t kWaitTries = 4000000;
+__device__ __forceinline__ bool bwd_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int code) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .u32 n, a;\n\t"
+      "mov.u32 n, %4;\n\t"
+      "WAIT:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\t"
+      "@p bra DONE;\n\t"
+      "ld.volatile.shared.u32 a, [%3];\n\t"
+      "sub.u32 n, n, 1;\n\t"
+      "setp.eq.u32 q, n, 0;\n\t"
+      "setp.ne.or.u32 q, a, 0, q;\n\t"
+      "@!q bra WAIT;\n\t"
+      "DONE:\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(smem_u32(const_cast<const int*>(abort))), "n"(kWaitTries)
+      : "memory");
+  if (__all_sync(0xffffffffu, ok != 0)) return true;
+  *abort = code;
+  return false;
+}
+
 // A work item: one stationary tile (and, at head dim 256, one half of the
 // output columns) against a slice of its streamed tiles.
 struct BwdItem {
+  int kind;                // kItemDkv, kItemDq, or kItemEnd: no more
   int b, h, tile;          // batch entry, head (of the stationary tile), 128-row tile
   int dcol0;               // first output column
   int q_row0, k_row0;      // the sequence's first rows in a packed tensor
@@ -273,8 +327,10 @@ struct BwdItem {
   int row0;                // first stationary row within the sequence
   int first, per_head;     // streamed tiles [first, first + per_head) of each head
   int begin, nt;           // this slice: streamed tiles begin .. begin + nt of all heads'
+  int begin_head, begin_tile;  // begin / per_head, begin % per_head
   int slice, slices;
 };
+enum BwdItemKind : int { kItemEnd, kItemDkv, kItemDq };
 
 // Streamed tiles of a stationary tile are cut into slices when there are too
 // few stationary tiles to fill the GPU; slice s of `slices` takes an even
@@ -321,6 +377,9 @@ __device__ __forceinline__ bool bwd_item(const FaBwdParams& p, int index, BwdIte
   if (w.slice >= w.slices) return false;
   w.begin = w.slice * share;
   w.nt = max(0, min(share, total - w.begin));
+  w.begin_head = w.per_head > 0 ? w.begin / w.per_head : 0;
+  w.begin_tile = w.begin - w.begin_head * w.per_head;
+  w.kind = kDkv ? kItemDkv : kItemDq;
   return true;
 }
 
@@ -367,155 +426,176 @@ struct BwdOut {
   }
 };
 
-// Shared memory, barriers and running counters of a CTA.  Every role keeps
-// its own copy of the counters, advanced alike.
+// Shared memory and barriers of a CTA.
 template <int kDP>
 struct BwdCta {
   using C = BwdCfg<kDP>;
-  uint8_t *sA0, *sA1, *sB;
+  uint8_t *sA0, *sA1, *sB0, *sB1;
   float* sStat;
-  uint64_t *full, *empty, *a_full, *a_empty, *s, *pr, *dp, *ds, *done, *acc_free, *fix, *sched_full, *sched_empty, *clc, *drained;
+  uint64_t *full0, *empty0, *full1, *empty1, *st_full, *st_empty, *a_full, *a_empty, *s, *pr, *dp, *ds, *turn, *done, *acc_free,
+      *fix, *sched_full, *sched_empty, *clc, *drained;
   uint32_t* tmem_slot;
   volatile int* abort_flag;
-  volatile int* next;  // [2]
+  BwdItem* item;  // [2]
   uint32_t clc_resp;
   __device__ __forceinline__ explicit BwdCta(uint8_t* smem) {
     sA0 = smem;
     sA1 = sA0 + C::kABytes;
-    sB = sA1 + C::kABytes;
-    sStat = reinterpret_cast<float*>(sB + C::kRing * C::kBBytes);
-    full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(sStat) + C::kStatBufs * C::kStatBytes);
-    empty = full + C::kRing;
-    a_full = empty + C::kRing;
+    sB0 = sA1 + C::kABytes;
+    sB1 = sB0 + C::kRing0 * C::kBBytes;
+    sStat = reinterpret_cast<float*>(sB1 + C::kRing1 * C::kBBytes);
+    full0 = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(sStat) + 2 * C::kStatBytes);
+    empty0 = full0 + C::kRing0;
+    full1 = empty0 + C::kRing0;
+    empty1 = full1 + C::kRing1;
+    st_full = empty1 + C::kRing1;
+    st_empty = st_full + 2;
+    a_full = st_empty + 2;
     a_empty = a_full + 2;
     s = a_empty + 2;    // S(i) complete
-    pr = s + 1;         // P(i) stored (dK/dV), S(i) read (dQ)
-    dp = pr + 1;        // dP(i) complete
-    ds = dp + 1;        // dS(i) stored
-    done = ds + 1;      // accumulators final
-    acc_free = done + 1;  // accumulators read
-    fix = acc_free + 1;   // ragged tile landed, before its rows are cleared
-    sched_full = fix + 1;
+    pr = s + 1;         // [2] P(i) half stored, stored (dK/dV); [1] S(i) read (dQ)
+    dp = pr + 2;        // dP(i) complete
+    ds = dp + 1;        // [2] dS(i) half stored, stored
+    turn = ds + 2;      // [2] issue order of the two issuers
+    done = turn + 2;    // [2] accumulator final
+    acc_free = done + 2;  // accumulators read
+    fix = acc_free + 1;   // [2] ragged tile landed, before its rows are cleared
+    sched_full = fix + 2;
     sched_empty = sched_full + 2;
     clc = sched_empty + 2;
     drained = clc + 1;
-    tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
+    tmem_slot = reinterpret_cast<uint32_t*>(drained + 2);
     abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    next = reinterpret_cast<volatile int*>(tmem_slot + 2);
-    clc_resp = (smem_u32(tmem_slot + 4) + 15u) & ~15u;
+    clc_resp = (smem_u32(tmem_slot + 2) + 15u) & ~15u;
+    item = reinterpret_cast<BwdItem*>(tmem_slot + 10);
+    static_assert(40 + 2 * sizeof(BwdItem) <= C::kTailBytes, "two items in the tail");
   }
 };
 
+// Running counters; every role keeps its own copy, advanced alike.
 struct BwdCount {
-  int t = 0;      // streamed tiles put into (taken from) the ring
-  int i = 0;      // pairs of them
+  int i = 0;      // streamed tiles, of each operand
   int items = 0;  // items with work
+  int stats = 0;  // statistics tiles (dK/dV items)
+  int fixes = 0;  // ragged tiles cleared
 };
 
-// ---------------------------------------------------------------- producer
-// The whole warp 0 runs this; lane 0 issues the copies.  a0/a1 are the maps
-// of the stationary operands (K and V, or Q and dO), b0/b1 of the streamed
-// ones (Q and dO, or K and V).
-template <typename T, int kDP, bool kDkv>
-__device__ __forceinline__ bool bwd_produce(const FaBwdParams& p, const BwdCta<kDP>& c, const CUtensorMap* a0,
-                                            const CUtensorMap* a1, const CUtensorMap* b0, const CUtensorMap* b1,
-                                            int index, BwdCount& n) {
+// --------------------------------------------------------------- producers
+// kRole 0 (warp 0): the first stationary and streamed operands (K and Q, or Q
+// and K) and the statistics; kRole 1 (warp 3): the second ones (V and dO, or
+// dO and V).  The whole warp runs this; lane 0 issues the copies.
+template <typename T, int kDP, bool kDkv, int kRole>
+__device__ __forceinline__ bool bwd_produce(const FaBwdParams& p, const BwdCta<kDP>& c, const CUtensorMap* map_a,
+                                            const CUtensorMap* map_s, const BwdItem& w, BwdCount& n) {
   using C = BwdCfg<kDP>;
-  constexpr int kBS = C::kBS, kRing = C::kRing;
-  BwdItem w;
-  if (!bwd_item<kDP, kDkv>(p, index, w) || w.nt == 0) return true;
+  constexpr int kBS = C::kBS, kRing = kRole == 0 ? C::kRing0 : C::kRing1;
+  if (w.nt == 0) return true;
   const int lane = threadIdx.x & 31;
   const bool packed = p.cu_q != nullptr;
   const int map_b = packed ? 0 : w.b;
-  const int a_row = (kDkv ? w.k_row0 : w.q_row0) + w.row0;
-#pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    if (!mbar_wait_warp(c.a_empty + x, (n.items & 1) ^ 1, c.abort_flag, kDevTimeoutEmpty)) return false;
-    if (lane == 0) {
-      mbar_arrive_expect_tx(c.a_full + x, C::kABytes);
-      for (int a = 0; a < C::kAtoms; ++a)
-        tma_load_4d((x ? c.sA1 : c.sA0) + a * C::kAAtomBytes, x ? a1 : a0, c.a_full + x, a * 64, a_row, w.h, map_b);
-    }
+  uint64_t* const full = kRole == 0 ? c.full0 : c.full1;
+  uint64_t* const empty = kRole == 0 ? c.empty0 : c.empty1;
+  uint8_t* const ring = kRole == 0 ? c.sB0 : c.sB1;
+  if (!bwd_wait(c.a_empty + kRole, (n.items & 1) ^ 1, c.abort_flag, kDevTimeoutEmpty)) return false;
+  if (lane == 0) {
+    mbar_arrive_expect_tx(c.a_full + kRole, C::kABytes);
+#pragma unroll 1
+    for (int a = 0; a < C::kAtoms; ++a)
+      tma_load_4d((kRole ? c.sA1 : c.sA0) + a * C::kAAtomBytes, map_a, c.a_full + kRole, a * 64,
+                  (kDkv ? w.k_row0 : w.q_row0) + w.row0, w.h, map_b);
   }
-  // What follows reads the statistics kernel's output.
-  if (n.items == 0) {
+  if (kRole == 0 && n.items == 0) {
+    // The statistics kernel's output is read from here on.
     asm volatile("griddepcontrol.wait;" ::: "memory");
     fence_proxy_async_global();
   }
   ++n.items;
-  const int stat_len = kDkv ? w.M : w.N;  // valid streamed rows of the sequence
-  const int row_base = kDkv ? w.q_row0 : w.k_row0;
-  const int h0 = kDkv ? w.h * p.group : w.h / p.group;
-  int g = w.begin / w.per_head, ti = w.begin % w.per_head;
-  for (int x = 0; x < 2 * w.nt; ++x, ++n.t) {
-    const int slot = n.t % kRing;
-    const bool second = (x & 1) != 0;
-    if (!mbar_wait_warp(c.empty + slot, ((n.t / kRing) & 1) ^ 1, c.abort_flag, kDevTimeoutEmpty)) return false;
-    const int tile = w.first + ti;
-    const int rows_left = stat_len - tile * kBS;
-    // A packed sequence's last tile runs into the next sequence's rows.  Rows
-    // of the summed dimension must be zero there (0 x NaN is NaN), so such a
-    // tile is cleared past the end before it is handed on.  V tiles of dQ
-    // items are exempt: they only feed dP columns that are masked.
-    const bool fix = packed && rows_left < kBS && (kDkv || !second);
-    uint8_t* dst = c.sB + slot * C::kBBytes;
+  // A packed sequence's last tile runs into the next sequence's rows.  Rows of
+  // the summed dimension must be zero there (0 x NaN is NaN), so such a tile
+  // is cleared past the end before it is handed on.  V tiles of dQ items are
+  // exempt: they only feed dP columns that are masked.
+  const int len = kDkv ? w.M : w.N;  // valid streamed rows of the sequence
+  const int ragged = packed && (kDkv || kRole == 0) && len % kBS != 0 ? len / kBS - w.first : -1;
+  const int row_first = (kDkv ? w.q_row0 : w.k_row0) + w.first * kBS;
+  int ti = w.begin_tile;
+  int head = (kDkv ? w.h * p.group : w.h / p.group) + w.begin_head;
+  const float* stat = nullptr;
+  if constexpr (kDkv && kRole == 0)
+    stat = p.stats + (bwd_stat_tile0(p, w.b, head, w.q_row0, kBS) + w.first) * (2 * kBS);
+  for (int i = 0; i < w.nt; ++i) {
+    const int slot = n.i % kRing;
+    if (!bwd_wait(empty + slot, ((n.i / kRing) & 1) ^ 1, c.abort_flag, kDevTimeoutEmpty)) return false;
+    ++n.i;
+    uint8_t* dst = ring + slot * C::kBBytes;
+    const bool fix = ti == ragged;
     if (lane == 0) {
-      // A query tile brings its rows' statistics along (same barrier; its
-      // buffer is free when its slot is: both were last used for dK).
-      uint64_t* bar = fix ? c.fix : c.full + slot;
-      const bool stat = kDkv && !second;
-      mbar_arrive_expect_tx(bar, C::kBBytes + (stat ? C::kStatBytes : 0));
-      if (stat)
-        bulk_load_g2s(c.sStat + (n.t / 2) % C::kStatBufs * (2 * kBS),
-                      p.stats + (bwd_stat_tile0(p, w.b, h0 + g, w.q_row0, kBS) + tile) * (2 * kBS), C::kStatBytes, bar);
-      const CUtensorMap* map = second ? b1 : b0;
+      uint64_t* bar = fix ? c.fix + kRole : full + slot;
+      mbar_arrive_expect_tx(bar, C::kBBytes);
+#pragma unroll
       for (int a = 0; a < C::kAtoms; ++a)
-        tma_load_4d(dst + a * C::kBAtomBytes, map, bar, a * 64, row_base + tile * kBS, h0 + g, map_b);
+        tma_load_4d(dst + a * C::kBAtomBytes, map_s, bar, a * 64, row_first + ti * kBS, head, map_b);
+    }
+    if constexpr (kDkv && kRole == 0) {
+      const int b = n.stats & 1;
+      if (!bwd_wait(c.st_empty + b, ((n.stats >> 1) & 1) ^ 1, c.abort_flag, kDevTimeoutEmpty)) return false;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(c.st_full + b, C::kStatBytes);
+        bulk_load_g2s(c.sStat + b * (2 * kBS), stat + ti * (2 * kBS), C::kStatBytes, c.st_full + b);
+      }
+      ++n.stats;
     }
     if (fix) {
-      if (!mbar_wait_warp(c.fix, n.i & 1, c.abort_flag, kDevTimeoutKV)) return false;
-      ++n.i;  // the producer counts cleared tiles here
-      const int chunks = (kBS - rows_left) * 8;  // 16-byte pieces of one atom's rows past the end
+      if (!bwd_wait(c.fix + kRole, n.fixes & 1, c.abort_flag, kDevTimeoutKV)) return false;
+      ++n.fixes;
+      const int rows = len % kBS, chunks = (kBS - rows) * 8;  // 16-byte pieces of one atom's rows past the end
+#pragma unroll 1
       for (int a = 0; a < C::kAtoms; ++a)
+#pragma unroll 1
         for (int k = lane; k < chunks; k += 32)
-          *reinterpret_cast<uint4*>(dst + a * C::kBAtomBytes + rows_left * 128 + k * 16) = make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(dst + a * C::kBAtomBytes + rows * 128 + k * 16) = make_uint4(0, 0, 0, 0);
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(c.full + slot);
+      if (lane == 0) mbar_arrive(full + slot);
     }
-    if (second && ++ti == w.per_head) {
+    if (++ti == w.per_head) {
       ti = 0;
-      ++g;
+      ++head;
+      if constexpr (kDkv && kRole == 0)
+        stat = p.stats + (bwd_stat_tile0(p, w.b, head, w.q_row0, kBS) + w.first) * (2 * kBS);
     }
   }
   return true;
 }
 
-// -------------------------------------------------------------- MMA issuer
-template <typename T, int kDP, bool kDkv>
-__device__ __forceinline__ bool bwd_issue(const FaBwdParams& p, const BwdCta<kDP>& c, uint32_t tmem, bool leader,
-                                          int index, BwdCount& n) {
+// ------------------------------------------------------------- MMA issuers
+// kRole 0 (warp 1): S and dV.  kRole 1 (warp 2): dP and dK or dQ.  A slot of
+// the ring is free when both roles' products that read it are complete.
+template <typename T, int kDP, bool kDkv, int kRole>
+__device__ __forceinline__ bool bwd_issue(const BwdCta<kDP>& c, uint32_t tmem, bool leader, const BwdItem& w,
+                                          BwdCount& n) {
   using C = BwdCfg<kDP>;
-  constexpr int kBS = C::kBS, kRing = C::kRing;
+  constexpr int kBS = C::kBS, kRing0 = C::kRing0, kRing1 = C::kRing1;
   constexpr int kOut = kDkv ? C::kOutDkv : kDP;  // columns of each accumulator
-  BwdItem w;
-  if (!bwd_item<kDP, kDkv>(p, index, w) || w.nt == 0) return true;
+  if (w.nt == 0) return true;
   const int nt = w.nt;
   constexpr uint32_t kFmt = BwdElem<T>::kFmt;
   constexpr uint32_t idesc_s = umma_idesc(kFmt, 128, kBS, 0, 0);
   constexpr uint32_t idesc_o = umma_idesc(kFmt, 128, kOut, 0, 1);
   constexpr uint32_t kHi = umma_desc_hi(1024, kLayoutSw128);
-  const uint32_t a0_lo = umma_desc_lo(smem_u32(c.sA0), 16);
-  const uint32_t a1_lo = umma_desc_lo(smem_u32(c.sA1), 16);
-  const uint32_t b_lo = umma_desc_lo(smem_u32(c.sB), 16);
-  // The same tiles as MN-major operands, from this item's first output column.
-  const uint32_t bn_lo = umma_desc_lo(smem_u32(c.sB) + (w.dcol0 / 64) * C::kBAtomBytes, C::kBAtomBytes);
+  const uint32_t a_lo = umma_desc_lo(smem_u32(kRole == 0 ? c.sA0 : c.sA1), 16);
+  // The streamed operand of the role's first product (S or dP), and, MN-major
+  // from this item's first output column, that of its second.
+  const uint32_t b_lo = umma_desc_lo(smem_u32(kRole == 0 ? c.sB0 : c.sB1), 16);
+  const uint32_t bn_lo = umma_desc_lo(smem_u32(kRole == 0 ? c.sB1 : c.sB0) + (w.dcol0 / 64) * C::kBAtomBytes,
+                                      C::kBAtomBytes);
+  constexpr int kPass = FAB_BWD_PASS;
   auto wait = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
-    return mbar_wait_warp(bar, parity, c.abort_flag, code);
+    return bwd_wait(bar, parity, c.abort_flag, code);
   };
-  // D[128 x kBS] = A (stationary) x B(slot)^T over the head dim.
-  auto issue_s = [&](uint32_t d, uint32_t alo, int s) {
-    uint32_t qa = alo, kb = b_lo + s * (C::kBBytes >> 4);
+  // D[128 x kBS] = A (stationary) x B(slot)^T over the head dim.  `pass`: the
+  // other issuer may go on when this burst is nearly out (see below).
+  auto issue_s = [&](uint32_t d, int s, bool pass) {
+    uint32_t qa = a_lo, kb = b_lo + s * (C::kBBytes >> 4);
     asm volatile("" : "+r"(qa), "+r"(kb));
 #pragma unroll
     for (int kk = 0; kk < kDP / 16; ++kk) {
@@ -523,89 +603,104 @@ __device__ __forceinline__ bool bwd_issue(const FaBwdParams& p, const BwdCta<kDP
       const uint32_t off = (kk & 3) * 32;
       const uint64_t ad = umma_desc_join(qa + ((a * C::kAAtomBytes + off) >> 4), kHi);
       const uint64_t bd = umma_desc_join(kb + ((a * C::kBAtomBytes + off) >> 4), kHi);
+      if (pass && kk == kPass && leader) mbar_arrive(c.turn + kRole);
       if (leader) mma_ss_f16(d, ad, bd, idesc_s, kk > 0 ? 1u : 0u);
     }
   };
   // D[128 x kOut] += A (TMEM, kBS wide) x B(slot).  Each softmax warpgroup's
   // half of A starts at its half of the fp32 columns.
-  auto issue_o = [&](uint32_t d, uint32_t a, int s, bool acc) {
+  // `part` 0 takes the first half of each warpgroup's columns, 1 the rest.
+  auto issue_o = [&](uint32_t d, uint32_t a, int s, bool acc, int part) {
     uint32_t vb = bn_lo + s * (C::kBBytes >> 4);
     asm volatile("" : "+r"(vb));
 #pragma unroll
-    for (int kk = 0; kk < kBS / 16; ++kk) {
+    for (int x = 0; x < kBS / 32; ++x) {
       constexpr int kHalf = kBS / 32;
+      const int kk = x / (kHalf / 2) * kHalf + x % (kHalf / 2) + part * (kHalf / 2);
       const uint32_t at = a + (kk / kHalf) * (kBS / 2) + (kk % kHalf) * 8;
       const uint64_t bd = umma_desc_join(vb + ((kk * 16 * 128) >> 4), kHi);
-      if (leader) mma_ts_f16(d, at, bd, idesc_o, (acc || kk > 0) ? 1u : 0u);
+      if (leader) mma_ts_f16(d, at, bd, idesc_o, (acc || x > 0) ? 1u : 0u);
     }
   };
   auto commit = [&](uint64_t* bar) {
     if (leader) mma_commit(bar);
   };
-  const uint32_t tS = tmem + C::kTmemS, tP = tmem + C::kTmemP;
-  const uint32_t tAcc0 = tmem + C::kTmemAcc, tAcc1 = tAcc0 + kOut;
-  auto slot = [](int t) { return t % kRing; };
-  auto par = [](int t) { return static_cast<uint32_t>((t / kRing) & 1); };
   const uint32_t turn = n.items & 1;
   ++n.items;
+  // This role's buffer, the barriers of its first product and of what the
+  // softmax warps make of it, its rings.
+  const uint32_t tBuf = tmem + (kRole == 0 ? C::kTmemS : C::kTmemP);
+  const uint32_t tAcc = tmem + C::kTmemAcc + (kRole == 0 ? kOut : 0);
+  uint64_t* const ready = kRole == 0 ? c.s : c.dp;
+  uint64_t* const stored = kRole == 0 ? c.pr : c.ds;
+  constexpr int kRingS = kRole == 0 ? kRing0 : kRing1, kRingO = kRole == 0 ? kRing1 : kRing0;
+  uint64_t* const full_s = kRole == 0 ? c.full0 : c.full1;
+  uint64_t* const empty_s = kRole == 0 ? c.empty0 : c.empty1;
+  uint64_t* const full_o = kRole == 0 ? c.full1 : c.full0;
+  uint64_t* const empty_o = kRole == 0 ? c.empty1 : c.empty0;
+  constexpr bool kSum = kRole == 1 || kDkv;  // has a second product: dV, dK or dQ
+  auto wait_s = [&](int i) { return wait(full_s + i % kRingS, (i / kRingS) & 1, kDevTimeoutKV); };
+  // The first product of streamed tile i, and what its completion frees: a
+  // slot counts two releases, one by each role, except that V tiles of dQ
+  // items are read by role 1 alone, which gives both.
+  auto first_product = [&](int i, bool last, bool pass) {
+    issue_s(tBuf, i % kRingS, pass);
+    commit(ready);
+    commit(empty_s + i % kRingS);
+    if (kRole == 1 && !kDkv) commit(empty_s + i % kRingS);
+    if (last) commit(c.a_empty + kRole);
+  };
 
-  // The previous item's last products are queued ahead: S and dP of this one
-  // overwrite buffers whose contents those read, in issue order.
-  if (!wait(c.a_full, turn, kDevTimeoutQ) || !wait(c.full + slot(n.t), par(n.t), kDevTimeoutKV)) return false;
+  // It needs no wait for the previous item's last products: it overwrites a
+  // buffer that those read, in issue order.
+  if (!wait(c.a_full + kRole, turn, kDevTimeoutQ) || !wait_s(n.i)) return false;
   tc_fence_after();
-  issue_s(tS, a0_lo, slot(n.t));
-  commit(c.s);
-  if (nt == 1) commit(c.a_empty);
-  if (!wait(c.a_full + 1, turn, kDevTimeoutQ) || !wait(c.full + slot(n.t + 1), par(n.t + 1), kDevTimeoutKV)) return false;
-  tc_fence_after();
-  issue_s(tP, a1_lo, slot(n.t + 1));
-  commit(c.dp);
-  if (nt == 1) commit(c.a_empty + 1);
-  if constexpr (!kDkv) commit(c.empty + slot(n.t + 1));
-  for (int i = 0; i < nt; ++i, ++n.i, n.t += 2) {
-    const int t0 = n.t, t1 = n.t + 1;
-    if (!wait(c.pr, n.i & 1, kDevTimeoutP)) return false;
-    // The first product into the accumulators waits until the previous item's
+  first_product(n.i, nt == 1, false);
+  for (int i = 0; i < nt; ++i, ++n.i) {
+    const bool more = i + 1 < nt;
+    // All waits come before the burst, so that its products go out together.
+    // (With one slot the tile of the next dP lands where the last one was,
+    // after this burst's first half: there it is waited for in between.)
+    constexpr bool kOneBurst = kRingS > 1;
+    if (kSum && !wait(full_o + n.i % kRingO, (n.i / kRingO) & 1, kDevTimeoutKV)) return false;
+    // The first product into an accumulator waits until the previous item's
     // sums have been read.
     if (i == 0 && !wait(c.acc_free, turn ^ 1, kDevTimeoutAcc)) return false;
-    tc_fence_after();
-    if constexpr (kDkv) {
-      issue_o(tAcc1, tS, slot(t1), i > 0);
-      commit(c.empty + slot(t1));
-    }
-    if (i + 1 < nt) {
-      if (!wait(c.full + slot(t0 + 2), par(t0 + 2), kDevTimeoutKV)) return false;
+    if (kOneBurst && more && !wait_s(n.i + 1)) return false;
+    // Bursts alternate between the issuers: role 0's i-th, role 1's i-th.
+    if (FAB_BWD_TURNS && !wait(c.turn + (kRole ^ 1), kRole == 0 ? (n.i & 1) ^ 1 : n.i & 1, kDevTimeoutP)) return false;
+    if (kSum && C::kHalves) {
+      if (!wait(stored, n.i & 1, kDevTimeoutP)) return false;
       tc_fence_after();
-      issue_s(tS, a0_lo, slot(t0 + 2));
-      commit(c.s);
-      if (i + 2 == nt) commit(c.a_empty);
+      issue_o(tAcc, tBuf, n.i % kRingO, i > 0, 0);
     }
-    if (!wait(c.ds, n.i & 1, kDevTimeoutP)) return false;
+    if (!wait(stored + 1, n.i & 1, kDevTimeoutP)) return false;
     tc_fence_after();
-    issue_o(tAcc0, tP, slot(t0), i > 0);
-    commit(c.empty + slot(t0));
-    if (i + 1 < nt) {
-      if (!wait(c.full + slot(t1 + 2), par(t1 + 2), kDevTimeoutKV)) return false;
-      tc_fence_after();
-      issue_s(tP, a1_lo, slot(t1 + 2));
-      commit(c.dp);
-      if (i + 2 == nt) commit(c.a_empty + 1);
-      if constexpr (!kDkv) commit(c.empty + slot(t1 + 2));
+    if (kSum) {
+      if (!C::kHalves) issue_o(tAcc, tBuf, n.i % kRingO, i > 0, 0);
+      issue_o(tAcc, tBuf, n.i % kRingO, true, 1);
+      commit(empty_o + n.i % kRingO);
+    }
+    if (!more && leader) mbar_arrive(c.turn + kRole);
+    if (more) {
+      if constexpr (!kOneBurst) {
+        if (!wait_s(n.i + 1)) return false;
+        tc_fence_after();
+      }
+      first_product(n.i + 1, i + 2 == nt, true);
     }
   }
-  commit(c.done);
+  commit(c.done + (kRole ^ 1));
   return true;
 }
 
 // ----------------------------------------------------------------- softmax
 template <typename T, int kDP, bool kDkv>
-__device__ __forceinline__ bool bwd_softmax(const FaBwdParams& p, const BwdCta<kDP>& c, uint32_t tmem, int index,
-                                            BwdCount& n) {
+__device__ __forceinline__ bool bwd_softmax(const FaBwdParams& p, const BwdCta<kDP>& c, uint32_t tmem,
+                                            const BwdItem& w, BwdCount& n) {
   using C = BwdCfg<kDP>;
-  constexpr int kBS = C::kBS, kRing = C::kRing;
+  constexpr int kBS = C::kBS;
   using Out = BwdOut<T, kDP, kDkv>;
-  BwdItem w;
-  if (!bwd_item<kDP, kDkv>(p, index, w)) return true;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int half = (warp - 4) >> 2;
   const int wq = warp & 3;
@@ -649,41 +744,47 @@ __device__ __forceinline__ bool bwd_softmax(const FaBwdParams& p, const BwdCta<k
   // not visible; `pos0` is the position of its first column.
   auto step = [&](auto masked, int pos0) -> bool {
     constexpr bool kMasked = decltype(masked)::value;
-    [[maybe_unused]] const float* st = c.sStat + n.i % C::kStatBufs * (2 * kBS) + half * kCols;
+    [[maybe_unused]] const float* st = c.sStat + (n.stats & 1) * (2 * kBS) + half * kCols;
     // Visible columns [lo, hi) of this lane.
     const int lo = kMasked && kDkv ? my - pos0 : 0;
     const int hi = kMasked && !kDkv ? (p.causal ? min(N, my + 1) : N) - pos0 : kCols;
     if constexpr (kDkv) {
-      // The statistics land with the query tile; S(i) implies it, but only
-      // this wait orders the copy before this thread's reads.
-      if (!mbar_wait_warp(c.full + (2 * n.i) % kRing, ((2 * n.i) / kRing) & 1, c.abort_flag, kDevTimeoutKV)) return false;
+      if (!bwd_wait(c.st_full + (n.stats & 1), (n.stats >> 1) & 1, c.abort_flag, kDevTimeoutKV)) return false;
     }
-    if (!mbar_wait_warp(c.s, n.i & 1, c.abort_flag, kDevTimeoutS)) return false;
+    if (!bwd_wait(c.s, n.i & 1, c.abort_flag, kDevTimeoutS)) return false;
     tc_fence_after();
+    // Chunks of 32 columns; the next one's load is under way while one is
+    // worked on.
+    constexpr int kChunks = kCols / 32;
     float pr[kCols];
-    {
-      uint32_t rr[kCols / 32][32];
+    uint32_t rr[kChunks][32];
+    tmem_ld32(tS, rr[0]);
 #pragma unroll
-      for (int cc = 0; cc < kCols / 32; ++cc) tmem_ld32(tS + cc * 32, rr[cc]);
+    for (int cc = 0; cc < kChunks; ++cc) {
       tmem_wait_ld();
-#pragma unroll
-      for (int x = 0; x < kCols; ++x) pr[x] = __uint_as_float(rr[x / 32][x % 32]);
-    }
-    if constexpr (!kDkv) {
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(c.pr);
-    }
-#pragma unroll
-    for (int cc = 0; cc < kCols / 32; ++cc) {
+      if (cc + 1 < kChunks) tmem_ld32(tS + (cc + 1) * 32, rr[cc + 1]);
+      if (!kDkv && cc + 1 == kChunks) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(c.pr + 1);
+      }
+      // The first half of P is handed on while the second is worked out.
+      if (kDkv && C::kHalves && cc == 1) {
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(c.pr);
+      }
       [[maybe_unused]] uint32_t pk[16];
 #pragma unroll
       for (int e = 0; e < 32; e += 4) {
         const int x = cc * 32 + e;
         float4 nl = make_float4(row_nl, row_nl, row_nl, row_nl);
         if constexpr (kDkv) nl = *reinterpret_cast<const float4*>(st + x);
-        const float2 a = __ffma2_rn(make_float2(pr[x], pr[x + 1]), c2, make_float2(nl.x, nl.y));
-        const float2 d = __ffma2_rn(make_float2(pr[x + 2], pr[x + 3]), c2, make_float2(nl.z, nl.w));
+        const float2 a = __ffma2_rn(make_float2(__uint_as_float(rr[cc][e]), __uint_as_float(rr[cc][e + 1])), c2,
+                                    make_float2(nl.x, nl.y));
+        const float2 d = __ffma2_rn(make_float2(__uint_as_float(rr[cc][e + 2]), __uint_as_float(rr[cc][e + 3])), c2,
+                                    make_float2(nl.z, nl.w));
         pr[x] = ex2_approx(a.x);
         pr[x + 1] = ex2_approx(a.y);
         pr[x + 2] = ex2_approx(d.x);
@@ -698,22 +799,28 @@ __device__ __forceinline__ bool bwd_softmax(const FaBwdParams& p, const BwdCta<k
           pk[e / 2 + 1] = BwdElem<T>::pack2(pr[x + 2], pr[x + 3]);
         }
       }
+      // P of 32 columns takes 16 of them: columns that are in registers.
       if constexpr (kDkv) tmem_st16(tS + cc * 16, pk);
     }
     if constexpr (kDkv) {
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(c.pr);
+      if (lane == 0) mbar_arrive(c.pr + 1);
     }
-    if (!mbar_wait_warp(c.dp, n.i & 1, c.abort_flag, kDevTimeoutS)) return false;
+    if (!bwd_wait(c.dp, n.i & 1, c.abort_flag, kDevTimeoutS)) return false;
     tc_fence_after();
-    uint32_t rr[kCols / 32][32];
+    tmem_ld32(tP, rr[0]);
 #pragma unroll
-    for (int cc = 0; cc < kCols / 32; ++cc) tmem_ld32(tP + cc * 32, rr[cc]);
-    tmem_wait_ld();
-#pragma unroll
-    for (int cc = 0; cc < kCols / 32; ++cc) {
+    for (int cc = 0; cc < kChunks; ++cc) {
+      tmem_wait_ld();
+      if (cc + 1 < kChunks) tmem_ld32(tP + (cc + 1) * 32, rr[cc + 1]);
+      if (C::kHalves && cc == 1) {
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(c.ds);
+      }
       [[maybe_unused]] uint32_t pk[16];
 #pragma unroll
       for (int e = 0; e < 32; e += 4) {
@@ -745,10 +852,14 @@ __device__ __forceinline__ bool bwd_softmax(const FaBwdParams& p, const BwdCta<k
     tmem_wait_st();
     tc_fence_before();
     __syncwarp();
-    if (lane == 0) mbar_arrive(c.ds);
+    if (lane == 0) {
+      mbar_arrive(c.ds + 1);
+      if constexpr (kDkv) mbar_arrive(c.st_empty + (n.stats & 1));
+    }
+    if constexpr (kDkv) ++n.stats;
     return true;
   };
-  int ti = w.nt > 0 ? w.begin % w.per_head : 0;
+  int ti = w.begin_tile;
   for (int i = 0; i < nt; ++i) {
     // Streamed rows of this tile: query positions (dK/dV) or key positions.
     const int pos0 = (w.first + ti) * kBS + half * kCols;
@@ -764,7 +875,7 @@ __device__ __forceinline__ bool bwd_softmax(const FaBwdParams& p, const BwdCta<k
 
   // -------------------------------------------------------------- epilogue
   if (nt > 0) {
-    if (!mbar_wait_warp(c.done, n.items & 1, c.abort_flag, kDevTimeoutO)) return false;
+    if (!bwd_wait(c.done + (kDkv ? half : 0), n.items & 1, c.abort_flag, kDevTimeoutO)) return false;
     tc_fence_after();
     ++n.items;
   }
@@ -814,31 +925,42 @@ __global__ void __launch_bounds__(384, 1)
                   const __grid_constant__ CUtensorMap g_a, const __grid_constant__ CUtensorMap k_b,
                   const __grid_constant__ CUtensorMap v_b) {
   using C = BwdCfg<kDP>;
-  extern __shared__ uint8_t smem_raw[];
-  const uint32_t raw = smem_u32(smem_raw);
-  const BwdCta<kDP> c(smem_raw + ((1024u - (raw & 1023u)) & 1023u));
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const BwdCta<kDP> c(smem_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < C::kRing; ++s) {
-      mbar_init(c.full + s, 1);
-      mbar_init(c.empty + s, 1);
+    for (int s = 0; s < C::kRing0; ++s) {
+      mbar_init(c.full0 + s, 1);
+      mbar_init(c.empty0 + s, 2);  // both issuers
+    }
+    for (int s = 0; s < C::kRing1; ++s) {
+      mbar_init(c.full1 + s, 1);
+      mbar_init(c.empty1 + s, 2);
     }
     for (int x = 0; x < 2; ++x) {
       mbar_init(c.a_full + x, 1);
       mbar_init(c.a_empty + x, 1);
       mbar_init(c.sched_full + x, 1);
-      mbar_init(c.sched_empty + x, 9);  // the issuer and the eight softmax warps
+      mbar_init(c.sched_empty + x, 11);  // every warp but warp 0
+      mbar_init(c.pr + x, 8);  // one arrival per softmax warp
+      mbar_init(c.ds + x, 8);
+      mbar_init(c.turn + x, 1);
+      mbar_init(c.st_full + x, 1);
+      mbar_init(c.st_empty + x, 8);
+      mbar_init(c.fix + x, 1);
+      mbar_init(c.done + x, 1);
+      mbar_init(c.drained + x, 1);
     }
     mbar_init(c.s, 1);
-    mbar_init(c.pr, 8);  // one arrival per softmax warp
     mbar_init(c.dp, 1);
-    mbar_init(c.ds, 8);
-    mbar_init(c.done, 1);
     mbar_init(c.acc_free, 8);
-    mbar_init(c.fix, 1);
     mbar_init(c.clc, 1);
-    mbar_init(c.drained, 1);
-    *c.abort_flag = *reinterpret_cast<volatile int*>(&g_fab_device_error) != 0 ? 1 : 0;
+    *c.abort_flag = *reinterpret_cast<volatile int*>(&g_fab_device_error) != 0 ? -1 : 0;
+    // The swizzled tiles need the base that the alignment above asks for.
+    if (smem_u32(smem_raw) & 1023u) {
+      record_device_error(kDevTimeoutTeardown);
+      *c.abort_flag = -1;
+    }
     mbar_fence_init();
   }
   if (warp == 1) {
@@ -850,77 +972,120 @@ __global__ void __launch_bounds__(384, 1)
   tc_fence_after();
   const uint32_t tmem = *c.tmem_slot;
   const bool skip = *c.abort_flag != 0;
-  // The item after the q-th, for the issuer and the softmax warps; -1: none.
-  auto next_item = [&](int q) -> int {
-    if (!mbar_wait_warp(c.sched_full + (q & 1), (q >> 1) & 1, c.abort_flag, kDevTimeoutSched)) return -1;
-    const int x = c.next[q & 1];
+  // The q-th item, for every warp but warp 0, which posts them.
+  auto get_item = [&](int q, BwdItem& w) {
+    w.kind = kItemEnd;
+    if (!bwd_wait(c.sched_full + (q & 1), (q >> 1) & 1, c.abort_flag, kDevTimeoutSched)) return;
+    w = c.item[q & 1];
     __syncwarp();
     if (lane == 0) mbar_arrive(c.sched_empty + (q & 1));
-    return x;
   };
 
   // Each warpgroup re-splits its registers first, whatever it does after.
   if (warp < 4) {
     setmaxnreg_dec<C::kLoadRegs>();
+    // No copy may still be landing when a producer leaves.
+    auto landed = [&](const BwdCount& n, uint64_t* a_full, uint64_t* full, int ring, bool with_stats) {
+      volatile int no_abort = 0;
+      if (lane == 0) {
+        if (n.items > 0) mbar_wait(a_full, (n.items - 1) & 1, &no_abort, kDevTimeoutTeardown);
+        for (int x = max(0, n.i - ring); x < n.i; ++x)
+          mbar_wait(full + x % ring, (x / ring) & 1, &no_abort, kDevTimeoutTeardown);
+        for (int x = max(0, n.stats - 2); with_stats && x < n.stats; ++x)
+          mbar_wait(c.st_full + (x & 1), (x >> 1) & 1, &no_abort, kDevTimeoutTeardown);
+      }
+      __syncwarp();
+    };
     if (warp == 0 && !skip) {
       BwdCount n;
       volatile int no_abort = 0;
       int index = static_cast<int>(blockIdx.x);
-      for (int q = 0; index >= 0; ++q) {
-        const bool ok = index < p.num_dkv
-                            ? bwd_produce<T, kDP, true>(p, c, &k_a, &v_a, &q_b, &g_b, index, n)
-                            : bwd_produce<T, kDP, false>(p, c, &q_a, &g_a, &k_b, &v_b, index - p.num_dkv, n);
-        if (!ok) break;
-        // All of this item's loads are under way: ask for the next one.
-        if (q >= 2 && !mbar_wait_warp(c.sched_empty + (q & 1), ((q - 2) >> 1) & 1, c.abort_flag, kDevTimeoutSched)) break;
+      int asked = 0;
+      auto ask = [&]() -> int {
         int x = -1;
         if (lane == 0) {
           mbar_arrive_expect_tx(c.clc, 16);
           clc_try_cancel(c.clc_resp, c.clc);
-          if (mbar_wait(c.clc, q & 1, &no_abort, kDevTimeoutSched)) x = clc_first_cta_x(c.clc_resp);
-          c.next[q & 1] = x;
+          if (mbar_wait(c.clc, asked & 1, &no_abort, kDevTimeoutSched)) x = clc_first_cta_x(c.clc_resp);
+        }
+        ++asked;
+        return __shfl_sync(0xffffffffu, x, 0);
+      };
+      for (int q = 0;; ++q) {
+        // The next item that exists: this block's, then the scheduler's.
+        BwdItem w;
+        bool found = false;
+        while (index >= 0 && !found) {
+          found = index < p.num_dkv ? bwd_item<kDP, true>(p, index, w) : bwd_item<kDP, false>(p, index - p.num_dkv, w);
+          if (!found) index = ask();
+        }
+        if (!found) w.kind = kItemEnd;
+        // Whatever is posted, the slot's last item must have been read.
+        if (q >= 2 && !bwd_wait(c.sched_empty + (q & 1), ((q - 2) >> 1) & 1, c.abort_flag, kDevTimeoutSched)) break;
+        if (lane == 0) {
+          c.item[q & 1] = w;
           mbar_arrive(c.sched_full + (q & 1));
         }
-        index = __shfl_sync(0xffffffffu, x, 0);
+        if (w.kind == kItemEnd) break;
+        if (!(w.kind == kItemDkv ? bwd_produce<T, kDP, true, 0>(p, c, &k_a, &q_b, w, n)
+                                 : bwd_produce<T, kDP, false, 0>(p, c, &q_a, &k_b, w, n)))
+          break;
+        // All of this item's loads are under way: time to ask for the next.
+        index = ask();
       }
-      // No copy may still be landing when the CTA leaves.
-      if (lane == 0) {
-        for (int x = 0; x < 2; ++x)
-          if (n.items > 0) mbar_wait(c.a_full + x, (n.items - 1) & 1, &no_abort, kDevTimeoutTeardown);
-        for (int x = max(0, n.t - C::kRing); x < n.t; ++x)
-          mbar_wait(c.full + (x % C::kRing), (x / C::kRing) & 1, &no_abort, kDevTimeoutTeardown);
-      }
-      __syncwarp();
-    } else if (warp == 1 && !skip) {
-      const bool leader = elect_one();
+      landed(n, c.a_full, c.full0, C::kRing0, true);
+    } else if (warp == 3 && !skip) {
       BwdCount n;
-      int index = static_cast<int>(blockIdx.x);
-      for (int q = 0; index >= 0; ++q) {
-        const bool ok = index < p.num_dkv ? bwd_issue<T, kDP, true>(p, c, tmem, leader, index, n)
-                                          : bwd_issue<T, kDP, false>(p, c, tmem, leader, index - p.num_dkv, n);
-        if (!ok) break;
-        index = next_item(q);
+      BwdItem w;
+      for (int q = 0;; ++q) {
+        get_item(q, w);
+        if (w.kind == kItemEnd) break;
+        if (!(w.kind == kItemDkv ? bwd_produce<T, kDP, true, 1>(p, c, &v_a, &g_b, w, n)
+                                 : bwd_produce<T, kDP, false, 1>(p, c, &g_a, &v_b, w, n)))
+          break;
       }
-      // Drain the tensor pipe before TMEM is released.
-      if (leader) mma_commit(c.drained);
-      volatile int no_abort = 0;
-      mbar_wait_warp(c.drained, 0, &no_abort, kDevTimeoutTeardown);
+      landed(n, c.a_full + 1, c.full1, C::kRing1, false);
+    } else if ((warp == 1 || warp == 2) && !skip) {
+      const bool leader = elect_one();
+      auto issue = [&](auto role) {
+        constexpr int kRole = decltype(role)::value;
+        BwdCount n;
+        BwdItem w;
+        for (int q = 0;; ++q) {
+          get_item(q, w);
+          if (w.kind == kItemEnd) break;
+          if (!(w.kind == kItemDkv ? bwd_issue<T, kDP, true, kRole>(c, tmem, leader, w, n)
+                                   : bwd_issue<T, kDP, false, kRole>(c, tmem, leader, w, n)))
+            break;
+        }
+        // Drain the tensor pipe before TMEM is released.
+        if (leader) mma_commit(c.drained + kRole);
+        volatile int no_abort = 0;
+        mbar_wait_warp(c.drained + kRole, 0, &no_abort, kDevTimeoutTeardown);
+      };
+      if (warp == 1)
+        issue(std::integral_constant<int, 0>{});
+      else
+        issue(std::integral_constant<int, 1>{});
     }
   } else {
     setmaxnreg_inc<C::kSoftmaxRegs>();
     if (!skip) {
       asm volatile("griddepcontrol.wait;" ::: "memory");  // the statistics
       BwdCount n;
-      int index = static_cast<int>(blockIdx.x);
-      for (int q = 0; index >= 0; ++q) {
-        const bool ok = index < p.num_dkv ? bwd_softmax<T, kDP, true>(p, c, tmem, index, n)
-                                          : bwd_softmax<T, kDP, false>(p, c, tmem, index - p.num_dkv, n);
-        if (!ok) break;
-        index = next_item(q);
+      BwdItem w;
+      for (int q = 0;; ++q) {
+        get_item(q, w);
+        if (w.kind == kItemEnd) break;
+        if (!(w.kind == kItemDkv ? bwd_softmax<T, kDP, true>(p, c, tmem, w, n) : bwd_softmax<T, kDP, false>(p, c, tmem, w, n)))
+          break;
       }
     }
   }
 
+  // A warp that gave up left its code.
+  __syncthreads();
+  if (threadIdx.x == 0 && *c.abort_flag > 0) record_device_error(*c.abort_flag);
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
