@@ -248,10 +248,10 @@ int launch(const fab_attention_bwd_params* p, FaBwdParams& kp, cudaStream_t stre
     }
     if (kp.dkv_slices > 1)
       fa_bwd_join_kernel<T, kDP, true>
-          <<<dim3(static_cast<unsigned>(dkv_tiles), BwdOut<T, kDP, true>::kCols / 32), 256, 0, stream>>>(kp);
+          <<<dim3(static_cast<unsigned>(dkv_tiles), C::kOutDkv / 32), 256, 0, stream>>>(kp);
     if (kp.dq_slices > 1)
       fa_bwd_join_kernel<T, kDP, false>
-          <<<dim3(static_cast<unsigned>(dq_tiles), BwdOut<T, kDP, false>::kCols / 32), 256, 0, stream>>>(kp);
+          <<<dim3(static_cast<unsigned>(dq_tiles), kDP / 64), 256, 0, stream>>>(kp);
   }
   return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
 }
@@ -332,7 +332,9 @@ int fab_attention_bwd(const fab_attention_bwd_params* p, void* stream) {
   kp.D = p->head_dim;
   kp.group = p->heads_q / p->heads_kv;
   kp.scale = p->sm_scale;
-  kp.scale_log2 = p->sm_scale * 1.4426950408889634f;
+  // A scale of zero keeps its zero in dq and dk; inside the exponential a
+  // vanishing one does the same and keeps masked scores masked.
+  kp.scale_log2 = (p->sm_scale == 0.f ? 1e-30f : p->sm_scale) * 1.4426950408889634f;
   kp.causal = p->causal ? 1 : 0;
   kp.cu_q = p->cu_seqlens_q;
   kp.cu_k = p->cu_seqlens_k;

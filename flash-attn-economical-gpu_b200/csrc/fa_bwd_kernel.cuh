@@ -120,7 +120,7 @@ struct BwdCfg {
   // S, P x 2, dP, dS x 2; issue order x 2; accumulators final x 2 and read; ragged tile x 2; next item
   // full/empty x 2; its request; teardown x 2.
   static constexpr int kNumBars = 2 * (kRing0 + kRing1) + 4 + 4 + 6 + 3 + 2 + 4 + 3 + 2;
-  static constexpr int kTailBytes = 208;  // TMEM address, abort flag, two items, the scheduler's response
+  static constexpr int kTailBytes = 208;  // TMEM address, abort flag, a zero word, two items, the scheduler's response
   static constexpr int kSmemBytes =
       2 * kABytes + (kRing0 + kRing1) * kBBytes + 2 * kStatBytes + kNumBars * 8 + kTailBytes;
   // P and dS are handed to the tensor core in two halves where a warp works
@@ -269,21 +269,48 @@ __global__ void __launch_bounds__(256) fa_bwd_stats_kernel(const FaBwdParams p) 
   }
 }
 
-// 32 fp32 values as part of an output row (16-byte aligned).
+// A 32-column chunk of a warp's 32 output rows: lane r brings row r's values,
+// packed.  Storing them as they lie would touch 32 lines per instruction; four
+// lanes exchange their 16-byte pieces first (a 4 x 4 transpose in two steps),
+// so that they store 64 consecutive bytes of one row at a time: 8 lines per
+// instruction (measured: 5400 cycles per 128 x 256 tile before, see below for
+// now).  `row` is this warp's first row at the chunk's first column; `rows`
+// and `cols` say how much of the chunk exists.  16-byte aligned rows.
 template <typename T>
-__device__ __forceinline__ void bwd_store32(T* dst, const float (&v)[32], int ncols) {
-  uint32_t w[16];
+__device__ __forceinline__ void bwd_store_chunk(T* row, int64_t stride, int rows, int cols, const uint32_t (&w)[16]) {
+  const int lane = threadIdx.x & 31;
+  const bool odd = lane & 1, high = lane & 2;
+  uint32_t t[16], u[16];
 #pragma unroll
-  for (int e = 0; e < 16; ++e) w[e] = BwdElem<T>::pack2(v[2 * e], v[2 * e + 1]);
-  if (ncols >= 32) {
-    uint4* d4 = reinterpret_cast<uint4*>(dst);
+  for (int e = 0; e < 4; ++e) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) d4[e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
-  } else {
-    uint16_t* d1 = reinterpret_cast<uint16_t*>(dst);
+    for (int h = 0; h < 16; h += 8) {
+      const uint32_t other = __shfl_xor_sync(0xffffffffu, odd ? w[h + e] : w[h + 4 + e], 1);
+      t[h + e] = odd ? other : w[h + e];
+      t[h + 4 + e] = odd ? w[h + 4 + e] : other;
+    }
+  }
 #pragma unroll
-    for (int e = 0; e < 32; ++e)
-      if (e < ncols) d1[e] = static_cast<uint16_t>((e & 1) ? w[e / 2] >> 16 : w[e / 2] & 0xFFFFu);
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, high ? t[e] : t[8 + e], 2);
+    u[e] = high ? other : t[e];
+    u[8 + e] = high ? t[8 + e] : other;
+  }
+  // u holds piece lane % 4 of the four rows of this group of lanes.
+  const int col = (lane & 3) * 8;
+  T* dst = row + (lane & ~3) * stride + col;
+#pragma unroll
+  for (int i = 0; i < 4; ++i, dst += stride) {
+    if ((lane & ~3) + i >= rows) continue;
+    if (col + 8 <= cols) {
+      *reinterpret_cast<uint4*>(dst) = make_uint4(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (col + e < cols)
+          reinterpret_cast<uint16_t*>(dst)[e] =
+              static_cast<uint16_t>((e & 1) ? u[4 * i + e / 2] >> 16 : u[4 * i + e / 2] & 0xFFFFu);
+    }
   }
 }
 
@@ -399,30 +426,41 @@ __device__ __forceinline__ int64_t bwd_part_slot(const FaBwdParams& p, const Bwd
   }
 }
 
-// Where thread (half, row r) writes: dK/dV items: warpgroup 0 dK, 1 dV; dQ
-// items: each half of the columns.
-template <typename T, int kDP, bool kDkv>
+// Where warp (half, rows wq * 32 ...) writes: dK/dV items: warpgroup 0 dK, 1
+// dV; dQ items: each half of the columns.
+template <typename T, int kDP>
 struct BwdOut {
-  static constexpr int kOut = kDkv ? BwdCfg<kDP>::kOutDkv : kDP;
-  static constexpr int kCols = kDkv ? kOut : kOut / 2;  // columns of one thread
-  T* row;     // the output row
-  float* part;  // this thread's column 0 of the slice's sums
-  int col0;   // its first column
-  bool row_ok;
-  __device__ __forceinline__ BwdOut(const FaBwdParams& p, const BwdItem& w, int half, int r) {
-    const int my = w.row0 + r;
-    row_ok = my < (kDkv ? w.N : w.M);
-    if constexpr (kDkv) {
-      const bool is_v = half == 1;
-      const int64_t ss = is_v ? p.dv_ss : p.dk_ss, sh = is_v ? p.dv_sh : p.dk_sh, sb = is_v ? p.dv_sb : p.dk_sb;
-      row = reinterpret_cast<T*>(is_v ? p.dv : p.dk) + (p.cu_k ? w.k_row0 * ss : w.b * sb) + w.h * sh + my * ss;
-      col0 = w.dcol0;
-      part = p.dkv_part + (bwd_part_slot<kDP, true>(p, w) * 2 + half) * (kOut * 128) + r;
-    } else {
-      row = reinterpret_cast<T*>(p.dq) + (p.cu_q ? w.q_row0 * p.dq_ss : w.b * p.dq_sb) + w.h * p.dq_sh + my * p.dq_ss;
-      col0 = half * kCols;
-      part = p.dq_part + bwd_part_slot<kDP, false>(p, w) * (kOut * 128) + col0 * 128 + r;
-    }
+  T* row;          // the warp's first output row
+  int64_t stride;  // between rows
+  int rows;        // of the warp's 32 that exist
+  int col0, cols;  // its columns of the row
+  int acc;         // its first accumulator column
+  float* part;     // this lane's column 0 of the slice's sums
+  int64_t slot;    // floats between slices
+  __device__ __forceinline__ BwdOut(const FaBwdParams& p, const BwdItem& w, int half, int wq) {
+    constexpr int kOutDkv = BwdCfg<kDP>::kOutDkv;
+    const int r0 = wq * 32, my = w.row0 + r0;
+    const bool dkv = w.kind == kItemDkv, is_v = half == 1;
+    rows = (dkv ? w.N : w.M) - my;
+    stride = !dkv ? p.dq_ss : is_v ? p.dv_ss : p.dk_ss;
+    const int64_t sh = !dkv ? p.dq_sh : is_v ? p.dv_sh : p.dk_sh, sb = !dkv ? p.dq_sb : is_v ? p.dv_sb : p.dk_sb;
+    const int64_t seq = p.cu_q != nullptr ? (dkv ? w.k_row0 : w.q_row0) * stride : w.b * sb;
+    row = reinterpret_cast<T*>(!dkv ? p.dq : is_v ? p.dv : p.dk) + seq + w.h * sh + my * stride;
+    cols = dkv ? kOutDkv : kDP / 2;
+    col0 = dkv ? w.dcol0 : half * cols;
+    acc = half * cols;
+    slot = dkv ? 2 * kOutDkv * 128 : kDP * 128;
+    part = (dkv ? p.dkv_part + bwd_part_slot<kDP, true>(p, w) * slot : p.dq_part + bwd_part_slot<kDP, false>(p, w) * slot) +
+           acc * 128 + r0 + (threadIdx.x & 31);
+  }
+  // 32 columns from the thread's column cc on.
+  __device__ __forceinline__ void store(int cc, const float (&v)[32], int head_dim) const {
+    const int left = head_dim - col0 - cc;
+    if (rows <= 0 || left <= 0) return;
+    uint32_t w[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) w[e] = BwdElem<T>::pack2(v[2 * e], v[2 * e + 1]);
+    bwd_store_chunk<T>(row + col0 + cc, stride, rows, left, w);
   }
 };
 
@@ -466,87 +504,105 @@ struct BwdCta {
     drained = clc + 1;
     tmem_slot = reinterpret_cast<uint32_t*>(drained + 2);
     abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    clc_resp = (smem_u32(tmem_slot + 2) + 15u) & ~15u;
-    item = reinterpret_cast<BwdItem*>(tmem_slot + 10);
-    static_assert(40 + 2 * sizeof(BwdItem) <= C::kTailBytes, "two items in the tail");
+    clc_resp = (smem_u32(tmem_slot + 3) + 15u) & ~15u;
+    item = reinterpret_cast<BwdItem*>(tmem_slot + 11);
+    static_assert(44 + 2 * sizeof(BwdItem) <= C::kTailBytes, "two items in the tail");
   }
 };
 
-// Running counters; every role keeps its own copy, advanced alike.
-struct BwdCount {
-  int i = 0;      // streamed tiles, of each operand
-  int items = 0;  // items with work
-  int stats = 0;  // statistics tiles (dK/dV items)
-  int fixes = 0;  // ragged tiles cleared
+// A position in a ring (or in a barrier's phases, with one slot).
+struct BwdPos {
+  int slot = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next(int size) {
+    if (++slot == size) {
+      slot = 0;
+      phase ^= 1;
+    }
+  }
 };
+
+// The roles below run one copy of their code each, whatever the item's kind
+// and whichever of their two warps they are: with a copy for every
+// combination the kernel was four times the size, and items of a few tiles
+// spent most of their time fetching instructions.
 
 // --------------------------------------------------------------- producers
-// kRole 0 (warp 0): the first stationary and streamed operands (K and Q, or Q
-// and K) and the statistics; kRole 1 (warp 3): the second ones (V and dO, or
+// Role 0 (warp 0): the first stationary and streamed operands (K and Q, or Q
+// and K) and the statistics; role 1 (warp 3): the second ones (V and dO, or
 // dO and V).  The whole warp runs this; lane 0 issues the copies.
-template <typename T, int kDP, bool kDkv, int kRole>
-__device__ __forceinline__ bool bwd_produce(const FaBwdParams& p, const BwdCta<kDP>& c, const CUtensorMap* map_a,
-                                            const CUtensorMap* map_s, const BwdItem& w, BwdCount& n) {
+struct BwdProducer {
+  BwdPos ring, a, stat, fix;
+  bool any = false;
+  int tiles = 0, stats = 0;
+};
+
+template <int kDP>
+__device__ __forceinline__ bool bwd_produce(const FaBwdParams& p, const BwdCta<kDP>& c, int role, const CUtensorMap* map_a,
+                                            const CUtensorMap* map_s, const BwdItem& w, BwdProducer& n) {
   using C = BwdCfg<kDP>;
-  constexpr int kBS = C::kBS, kRing = kRole == 0 ? C::kRing0 : C::kRing1;
+  constexpr int kBS = C::kBS;
   if (w.nt == 0) return true;
   const int lane = threadIdx.x & 31;
-  const bool packed = p.cu_q != nullptr;
+  const bool packed = p.cu_q != nullptr, dkv = w.kind == kItemDkv;
   const int map_b = packed ? 0 : w.b;
-  uint64_t* const full = kRole == 0 ? c.full0 : c.full1;
-  uint64_t* const empty = kRole == 0 ? c.empty0 : c.empty1;
-  uint8_t* const ring = kRole == 0 ? c.sB0 : c.sB1;
-  if (!bwd_wait(c.a_empty + kRole, (n.items & 1) ^ 1, c.abort_flag, kDevTimeoutEmpty)) return false;
+  uint64_t* const full = role == 0 ? c.full0 : c.full1;
+  uint64_t* const empty = role == 0 ? c.empty0 : c.empty1;
+  uint8_t* const ring = role == 0 ? c.sB0 : c.sB1;
+  const int size = role == 0 ? C::kRing0 : C::kRing1;
+  if (!bwd_wait(c.a_empty + role, n.a.phase ^ 1, c.abort_flag, kDevTimeoutEmpty)) return false;
   if (lane == 0) {
-    mbar_arrive_expect_tx(c.a_full + kRole, C::kABytes);
+    mbar_arrive_expect_tx(c.a_full + role, C::kABytes);
 #pragma unroll 1
     for (int a = 0; a < C::kAtoms; ++a)
-      tma_load_4d((kRole ? c.sA1 : c.sA0) + a * C::kAAtomBytes, map_a, c.a_full + kRole, a * 64,
-                  (kDkv ? w.k_row0 : w.q_row0) + w.row0, w.h, map_b);
+      tma_load_4d((role ? c.sA1 : c.sA0) + a * C::kAAtomBytes, map_a, c.a_full + role, a * 64,
+                  (dkv ? w.k_row0 : w.q_row0) + w.row0, w.h, map_b);
   }
-  if (kRole == 0 && n.items == 0) {
+  n.a.next(1);
+  if (role == 0 && !n.any) {
     // The statistics kernel's output is read from here on.
     asm volatile("griddepcontrol.wait;" ::: "memory");
     fence_proxy_async_global();
   }
-  ++n.items;
+  n.any = true;
   // A packed sequence's last tile runs into the next sequence's rows.  Rows of
   // the summed dimension must be zero there (0 x NaN is NaN), so such a tile
-  // is cleared past the end before it is handed on.  V tiles of dQ items are
-  // exempt: they only feed dP columns that are masked.
-  const int len = kDkv ? w.M : w.N;  // valid streamed rows of the sequence
-  const int ragged = packed && (kDkv || kRole == 0) && len % kBS != 0 ? len / kBS - w.first : -1;
-  const int row_first = (kDkv ? w.q_row0 : w.k_row0) + w.first * kBS;
+  // is cleared past the end before it is handed on.
+  const int len = dkv ? w.M : w.N;  // valid streamed rows of the sequence
+  const int ragged = packed && len % kBS != 0 ? len / kBS - w.first : -1;
+  const int row_first = (dkv ? w.q_row0 : w.k_row0) + w.first * kBS;
   int ti = w.begin_tile;
-  int head = (kDkv ? w.h * p.group : w.h / p.group) + w.begin_head;
-  const float* stat = nullptr;
-  if constexpr (kDkv && kRole == 0)
-    stat = p.stats + (bwd_stat_tile0(p, w.b, head, w.q_row0, kBS) + w.first) * (2 * kBS);
+  int head = (dkv ? w.h * p.group : w.h / p.group) + w.begin_head;
+  const bool stats = dkv && role == 0;
+  const float* stat = p.stats + (bwd_stat_tile0(p, w.b, head, w.q_row0, kBS) + w.first) * (2 * kBS);
+  const int64_t stat_head = static_cast<int64_t>(p.stat_tiles) * (2 * kBS);
+#pragma unroll 1
   for (int i = 0; i < w.nt; ++i) {
-    const int slot = n.i % kRing;
-    if (!bwd_wait(empty + slot, ((n.i / kRing) & 1) ^ 1, c.abort_flag, kDevTimeoutEmpty)) return false;
-    ++n.i;
-    uint8_t* dst = ring + slot * C::kBBytes;
+    if (!bwd_wait(empty + n.ring.slot, n.ring.phase ^ 1, c.abort_flag, kDevTimeoutEmpty)) return false;
+    uint8_t* dst = ring + n.ring.slot * C::kBBytes;
+    uint64_t* const landed = full + n.ring.slot;
+    n.ring.next(size);
+    ++n.tiles;
     const bool fix = ti == ragged;
     if (lane == 0) {
-      uint64_t* bar = fix ? c.fix + kRole : full + slot;
+      uint64_t* bar = fix ? c.fix + role : landed;
       mbar_arrive_expect_tx(bar, C::kBBytes);
 #pragma unroll
       for (int a = 0; a < C::kAtoms; ++a)
         tma_load_4d(dst + a * C::kBAtomBytes, map_s, bar, a * 64, row_first + ti * kBS, head, map_b);
     }
-    if constexpr (kDkv && kRole == 0) {
-      const int b = n.stats & 1;
-      if (!bwd_wait(c.st_empty + b, ((n.stats >> 1) & 1) ^ 1, c.abort_flag, kDevTimeoutEmpty)) return false;
+    if (stats) {
+      if (!bwd_wait(c.st_empty + n.stat.slot, n.stat.phase ^ 1, c.abort_flag, kDevTimeoutEmpty)) return false;
       if (lane == 0) {
-        mbar_arrive_expect_tx(c.st_full + b, C::kStatBytes);
-        bulk_load_g2s(c.sStat + b * (2 * kBS), stat + ti * (2 * kBS), C::kStatBytes, c.st_full + b);
+        mbar_arrive_expect_tx(c.st_full + n.stat.slot, C::kStatBytes);
+        bulk_load_g2s(c.sStat + n.stat.slot * (2 * kBS), stat + ti * (2 * kBS), C::kStatBytes, c.st_full + n.stat.slot);
       }
+      n.stat.next(2);
       ++n.stats;
     }
     if (fix) {
-      if (!bwd_wait(c.fix + kRole, n.fixes & 1, c.abort_flag, kDevTimeoutKV)) return false;
-      ++n.fixes;
+      if (!bwd_wait(c.fix + role, n.fix.phase, c.abort_flag, kDevTimeoutKV)) return false;
+      n.fix.next(1);
       const int rows = len % kBS, chunks = (kBS - rows) * 8;  // 16-byte pieces of one atom's rows past the end
 #pragma unroll 1
       for (int a = 0; a < C::kAtoms; ++a)
@@ -555,47 +611,122 @@ __device__ __forceinline__ bool bwd_produce(const FaBwdParams& p, const BwdCta<k
           *reinterpret_cast<uint4*>(dst + a * C::kBAtomBytes + rows * 128 + k * 16) = make_uint4(0, 0, 0, 0);
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(full + slot);
+      if (lane == 0) mbar_arrive(landed);
     }
     if (++ti == w.per_head) {
       ti = 0;
       ++head;
-      if constexpr (kDkv && kRole == 0)
-        stat = p.stats + (bwd_stat_tile0(p, w.b, head, w.q_row0, kBS) + w.first) * (2 * kBS);
+      stat += stat_head;
     }
   }
   return true;
 }
 
 // ------------------------------------------------------------- MMA issuers
-// kRole 0 (warp 1): S and dV.  kRole 1 (warp 2): dP and dK or dQ.  A slot of
-// the ring is free when both roles' products that read it are complete.
-template <typename T, int kDP, bool kDkv, int kRole>
-__device__ __forceinline__ bool bwd_issue(const BwdCta<kDP>& c, uint32_t tmem, bool leader, const BwdItem& w,
-                                          BwdCount& n) {
+// Role 0 (warp 1): S and dV.  Role 1 (warp 2): dP and dK or dQ.  A slot of a
+// ring is free when both roles' products that read it are complete.
+struct BwdIssuer {
+  BwdPos s, o;      // the rings of the first and of the second product's operand
+  BwdPos item, it;  // items, streamed tiles
+};
+
+template <typename T, int kDP>
+__device__ __forceinline__ bool bwd_issue(const BwdCta<kDP>& c, uint32_t tmem, bool leader, int role, const BwdItem& w,
+                                          BwdIssuer& n) {
   using C = BwdCfg<kDP>;
-  constexpr int kBS = C::kBS, kRing0 = C::kRing0, kRing1 = C::kRing1;
-  constexpr int kOut = kDkv ? C::kOutDkv : kDP;  // columns of each accumulator
+  constexpr int kBS = C::kBS;
   if (w.nt == 0) return true;
   const int nt = w.nt;
+  const bool dkv = w.kind == kItemDkv;
   constexpr uint32_t kFmt = BwdElem<T>::kFmt;
   constexpr uint32_t idesc_s = umma_idesc(kFmt, 128, kBS, 0, 0);
-  constexpr uint32_t idesc_o = umma_idesc(kFmt, 128, kOut, 0, 1);
+  const uint32_t idesc_o = dkv ? umma_idesc(kFmt, 128, C::kOutDkv, 0, 1) : umma_idesc(kFmt, 128, kDP, 0, 1);
   constexpr uint32_t kHi = umma_desc_hi(1024, kLayoutSw128);
-  const uint32_t a_lo = umma_desc_lo(smem_u32(kRole == 0 ? c.sA0 : c.sA1), 16);
+  const uint32_t a_lo = umma_desc_lo(smem_u32(role == 0 ? c.sA0 : c.sA1), 16);
   // The streamed operand of the role's first product (S or dP), and, MN-major
   // from this item's first output column, that of its second.
-  const uint32_t b_lo = umma_desc_lo(smem_u32(kRole == 0 ? c.sB0 : c.sB1), 16);
-  const uint32_t bn_lo = umma_desc_lo(smem_u32(kRole == 0 ? c.sB1 : c.sB0) + (w.dcol0 / 64) * C::kBAtomBytes,
+  const uint32_t b_lo = umma_desc_lo(smem_u32(role == 0 ? c.sB0 : c.sB1), 16);
+  const uint32_t bn_lo = umma_desc_lo(smem_u32(role == 0 ? c.sB1 : c.sB0) + (w.dcol0 / 64) * C::kBAtomBytes,
                                       C::kBAtomBytes);
-  constexpr int kPass = FAB_BWD_PASS;
+  // This role's buffer, the barriers of its first product and of what the
+  // softmax warps make of it, its rings.
+  const uint32_t tBuf = tmem + (role == 0 ? C::kTmemS : C::kTmemP);
+  const uint32_t tAcc = tmem + C::kTmemAcc + (role == 0 ? C::kOutDkv : 0);
+  uint64_t* const ready = role == 0 ? c.s : c.dp;
+  uint64_t* const stored = role == 0 ? c.pr : c.ds;
+  const int size_s = role == 0 ? C::kRing0 : C::kRing1, size_o = role == 0 ? C::kRing1 : C::kRing0;
+  uint64_t* const full_s = role == 0 ? c.full0 : c.full1;
+  uint64_t* const empty_s = role == 0 ? c.empty0 : c.empty1;
+  uint64_t* const full_o = role == 0 ? c.full1 : c.full0;
+  uint64_t* const empty_o = role == 0 ? c.empty1 : c.empty0;
+  const bool sum = role == 1 || dkv;  // has a second product: dV, dK or dQ
+  // With one slot the tile of the next dP lands where the last one was, after
+  // the burst's first half: it can only be waited for in between.
+  const bool one_burst = C::kRing1 > 1 || role == 0;
   auto wait = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
     return bwd_wait(bar, parity, c.abort_flag, code);
   };
-  // D[128 x kBS] = A (stationary) x B(slot)^T over the head dim.  `pass`: the
-  // other issuer may go on when this burst is nearly out (see below).
-  auto issue_s = [&](uint32_t d, int s, bool pass) {
-    uint32_t qa = a_lo, kb = b_lo + s * (C::kBBytes >> 4);
+  auto commit = [&](uint64_t* bar) {
+    if (leader) mma_commit(bar);
+  };
+  // D[128 x kOut] += A (TMEM, kBS wide) x B(slot).  Each softmax warpgroup's
+  // half of A starts at its half of the fp32 columns; `part` 0 takes the first
+  // half of each warpgroup's columns, 1 the rest.
+  auto second_product = [&](bool acc, int part) {
+    uint32_t vb = bn_lo + n.o.slot * (C::kBBytes >> 4) + part * ((kBS / 64 * 16 * 128) >> 4);
+    uint32_t at = tBuf + part * (kBS / 8);
+    asm volatile("" : "+r"(vb), "+r"(at));
+#pragma unroll
+    for (int x = 0; x < kBS / 32; ++x) {
+      constexpr int kHalf = kBS / 32;  // steps of a warpgroup's columns
+      const int kk = x / (kHalf / 2) * kHalf + x % (kHalf / 2);
+      const uint64_t bd = umma_desc_join(vb + ((kk * 16 * 128) >> 4), kHi);
+      if (leader) mma_ts_f16(tAcc, at + (kk / kHalf) * (kBS / 2) + (kk % kHalf) * 8, bd, idesc_o, (acc || x > 0) ? 1u : 0u);
+    }
+  };
+
+  // One pass per streamed tile, after one for the first tile's first product
+  // alone, which needs no wait for the previous item's last products: it
+  // overwrites a buffer that those read, in issue order.
+#pragma unroll 1
+  for (int i = -1; i < nt; ++i) {
+    const bool more = i + 1 < nt;
+    // All waits come before the burst, so that its products go out together.
+    if (i < 0) {
+      if (!wait(c.a_full + role, n.item.phase, kDevTimeoutQ)) return false;
+    } else {
+      if (sum && !wait(full_o + n.o.slot, n.o.phase, kDevTimeoutKV)) return false;
+      // The first product into an accumulator waits until the previous item's
+      // sums have been read.
+      if (i == 0 && !wait(c.acc_free, n.item.phase ^ 1, kDevTimeoutAcc)) return false;
+    }
+    if (more && (one_burst || i < 0) && !wait(full_s + n.s.slot, n.s.phase, kDevTimeoutKV)) return false;
+    if (i >= 0) {
+      // Bursts alternate between the issuers: role 0's i-th, role 1's i-th.
+      if (!wait(c.turn + (role ^ 1), n.it.phase ^ (role ^ 1), kDevTimeoutP)) return false;
+      if (sum && C::kHalves) {
+        if (!wait(stored, n.it.phase, kDevTimeoutP)) return false;
+        tc_fence_after();
+        second_product(i > 0, 0);
+      }
+      if (!wait(stored + 1, n.it.phase, kDevTimeoutP)) return false;
+      tc_fence_after();
+      if (sum) {
+        if (!C::kHalves) second_product(i > 0, 0);
+        second_product(true, 1);
+        commit(empty_o + n.o.slot);
+      }
+      n.o.next(size_o);
+      n.it.next(1);
+      if (!more) {
+        if (leader) mbar_arrive(c.turn + role);
+        break;
+      }
+      if (!one_burst && !wait(full_s + n.s.slot, n.s.phase, kDevTimeoutKV)) return false;
+    }
+    tc_fence_after();
+    // D[128 x kBS] = A (stationary) x B(slot)^T over the head dim.
+    uint32_t qa = a_lo, kb = b_lo + n.s.slot * (C::kBBytes >> 4);
     asm volatile("" : "+r"(qa), "+r"(kb));
 #pragma unroll
     for (int kk = 0; kk < kDP / 16; ++kk) {
@@ -603,159 +734,79 @@ __device__ __forceinline__ bool bwd_issue(const BwdCta<kDP>& c, uint32_t tmem, b
       const uint32_t off = (kk & 3) * 32;
       const uint64_t ad = umma_desc_join(qa + ((a * C::kAAtomBytes + off) >> 4), kHi);
       const uint64_t bd = umma_desc_join(kb + ((a * C::kBAtomBytes + off) >> 4), kHi);
-      if (pass && kk == kPass && leader) mbar_arrive(c.turn + kRole);
-      if (leader) mma_ss_f16(d, ad, bd, idesc_s, kk > 0 ? 1u : 0u);
+      // The other issuer may go on when this burst is nearly out.
+      if (kk == kDP / 32 && i >= 0 && leader) mbar_arrive(c.turn + role);
+      if (leader) mma_ss_f16(tBuf, ad, bd, idesc_s, kk > 0 ? 1u : 0u);
     }
-  };
-  // D[128 x kOut] += A (TMEM, kBS wide) x B(slot).  Each softmax warpgroup's
-  // half of A starts at its half of the fp32 columns.
-  // `part` 0 takes the first half of each warpgroup's columns, 1 the rest.
-  auto issue_o = [&](uint32_t d, uint32_t a, int s, bool acc, int part) {
-    uint32_t vb = bn_lo + s * (C::kBBytes >> 4);
-    asm volatile("" : "+r"(vb));
-#pragma unroll
-    for (int x = 0; x < kBS / 32; ++x) {
-      constexpr int kHalf = kBS / 32;
-      const int kk = x / (kHalf / 2) * kHalf + x % (kHalf / 2) + part * (kHalf / 2);
-      const uint32_t at = a + (kk / kHalf) * (kBS / 2) + (kk % kHalf) * 8;
-      const uint64_t bd = umma_desc_join(vb + ((kk * 16 * 128) >> 4), kHi);
-      if (leader) mma_ts_f16(d, at, bd, idesc_o, (acc || x > 0) ? 1u : 0u);
-    }
-  };
-  auto commit = [&](uint64_t* bar) {
-    if (leader) mma_commit(bar);
-  };
-  const uint32_t turn = n.items & 1;
-  ++n.items;
-  // This role's buffer, the barriers of its first product and of what the
-  // softmax warps make of it, its rings.
-  const uint32_t tBuf = tmem + (kRole == 0 ? C::kTmemS : C::kTmemP);
-  const uint32_t tAcc = tmem + C::kTmemAcc + (kRole == 0 ? kOut : 0);
-  uint64_t* const ready = kRole == 0 ? c.s : c.dp;
-  uint64_t* const stored = kRole == 0 ? c.pr : c.ds;
-  constexpr int kRingS = kRole == 0 ? kRing0 : kRing1, kRingO = kRole == 0 ? kRing1 : kRing0;
-  uint64_t* const full_s = kRole == 0 ? c.full0 : c.full1;
-  uint64_t* const empty_s = kRole == 0 ? c.empty0 : c.empty1;
-  uint64_t* const full_o = kRole == 0 ? c.full1 : c.full0;
-  uint64_t* const empty_o = kRole == 0 ? c.empty1 : c.empty0;
-  constexpr bool kSum = kRole == 1 || kDkv;  // has a second product: dV, dK or dQ
-  auto wait_s = [&](int i) { return wait(full_s + i % kRingS, (i / kRingS) & 1, kDevTimeoutKV); };
-  // The first product of streamed tile i, and what its completion frees: a
-  // slot counts two releases, one by each role, except that V tiles of dQ
-  // items are read by role 1 alone, which gives both.
-  auto first_product = [&](int i, bool last, bool pass) {
-    issue_s(tBuf, i % kRingS, pass);
     commit(ready);
-    commit(empty_s + i % kRingS);
-    if (kRole == 1 && !kDkv) commit(empty_s + i % kRingS);
-    if (last) commit(c.a_empty + kRole);
-  };
-
-  // It needs no wait for the previous item's last products: it overwrites a
-  // buffer that those read, in issue order.
-  if (!wait(c.a_full + kRole, turn, kDevTimeoutQ) || !wait_s(n.i)) return false;
-  tc_fence_after();
-  first_product(n.i, nt == 1, false);
-  for (int i = 0; i < nt; ++i, ++n.i) {
-    const bool more = i + 1 < nt;
-    // All waits come before the burst, so that its products go out together.
-    // (With one slot the tile of the next dP lands where the last one was,
-    // after this burst's first half: there it is waited for in between.)
-    constexpr bool kOneBurst = kRingS > 1;
-    if (kSum && !wait(full_o + n.i % kRingO, (n.i / kRingO) & 1, kDevTimeoutKV)) return false;
-    // The first product into an accumulator waits until the previous item's
-    // sums have been read.
-    if (i == 0 && !wait(c.acc_free, turn ^ 1, kDevTimeoutAcc)) return false;
-    if (kOneBurst && more && !wait_s(n.i + 1)) return false;
-    // Bursts alternate between the issuers: role 0's i-th, role 1's i-th.
-    if (FAB_BWD_TURNS && !wait(c.turn + (kRole ^ 1), kRole == 0 ? (n.i & 1) ^ 1 : n.i & 1, kDevTimeoutP)) return false;
-    if (kSum && C::kHalves) {
-      if (!wait(stored, n.i & 1, kDevTimeoutP)) return false;
-      tc_fence_after();
-      issue_o(tAcc, tBuf, n.i % kRingO, i > 0, 0);
-    }
-    if (!wait(stored + 1, n.i & 1, kDevTimeoutP)) return false;
-    tc_fence_after();
-    if (kSum) {
-      if (!C::kHalves) issue_o(tAcc, tBuf, n.i % kRingO, i > 0, 0);
-      issue_o(tAcc, tBuf, n.i % kRingO, true, 1);
-      commit(empty_o + n.i % kRingO);
-    }
-    if (!more && leader) mbar_arrive(c.turn + kRole);
-    if (more) {
-      if constexpr (!kOneBurst) {
-        if (!wait_s(n.i + 1)) return false;
-        tc_fence_after();
-      }
-      first_product(n.i + 1, i + 2 == nt, true);
-    }
+    // A slot counts two releases, one by each role, except that V tiles of dQ
+    // items are read by role 1 alone, which gives both.
+    commit(empty_s + n.s.slot);
+    if (role == 1 && !dkv) commit(empty_s + n.s.slot);
+    if (i + 2 == nt) commit(c.a_empty + role);
+    n.s.next(size_s);
   }
-  commit(c.done + (kRole ^ 1));
+  commit(c.done + (role ^ 1));
+  n.item.next(1);
   return true;
 }
 
 // ----------------------------------------------------------------- softmax
-template <typename T, int kDP, bool kDkv>
-__device__ __forceinline__ bool bwd_softmax(const FaBwdParams& p, const BwdCta<kDP>& c, uint32_t tmem,
-                                            const BwdItem& w, BwdCount& n) {
-  using C = BwdCfg<kDP>;
-  constexpr int kBS = C::kBS;
-  using Out = BwdOut<T, kDP, kDkv>;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int half = (warp - 4) >> 2;
-  const int wq = warp & 3;
-  const int r = wq * 32 + lane;  // TMEM lane: stationary row
-  const uint32_t lane_base = static_cast<uint32_t>(wq * 32) << 16;
-  constexpr int kCols = kBS / 2;  // columns of one warpgroup
-  const uint32_t tS = tmem + lane_base + C::kTmemS + half * kCols;
-  const uint32_t tP = tmem + lane_base + C::kTmemP + half * kCols;
-  const int my = w.row0 + r;  // position of this lane's row in the sequence
-  const int M = w.M, N = w.N, row0 = w.row0, nt = w.nt;
-  const float2 c2 = make_float2(p.scale_log2, p.scale_log2);
-  [[maybe_unused]] float row_nl = 0.f, row_nd = 0.f, cta_scale = 1.f;
-  float unscale = 1.f;
-  if constexpr (!kDkv) {
-    if (nt > 0 && my < M) {
-      const int64_t st_tile = bwd_stat_tile0(p, w.b, w.h, w.q_row0, kBS) + my / kBS;
-      row_nl = p.stats[st_tile * (2 * kBS) + my % kBS];
-      row_nd = p.stats[st_tile * (2 * kBS) + kBS + my % kBS];
-      if constexpr (BwdElem<T>::kScaled) {
-        const float e = p.row_exp[st_tile * kBS + my % kBS];
-        row_nl += e - BwdElem<T>::kPExp;  // P, hence dS, times 2^e
-        unscale = exp2f(-e);
-      }
-    }
-  } else if constexpr (BwdElem<T>::kScaled) {
-    // Largest |dO| over every row this item sums.
-    float big = 0.f;
-    for (int x = lane; x < nt; x += 32) {
-      const int j = w.begin + x;
-      big = fmaxf(big, p.tile_max[bwd_stat_tile0(p, w.b, w.h * p.group + j / w.per_head, w.q_row0, kBS) + w.first +
-                                  j % w.per_head]);
-    }
+// Sets columns outside [lo, hi) of this lane's kCols columns to `value`, in
+// TMEM: the few tiles that the mask's edge crosses are prepared with this, so
+// that one copy of the code below serves all.
+template <int kCols>
+__device__ __forceinline__ void bwd_mask(uint32_t addr, int lo, int hi, uint32_t value) {
+#pragma unroll 1
+  for (int cc = 0; cc < kCols; cc += 32) {
+    uint32_t rr[32];
+    tmem_ld32(addr + cc, rr);
+    tmem_wait_ld();
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
-    const float e = big > 0.f ? floorf(log2f(big)) : 0.f;
-    cta_scale = exp2f(-e - BwdElem<T>::kPExp);
-    unscale = exp2f(e);
+    for (int e = 0; e < 32; ++e)
+      if (cc + e < lo || cc + e >= hi) rr[e] = value;
+    tmem_st32(addr + cc, rr);
   }
+  tmem_wait_st();
+}
 
-  // One streamed tile.  `masked`: some pair of this warpgroup's columns is
-  // not visible; `pos0` is the position of its first column.
-  auto step = [&](auto masked, int pos0) -> bool {
-    constexpr bool kMasked = decltype(masked)::value;
-    [[maybe_unused]] const float* st = c.sStat + (n.stats & 1) * (2 * kBS) + half * kCols;
-    // Visible columns [lo, hi) of this lane.
-    const int lo = kMasked && kDkv ? my - pos0 : 0;
-    const int hi = kMasked && !kDkv ? (p.causal ? min(N, my + 1) : N) - pos0 : kCols;
-    if constexpr (kDkv) {
-      if (!bwd_wait(c.st_full + (n.stats & 1), (n.stats >> 1) & 1, c.abort_flag, kDevTimeoutKV)) return false;
-    }
-    if (!bwd_wait(c.s, n.i & 1, c.abort_flag, kDevTimeoutS)) return false;
+struct BwdSoftmax {
+  BwdPos it, item, stat;
+};
+
+// The streamed tiles of one item.
+template <typename T, int kDP, bool kDkv>
+__device__ __forceinline__ bool bwd_tiles(const FaBwdParams& p, const BwdCta<kDP>& c, uint32_t tS, uint32_t tP, int half,
+                                          int r, float row_nl, float row_nd, float cta_scale, const BwdItem& w,
+                                          BwdSoftmax& n) {
+  using C = BwdCfg<kDP>;
+  constexpr int kBS = C::kBS, kCols = kBS / 2, kChunks = kCols / 32;  // columns of one warpgroup
+  const int lane = threadIdx.x & 31;
+  const float2 c2 = make_float2(p.scale_log2, p.scale_log2);
+  const int my = w.row0 + r;  // position of this lane's row in the sequence
+  // Never-visible scores become -inf whatever the scale's sign.
+  const uint32_t out = p.scale_log2 < 0.f ? 0x7f800000u : 0xff800000u;
+  auto arrive = [&](uint64_t* bar) {
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar);
+  };
+  int ti = w.begin_tile;
+#pragma unroll 1
+  for (int i = 0; i < w.nt; ++i) {
+    // Positions of this tile's columns: queries (dK/dV) or keys.
+    const int pos0 = (w.first + ti) * kBS + half * kCols;
+    const int lo = kDkv && p.causal ? my - pos0 : 0;
+    const int hi = kDkv ? kCols : (p.causal ? min(w.N, my + 1) : w.N) - pos0;
+    const bool need_mask = kDkv ? p.causal && pos0 < w.row0 + 127
+                                : pos0 + kCols > w.N || (p.causal && pos0 + kCols - 1 > w.row0);
+    const float* st = c.sStat + n.stat.slot * (2 * kBS) + half * kCols;
+    if (kDkv && !bwd_wait(c.st_full + n.stat.slot, n.stat.phase, c.abort_flag, kDevTimeoutKV)) return false;
+    if (!bwd_wait(c.s, n.it.phase, c.abort_flag, kDevTimeoutS)) return false;
     tc_fence_after();
+    if (need_mask) bwd_mask<kCols>(tS, lo, hi, out);
     // Chunks of 32 columns; the next one's load is under way while one is
     // worked on.
-    constexpr int kChunks = kCols / 32;
     float pr[kCols];
     uint32_t rr[kChunks][32];
     tmem_ld32(tS, rr[0]);
@@ -764,16 +815,13 @@ __device__ __forceinline__ bool bwd_softmax(const FaBwdParams& p, const BwdCta<k
       tmem_wait_ld();
       if (cc + 1 < kChunks) tmem_ld32(tS + (cc + 1) * 32, rr[cc + 1]);
       if (!kDkv && cc + 1 == kChunks) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(c.pr + 1);
+        arrive(c.pr + 1);
+        if (C::kHalves && lane == 0) mbar_arrive(c.pr);  // its phases go with the tiles of both kinds
       }
       // The first half of P is handed on while the second is worked out.
       if (kDkv && C::kHalves && cc == 1) {
         tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(c.pr);
+        arrive(c.pr);
       }
       [[maybe_unused]] uint32_t pk[16];
 #pragma unroll
@@ -789,11 +837,6 @@ __device__ __forceinline__ bool bwd_softmax(const FaBwdParams& p, const BwdCta<k
         pr[x + 1] = ex2_approx(a.y);
         pr[x + 2] = ex2_approx(d.x);
         pr[x + 3] = ex2_approx(d.y);
-        if constexpr (kMasked) {
-#pragma unroll
-          for (int y = x; y < x + 4; ++y)
-            if (y < lo || y >= hi) pr[y] = 0.f;
-        }
         if constexpr (kDkv) {
           pk[e / 2] = BwdElem<T>::pack2(pr[x], pr[x + 1]);
           pk[e / 2 + 1] = BwdElem<T>::pack2(pr[x + 2], pr[x + 3]);
@@ -804,12 +847,12 @@ __device__ __forceinline__ bool bwd_softmax(const FaBwdParams& p, const BwdCta<k
     }
     if constexpr (kDkv) {
       tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(c.pr + 1);
+      arrive(c.pr + 1);
     }
-    if (!bwd_wait(c.dp, n.i & 1, c.abort_flag, kDevTimeoutS)) return false;
+    if (!bwd_wait(c.dp, n.it.phase, c.abort_flag, kDevTimeoutS)) return false;
     tc_fence_after();
+    // P is 0 where nothing is visible, but dP may be infinite or NaN.
+    if (need_mask) bwd_mask<kCols>(tP, lo, hi, 0u);
     tmem_ld32(tP, rr[0]);
 #pragma unroll
     for (int cc = 0; cc < kChunks; ++cc) {
@@ -817,11 +860,9 @@ __device__ __forceinline__ bool bwd_softmax(const FaBwdParams& p, const BwdCta<k
       if (cc + 1 < kChunks) tmem_ld32(tP + (cc + 1) * 32, rr[cc + 1]);
       if (C::kHalves && cc == 1) {
         tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(c.ds);
+        arrive(c.ds);
       }
-      [[maybe_unused]] uint32_t pk[16];
+      uint32_t pk[16];
 #pragma unroll
       for (int e = 0; e < 32; e += 4) {
         const int x = cc * 32 + e;
@@ -837,75 +878,95 @@ __device__ __forceinline__ bool bwd_softmax(const FaBwdParams& p, const BwdCta<k
           d0 = __fmul2_rn(d0, make_float2(cta_scale, cta_scale));
           d1 = __fmul2_rn(d1, make_float2(cta_scale, cta_scale));
         }
-        if constexpr (kMasked) {
-          // P is 0 there, but dP may be infinite or NaN.
-          if (x < lo || x >= hi) d0.x = 0.f;
-          if (x + 1 < lo || x + 1 >= hi) d0.y = 0.f;
-          if (x + 2 < lo || x + 2 >= hi) d1.x = 0.f;
-          if (x + 3 < lo || x + 3 >= hi) d1.y = 0.f;
-        }
         pk[e / 2] = BwdElem<T>::pack2(d0.x, d0.y);
         pk[e / 2 + 1] = BwdElem<T>::pack2(d1.x, d1.y);
       }
       tmem_st16(tP + cc * 16, pk);
     }
     tmem_wait_st();
-    tc_fence_before();
-    __syncwarp();
-    if (lane == 0) {
-      mbar_arrive(c.ds + 1);
-      if constexpr (kDkv) mbar_arrive(c.st_empty + (n.stats & 1));
+    arrive(c.ds + 1);
+    if constexpr (kDkv) {
+      if (lane == 0) mbar_arrive(c.st_empty + n.stat.slot);
+      n.stat.next(2);
     }
-    if constexpr (kDkv) ++n.stats;
-    return true;
-  };
-  int ti = w.begin_tile;
-  for (int i = 0; i < nt; ++i) {
-    // Streamed rows of this tile: query positions (dK/dV) or key positions.
-    const int pos0 = (w.first + ti) * kBS + half * kCols;
-    bool need_mask;
-    if constexpr (kDkv)
-      need_mask = p.causal && pos0 < row0 + 127;
-    else
-      need_mask = pos0 + kCols > N || (p.causal && pos0 + kCols - 1 > row0);
-    if (!(need_mask ? step(std::true_type{}, pos0) : step(std::false_type{}, pos0))) return false;
-    ++n.i;
+    n.it.next(1);
     if (++ti == w.per_head) ti = 0;
   }
+  return true;
+}
 
-  // -------------------------------------------------------------- epilogue
-  if (nt > 0) {
-    if (!bwd_wait(c.done + (kDkv ? half : 0), n.items & 1, c.abort_flag, kDevTimeoutO)) return false;
+template <typename T, int kDP>
+__device__ __forceinline__ bool bwd_softmax(const FaBwdParams& p, const BwdCta<kDP>& c, uint32_t tmem, const BwdItem& w,
+                                            BwdSoftmax& n) {
+  using C = BwdCfg<kDP>;
+  constexpr int kBS = C::kBS;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int half = (warp - 4) >> 2;
+  const int wq = warp & 3;
+  const int r = wq * 32 + lane;  // TMEM lane: stationary row
+  const uint32_t mine = tmem + (static_cast<uint32_t>(wq * 32) << 16);
+  const uint32_t tS = mine + C::kTmemS + half * (kBS / 2), tP = mine + C::kTmemP + half * (kBS / 2);
+  const bool dkv = w.kind == kItemDkv;
+  float unscale = 1.f;  // what the epilogue takes back of dS's scale
+  if (w.nt > 0) {
+    if (dkv) {
+      float cta_scale = 1.f;
+      if constexpr (BwdElem<T>::kScaled) {
+        // Largest |dO| over every row this item sums.
+        float big = 0.f;
+        for (int x = lane; x < w.nt; x += 32) {
+          const int j = w.begin + x;
+          big = fmaxf(big, p.tile_max[bwd_stat_tile0(p, w.b, w.h * p.group + j / w.per_head, w.q_row0, kBS) + w.first +
+                                      j % w.per_head]);
+        }
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
+        const float e = big > 0.f ? floorf(log2f(big)) : 0.f;
+        cta_scale = exp2f(-e - BwdElem<T>::kPExp);
+        unscale = exp2f(e);
+      }
+      if (!bwd_tiles<T, kDP, true>(p, c, tS, tP, half, r, 0.f, 0.f, cta_scale, w, n)) return false;
+    } else {
+      float row_nl = 0.f, row_nd = 0.f;
+      const int my = w.row0 + r;
+      if (my < w.M) {
+        const int64_t st_tile = bwd_stat_tile0(p, w.b, w.h, w.q_row0, kBS) + my / kBS;
+        row_nl = p.stats[st_tile * (2 * kBS) + my % kBS];
+        row_nd = p.stats[st_tile * (2 * kBS) + kBS + my % kBS];
+        if constexpr (BwdElem<T>::kScaled) {
+          const float e = p.row_exp[st_tile * kBS + my % kBS];
+          row_nl += e - BwdElem<T>::kPExp;  // P, hence dS, times 2^e
+          unscale = exp2f(-e);
+        }
+      }
+      if (!bwd_tiles<T, kDP, false>(p, c, tS, tP, half, r, row_nl, row_nd, 1.f, w, n)) return false;
+    }
+    if (!bwd_wait(c.done + (dkv ? half : 0), n.item.phase, c.abort_flag, kDevTimeoutO)) return false;
     tc_fence_after();
-    ++n.items;
+    n.item.next(1);
   }
-  const Out out(p, w, half, r);
-  const bool is_v = kDkv && half == 1;
-  const float mul = is_v ? exp2f(-BwdElem<T>::kPExp) : p.scale * unscale;
-  const uint32_t t_acc = tmem + lane_base + C::kTmemAcc + (kDkv ? (is_v ? Out::kOut : 0) : out.col0);
-  const bool sliced = w.slices > 1;
+  const BwdOut<T, kDP> out(p, w, half, wq);
+  const float mul = dkv && half == 1 ? exp2f(-BwdElem<T>::kPExp) : p.scale * unscale;
 #pragma unroll 1
-  for (int cc = 0; cc < Out::kCols / 32; ++cc) {
+  for (int cc = 0; cc < out.cols; cc += 32) {
     float v[32];
-    if (nt > 0) {
+#pragma unroll
+    for (int e = 0; e < 32; ++e) v[e] = 0.f;  // where no pair is visible
+    if (w.nt > 0) {
       uint32_t rr[32];
-      tmem_ld32(t_acc + cc * 32, rr);
+      tmem_ld32(mine + C::kTmemAcc + out.acc + cc, rr);
       tmem_wait_ld();
 #pragma unroll
       for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(rr[e]) * mul;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 32; ++e) v[e] = 0.f;  // no pair is visible
     }
-    if (sliced) {
+    if (w.slices > 1) {
 #pragma unroll
-      for (int e = 0; e < 32; ++e) out.part[(cc * 32 + e) * 128] = v[e];
+      for (int e = 0; e < 32; ++e) out.part[(cc + e) * 128] = v[e];
     } else {
-      const int left = p.D - out.col0 - cc * 32;
-      if (out.row_ok && left > 0) bwd_store32<T>(out.row + out.col0 + cc * 32, v, left);
+      out.store(cc, v, p.D);
     }
   }
-  if (nt > 0) {
+  if (w.nt > 0) {
     tc_fence_before();
     __syncwarp();
     if (lane == 0) mbar_arrive(c.acc_free);
@@ -956,6 +1017,7 @@ __global__ void __launch_bounds__(384, 1)
     mbar_init(c.acc_free, 8);
     mbar_init(c.clc, 1);
     *c.abort_flag = *reinterpret_cast<volatile int*>(&g_fab_device_error) != 0 ? -1 : 0;
+    c.abort_flag[1] = 0;
     // The swizzled tiles need the base that the alignment above asks for.
     if (smem_u32(smem_raw) & 1023u) {
       record_device_error(kDevTimeoutTeardown);
@@ -984,108 +1046,105 @@ __global__ void __launch_bounds__(384, 1)
   // Each warpgroup re-splits its registers first, whatever it does after.
   if (warp < 4) {
     setmaxnreg_dec<C::kLoadRegs>();
-    // No copy may still be landing when a producer leaves.
-    auto landed = [&](const BwdCount& n, uint64_t* a_full, uint64_t* full, int ring, bool with_stats) {
-      volatile int no_abort = 0;
-      if (lane == 0) {
-        if (n.items > 0) mbar_wait(a_full, (n.items - 1) & 1, &no_abort, kDevTimeoutTeardown);
-        for (int x = max(0, n.i - ring); x < n.i; ++x)
-          mbar_wait(full + x % ring, (x / ring) & 1, &no_abort, kDevTimeoutTeardown);
-        for (int x = max(0, n.stats - 2); with_stats && x < n.stats; ++x)
-          mbar_wait(c.st_full + (x & 1), (x >> 1) & 1, &no_abort, kDevTimeoutTeardown);
-      }
-      __syncwarp();
-    };
-    if (warp == 0 && !skip) {
-      BwdCount n;
-      volatile int no_abort = 0;
+    if ((warp == 0 || warp == 3) && !skip) {
+      const int role = warp == 0 ? 0 : 1;
+      BwdProducer n;
+      BwdItem w;
       int index = static_cast<int>(blockIdx.x);
-      int asked = 0;
+      BwdPos answer;
+      // The scheduler's next block index, -1 when there is none.
       auto ask = [&]() -> int {
-        int x = -1;
         if (lane == 0) {
           mbar_arrive_expect_tx(c.clc, 16);
           clc_try_cancel(c.clc_resp, c.clc);
-          if (mbar_wait(c.clc, asked & 1, &no_abort, kDevTimeoutSched)) x = clc_first_cta_x(c.clc_resp);
         }
-        ++asked;
-        return __shfl_sync(0xffffffffu, x, 0);
+        // The answer must have landed before this CTA may leave: the word
+        // after the abort flag stays zero, so only the tries bound this wait.
+        const bool ok = bwd_wait(c.clc, answer.phase, c.abort_flag + 1, kDevTimeoutSched);
+        answer.next(1);
+        return ok ? clc_first_cta_x(c.clc_resp) : -1;
       };
+#pragma unroll 1
       for (int q = 0;; ++q) {
-        // The next item that exists: this block's, then the scheduler's.
-        BwdItem w;
-        bool found = false;
-        while (index >= 0 && !found) {
-          found = index < p.num_dkv ? bwd_item<kDP, true>(p, index, w) : bwd_item<kDP, false>(p, index - p.num_dkv, w);
-          if (!found) index = ask();
-        }
-        if (!found) w.kind = kItemEnd;
-        // Whatever is posted, the slot's last item must have been read.
-        if (q >= 2 && !bwd_wait(c.sched_empty + (q & 1), ((q - 2) >> 1) & 1, c.abort_flag, kDevTimeoutSched)) break;
-        if (lane == 0) {
-          c.item[q & 1] = w;
-          mbar_arrive(c.sched_full + (q & 1));
+        if (role == 0) {
+          // The next item that exists: this block's, then the scheduler's.
+          bool found = false;
+#pragma unroll 1
+          while (index >= 0 && !found) {
+            found = index < p.num_dkv ? bwd_item<kDP, true>(p, index, w) : bwd_item<kDP, false>(p, index - p.num_dkv, w);
+            if (!found) index = ask();
+          }
+          if (!found) w.kind = kItemEnd;
+          // Whatever is posted, the slot's last item must have been read.
+          if (q >= 2 && !bwd_wait(c.sched_empty + (q & 1), ((q - 2) >> 1) & 1, c.abort_flag, kDevTimeoutSched)) break;
+          if (lane == 0) {
+            c.item[q & 1] = w;
+            mbar_arrive(c.sched_full + (q & 1));
+          }
+        } else {
+          get_item(q, w);
         }
         if (w.kind == kItemEnd) break;
-        if (!(w.kind == kItemDkv ? bwd_produce<T, kDP, true, 0>(p, c, &k_a, &q_b, w, n)
-                                 : bwd_produce<T, kDP, false, 0>(p, c, &q_a, &k_b, w, n)))
-          break;
+        const bool dkv = w.kind == kItemDkv;
+        const CUtensorMap* map_a = dkv ? (role ? &v_a : &k_a) : role ? &g_a : &q_a;
+        const CUtensorMap* map_s = dkv ? (role ? &g_b : &q_b) : role ? &v_b : &k_b;
+        if (!bwd_produce<kDP>(p, c, role, map_a, map_s, w, n)) break;
         // All of this item's loads are under way: time to ask for the next.
-        index = ask();
+        if (role == 0) index = ask();
       }
-      landed(n, c.a_full, c.full0, C::kRing0, true);
-    } else if (warp == 3 && !skip) {
-      BwdCount n;
+      // No copy may still be landing when a producer leaves: the last one
+      // into every buffer, whether or not its tile was handed on.
+      if (n.any) bwd_wait(c.a_full + role, n.a.phase ^ 1, c.abort_flag + 1, kDevTimeoutTeardown);
+      uint64_t* const full = role == 0 ? c.full0 : c.full1;
+      const int size = role == 0 ? C::kRing0 : C::kRing1;
+      BwdPos last = n.ring;  // the oldest of the last `size` loads, if there were as many
+      if (n.tiles < size) last = BwdPos();
+      else last.phase ^= 1;
+#pragma unroll 1
+      for (int x = min(n.tiles, size); x > 0; --x) {
+        bwd_wait(full + last.slot, last.phase, c.abort_flag + 1, kDevTimeoutTeardown);
+        last.next(size);
+      }
+      BwdPos stat = n.stat;
+      if (n.stats < 2) stat = BwdPos();
+      else stat.phase ^= 1;
+#pragma unroll 1
+      for (int x = min(n.stats, 2); x > 0; --x) {
+        bwd_wait(c.st_full + stat.slot, stat.phase, c.abort_flag + 1, kDevTimeoutTeardown);
+        stat.next(2);
+      }
+    } else if (!skip) {
+      const bool leader = elect_one();
+      const int role = warp - 1;
+      BwdIssuer n;
       BwdItem w;
+#pragma unroll 1
       for (int q = 0;; ++q) {
         get_item(q, w);
-        if (w.kind == kItemEnd) break;
-        if (!(w.kind == kItemDkv ? bwd_produce<T, kDP, true, 1>(p, c, &v_a, &g_b, w, n)
-                                 : bwd_produce<T, kDP, false, 1>(p, c, &g_a, &v_b, w, n)))
-          break;
+        if (w.kind == kItemEnd || !bwd_issue<T, kDP>(c, tmem, leader, role, w, n)) break;
       }
-      landed(n, c.a_full + 1, c.full1, C::kRing1, false);
-    } else if ((warp == 1 || warp == 2) && !skip) {
-      const bool leader = elect_one();
-      auto issue = [&](auto role) {
-        constexpr int kRole = decltype(role)::value;
-        BwdCount n;
-        BwdItem w;
-        for (int q = 0;; ++q) {
-          get_item(q, w);
-          if (w.kind == kItemEnd) break;
-          if (!(w.kind == kItemDkv ? bwd_issue<T, kDP, true, kRole>(c, tmem, leader, w, n)
-                                   : bwd_issue<T, kDP, false, kRole>(c, tmem, leader, w, n)))
-            break;
-        }
-        // Drain the tensor pipe before TMEM is released.
-        if (leader) mma_commit(c.drained + kRole);
-        volatile int no_abort = 0;
-        mbar_wait_warp(c.drained + kRole, 0, &no_abort, kDevTimeoutTeardown);
-      };
-      if (warp == 1)
-        issue(std::integral_constant<int, 0>{});
-      else
-        issue(std::integral_constant<int, 1>{});
+      // Drain the tensor pipe before TMEM is released.
+      if (leader) mma_commit(c.drained + role);
+      bwd_wait(c.drained + role, 0, c.abort_flag + 1, kDevTimeoutTeardown);
     }
   } else {
     setmaxnreg_inc<C::kSoftmaxRegs>();
     if (!skip) {
       asm volatile("griddepcontrol.wait;" ::: "memory");  // the statistics
-      BwdCount n;
+      BwdSoftmax n;
       BwdItem w;
+#pragma unroll 1
       for (int q = 0;; ++q) {
         get_item(q, w);
-        if (w.kind == kItemEnd) break;
-        if (!(w.kind == kItemDkv ? bwd_softmax<T, kDP, true>(p, c, tmem, w, n) : bwd_softmax<T, kDP, false>(p, c, tmem, w, n)))
-          break;
+        if (w.kind == kItemEnd || !bwd_softmax<T, kDP>(p, c, tmem, w, n)) break;
       }
     }
   }
 
   // A warp that gave up left its code.
   __syncthreads();
-  if (threadIdx.x == 0 && *c.abort_flag > 0) record_device_error(*c.abort_flag);
+  if (threadIdx.x == 0 && c.abort_flag[0] > 0) record_device_error(c.abort_flag[0]);
+  if (threadIdx.x == 0 && c.abort_flag[1] > 0) record_device_error(c.abort_flag[1]);
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
@@ -1099,25 +1158,21 @@ __global__ void __launch_bounds__(384, 1)
 // blockIdx.y: 32-column chunk of a thread's columns.
 template <typename T, int kDP, bool kDkv>
 __global__ void __launch_bounds__(256) fa_bwd_join_kernel(const FaBwdParams p) {
-  using Out = BwdOut<T, kDP, kDkv>;
   const int max_slices = kDkv ? p.dkv_slices : p.dq_slices;
   BwdItem w;
   if (!bwd_item<kDP, kDkv>(p, static_cast<int>(blockIdx.x) * max_slices, w) || w.slices <= 1) return;
-  const Out out(p, w, threadIdx.x >> 7, threadIdx.x & 127);
-  const int cc = blockIdx.y;
-  const int left = p.D - out.col0 - cc * 32;
-  if (!out.row_ok || left <= 0) return;
-  constexpr int64_t kSlot = static_cast<int64_t>(kDkv ? 2 : 1) * Out::kOut * 128;
-  const float* src = out.part + cc * 32 * 128;
+  const BwdOut<T, kDP> out(p, w, threadIdx.x >> 7, (threadIdx.x >> 5) & 3);
+  const int cc = blockIdx.y * 32;
+  const float* src = out.part + cc * 128;
   float v[32];
 #pragma unroll
   for (int e = 0; e < 32; ++e) v[e] = src[e * 128];
   for (int s = 1; s < w.slices; ++s) {
-    src += kSlot;
+    src += out.slot;
 #pragma unroll
     for (int e = 0; e < 32; ++e) v[e] += src[e * 128];
   }
-  bwd_store32<T>(out.row + out.col0 + cc * 32, v, left);
+  out.store(cc, v, p.D);
 }
 
 }  // namespace fab
