@@ -318,6 +318,32 @@ def device_limits(device: int) -> FabDeviceLimits:
 
 
 def current_stream_handle(device) -> int:
+    """The cudaStream_t of torch's current stream on `device`."""
     import torch
 
+    # The same handle without a Stream object around it, where torch offers it: a tenth of the time.
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    index = getattr(device, "index", None)
+    if raw is not None and index is not None:
+        return raw(index)
     return int(torch.cuda.current_stream(device).cuda_stream)
+
+
+class _CurrentDevice:
+    """The context of a call whose tensors are on the current device already."""
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_CURRENT = _CurrentDevice()
+
+
+def on_device(device):
+    """`torch.cuda.device(device)`, or a context that does nothing where that is the current device."""
+    import torch
+
+    return _CURRENT if torch.cuda.current_device() == device.index else torch.cuda.device(device)

@@ -120,7 +120,7 @@ struct BwdCfg {
   // S, P x 2, dP, dS x 2; issue order x 2; accumulators final x 2 and read; ragged tile x 2; next item
   // full/empty x 2; its request; teardown x 2.
   static constexpr int kNumBars = 2 * (kRing0 + kRing1) + 4 + 4 + 6 + 3 + 2 + 4 + 3 + 2;
-  static constexpr int kTailBytes = 208;  // TMEM address, abort flag, a zero word, two items, the scheduler's response
+  static constexpr int kTailBytes = 304;  // TMEM address, abort flag, a zero word, two items, the scheduler's response
   static constexpr int kSmemBytes =
       2 * kABytes + (kRing0 + kRing1) * kBBytes + 2 * kStatBytes + kNumBars * 8 + kTailBytes;
   // P and dS are handed to the tensor core in two halves where a warp works
@@ -270,14 +270,15 @@ __global__ void __launch_bounds__(256) fa_bwd_stats_kernel(const FaBwdParams p) 
 }
 
 // A 32-column chunk of a warp's 32 output rows: lane r brings row r's values,
-// packed.  Storing them as they lie would touch 32 lines per instruction; four
-// lanes exchange their 16-byte pieces first (a 4 x 4 transpose in two steps),
-// so that they store 64 consecutive bytes of one row at a time: 8 lines per
-// instruction (measured: 5400 cycles per 128 x 256 tile before, see below for
-// now).  `row` is this warp's first row at the chunk's first column; `rows`
-// and `cols` say how much of the chunk exists.  16-byte aligned rows.
+// packed.  Four lanes exchange their 16-byte pieces (a 4 x 4 transpose in two
+// steps) and store 64 consecutive bytes of one row at a time, 8 lines per
+// instruction instead of 32.  An SM writes some 30 bytes a cycle whichever way
+// (measured; 32-byte stores of whole sectors without the exchange were 3 %
+// slower at 4 x 32 heads, S 1024, causal).  `row` is the warp's first row at
+// the chunk's first column, `stride` in bytes; `rows` and `cols` say how much
+// of the chunk exists.  16-byte aligned rows.
 template <typename T>
-__device__ __forceinline__ void bwd_store_chunk(T* row, int64_t stride, int rows, int cols, const uint32_t (&w)[16]) {
+__device__ __forceinline__ void bwd_store_chunk(int64_t row, int64_t stride, int rows, int cols, const uint32_t (&w)[16]) {
   const int lane = threadIdx.x & 31;
   const bool odd = lane & 1, high = lane & 2;
   uint32_t t[16], u[16];
@@ -298,19 +299,22 @@ __device__ __forceinline__ void bwd_store_chunk(T* row, int64_t stride, int rows
   }
   // u holds piece lane % 4 of the four rows of this group of lanes.
   const int col = (lane & 3) * 8;
-  T* dst = row + (lane & ~3) * stride + col;
+  T* dst = reinterpret_cast<T*>(row + (lane & ~3) * stride) + col;
+  rows -= lane & ~3;
 #pragma unroll
-  for (int i = 0; i < 4; ++i, dst += stride) {
-    if ((lane & ~3) + i >= rows) continue;
-    if (col + 8 <= cols) {
-      *reinterpret_cast<uint4*>(dst) = make_uint4(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
-    } else {
+  for (int i = 0; i < 4; ++i) {
+    if (i < rows) {
+      if (col + 8 <= cols) {
+        *reinterpret_cast<uint4*>(dst) = make_uint4(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
+      } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (col + e < cols)
-          reinterpret_cast<uint16_t*>(dst)[e] =
-              static_cast<uint16_t>((e & 1) ? u[4 * i + e / 2] >> 16 : u[4 * i + e / 2] & 0xFFFFu);
+        for (int e = 0; e < 8; ++e)
+          if (col + e < cols)
+            reinterpret_cast<uint16_t*>(dst)[e] =
+                static_cast<uint16_t>((e & 1) ? u[4 * i + e / 2] >> 16 : u[4 * i + e / 2] & 0xFFFFu);
+      }
     }
+    dst = reinterpret_cast<T*>(reinterpret_cast<int64_t>(dst) + stride);
   }
 }
 
@@ -356,6 +360,9 @@ struct BwdItem {
   int begin, nt;           // this slice: streamed tiles begin .. begin + nt of all heads'
   int begin_head, begin_tile;  // begin / per_head, begin % per_head
   int slice, slices;
+  // The tile's first row in dK or dQ [0] and in dV [1], the bytes between
+  // rows, and the slice's sums where there are several slices.
+  int64_t out[2], stride[2], part;
 };
 enum BwdItemKind : int { kItemEnd, kItemDkv, kItemDq };
 
@@ -426,41 +433,53 @@ __device__ __forceinline__ int64_t bwd_part_slot(const FaBwdParams& p, const Bwd
   }
 }
 
-// Where warp (half, rows wq * 32 ...) writes: dK/dV items: warpgroup 0 dK, 1
-// dV; dQ items: each half of the columns.
+// Where the item's results go.
+template <typename T, int kDP, bool kDkv>
+__device__ __forceinline__ void bwd_outputs(const FaBwdParams& p, BwdItem& w) {
+  constexpr int64_t kSize = sizeof(T);
+  auto at = [&](const void* base, int64_t sb, int64_t sh, int64_t ss, int row0) {
+    return reinterpret_cast<int64_t>(base) + ((p.cu_q ? row0 * ss : w.b * sb) + w.h * sh + w.row0 * ss) * kSize;
+  };
+  if constexpr (kDkv) {
+    w.out[0] = at(p.dk, p.dk_sb, p.dk_sh, p.dk_ss, w.k_row0);
+    w.out[1] = at(p.dv, p.dv_sb, p.dv_sh, p.dv_ss, w.k_row0);
+    w.stride[0] = p.dk_ss * kSize;
+    w.stride[1] = p.dv_ss * kSize;
+    w.part = reinterpret_cast<int64_t>(p.dkv_part + bwd_part_slot<kDP, true>(p, w) * (2 * BwdCfg<kDP>::kOutDkv * 128));
+  } else {
+    w.out[0] = w.out[1] = at(p.dq, p.dq_sb, p.dq_sh, p.dq_ss, w.q_row0);
+    w.stride[0] = w.stride[1] = p.dq_ss * kSize;
+    w.part = reinterpret_cast<int64_t>(p.dq_part + bwd_part_slot<kDP, false>(p, w) * (kDP * 128));
+  }
+}
+
+// What warp (half, rows wq * 32 ...) of the tile writes: dK/dV items:
+// warpgroup 0 dK, 1 dV; dQ items: each half of the columns.
 template <typename T, int kDP>
 struct BwdOut {
-  T* row;          // the warp's first output row
-  int64_t stride;  // between rows
-  int rows;        // of the warp's 32 that exist
-  int col0, cols;  // its columns of the row
-  int acc;         // its first accumulator column
-  float* part;     // this lane's column 0 of the slice's sums
-  int64_t slot;    // floats between slices
-  __device__ __forceinline__ BwdOut(const FaBwdParams& p, const BwdItem& w, int half, int wq) {
-    constexpr int kOutDkv = BwdCfg<kDP>::kOutDkv;
-    const int r0 = wq * 32, my = w.row0 + r0;
-    const bool dkv = w.kind == kItemDkv, is_v = half == 1;
-    rows = (dkv ? w.N : w.M) - my;
-    stride = !dkv ? p.dq_ss : is_v ? p.dv_ss : p.dk_ss;
-    const int64_t sh = !dkv ? p.dq_sh : is_v ? p.dv_sh : p.dk_sh, sb = !dkv ? p.dq_sb : is_v ? p.dv_sb : p.dk_sb;
-    const int64_t seq = p.cu_q != nullptr ? (dkv ? w.k_row0 : w.q_row0) * stride : w.b * sb;
-    row = reinterpret_cast<T*>(!dkv ? p.dq : is_v ? p.dv : p.dk) + seq + w.h * sh + my * stride;
-    cols = dkv ? kOutDkv : kDP / 2;
-    col0 = dkv ? w.dcol0 : half * cols;
+  int64_t row, stride;  // the warp's first row at its first column, bytes between rows
+  int rows, left;       // rows of the warp's 32, columns from there on, that exist
+  int cols;             // columns of a warp
+  int acc;              // its first accumulator column
+  float* part;          // this lane's column 0 of the slice's sums
+  __device__ __forceinline__ BwdOut(const BwdItem& w, int half, int wq, int head_dim) {
+    const bool dkv = w.kind == kItemDkv;
+    cols = dkv ? BwdCfg<kDP>::kOutDkv : kDP / 2;
+    const int col0 = dkv ? w.dcol0 : half * cols;
+    stride = half ? w.stride[1] : w.stride[0];
+    row = (half ? w.out[1] : w.out[0]) + wq * 32 * stride + col0 * static_cast<int>(sizeof(T));
+    rows = (dkv ? w.N : w.M) - w.row0 - wq * 32;
+    left = head_dim - col0;
     acc = half * cols;
-    slot = dkv ? 2 * kOutDkv * 128 : kDP * 128;
-    part = (dkv ? p.dkv_part + bwd_part_slot<kDP, true>(p, w) * slot : p.dq_part + bwd_part_slot<kDP, false>(p, w) * slot) +
-           acc * 128 + r0 + (threadIdx.x & 31);
+    part = reinterpret_cast<float*>(w.part) + acc * 128 + wq * 32 + (threadIdx.x & 31);
   }
-  // 32 columns from the thread's column cc on.
-  __device__ __forceinline__ void store(int cc, const float (&v)[32], int head_dim) const {
-    const int left = head_dim - col0 - cc;
-    if (rows <= 0 || left <= 0) return;
+  // 32 columns from the warp's column cc on.
+  __device__ __forceinline__ void store(int cc, const float (&v)[32]) const {
+    if (rows <= 0 || cc >= left) return;
     uint32_t w[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) w[e] = BwdElem<T>::pack2(v[2 * e], v[2 * e + 1]);
-    bwd_store_chunk<T>(row + col0 + cc, stride, rows, left, w);
+    bwd_store_chunk<T>(row + cc * static_cast<int>(sizeof(T)), stride, rows, left - cc, w);
   }
 };
 
@@ -505,8 +524,8 @@ struct BwdCta {
     tmem_slot = reinterpret_cast<uint32_t*>(drained + 2);
     abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     clc_resp = (smem_u32(tmem_slot + 3) + 15u) & ~15u;
-    item = reinterpret_cast<BwdItem*>(tmem_slot + 11);
-    static_assert(44 + 2 * sizeof(BwdItem) <= C::kTailBytes, "two items in the tail");
+    item = reinterpret_cast<BwdItem*>(tmem_slot + 12);
+    static_assert(48 + 2 * sizeof(BwdItem) <= C::kTailBytes, "two items in the tail");
   }
 };
 
@@ -945,7 +964,7 @@ __device__ __forceinline__ bool bwd_softmax(const FaBwdParams& p, const BwdCta<k
     tc_fence_after();
     n.item.next(1);
   }
-  const BwdOut<T, kDP> out(p, w, half, wq);
+  const BwdOut<T, kDP> out(w, half, wq, p.D);
   const float mul = dkv && half == 1 ? exp2f(-BwdElem<T>::kPExp) : p.scale * unscale;
 #pragma unroll 1
   for (int cc = 0; cc < out.cols; cc += 32) {
@@ -963,7 +982,7 @@ __device__ __forceinline__ bool bwd_softmax(const FaBwdParams& p, const BwdCta<k
 #pragma unroll
       for (int e = 0; e < 32; ++e) out.part[(cc + e) * 128] = v[e];
     } else {
-      out.store(cc, v, p.D);
+      out.store(cc, v);
     }
   }
   if (w.nt > 0) {
@@ -1074,7 +1093,12 @@ __global__ void __launch_bounds__(384, 1)
             found = index < p.num_dkv ? bwd_item<kDP, true>(p, index, w) : bwd_item<kDP, false>(p, index - p.num_dkv, w);
             if (!found) index = ask();
           }
-          if (!found) w.kind = kItemEnd;
+          if (!found)
+            w.kind = kItemEnd;
+          else if (w.kind == kItemDkv)
+            bwd_outputs<T, kDP, true>(p, w);
+          else
+            bwd_outputs<T, kDP, false>(p, w);
           // Whatever is posted, the slot's last item must have been read.
           if (q >= 2 && !bwd_wait(c.sched_empty + (q & 1), ((q - 2) >> 1) & 1, c.abort_flag, kDevTimeoutSched)) break;
           if (lane == 0) {
@@ -1161,18 +1185,20 @@ __global__ void __launch_bounds__(256) fa_bwd_join_kernel(const FaBwdParams p) {
   const int max_slices = kDkv ? p.dkv_slices : p.dq_slices;
   BwdItem w;
   if (!bwd_item<kDP, kDkv>(p, static_cast<int>(blockIdx.x) * max_slices, w) || w.slices <= 1) return;
-  const BwdOut<T, kDP> out(p, w, threadIdx.x >> 7, (threadIdx.x >> 5) & 3);
+  bwd_outputs<T, kDP, kDkv>(p, w);
+  const BwdOut<T, kDP> out(w, threadIdx.x >> 7, (threadIdx.x >> 5) & 3, p.D);
   const int cc = blockIdx.y * 32;
+  constexpr int64_t kSlot = (kDkv ? 2 * BwdCfg<kDP>::kOutDkv : kDP) * 128;
   const float* src = out.part + cc * 128;
   float v[32];
 #pragma unroll
   for (int e = 0; e < 32; ++e) v[e] = src[e * 128];
   for (int s = 1; s < w.slices; ++s) {
-    src += out.slot;
+    src += kSlot;
 #pragma unroll
     for (int e = 0; e < 32; ++e) v[e] += src[e * 128];
   }
-  out.store(cc, v, p.D);
+  out.store(cc, v);
 }
 
 }  // namespace fab

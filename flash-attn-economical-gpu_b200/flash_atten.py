@@ -16,7 +16,9 @@ benchmarks: same maths, plus grouped-query heads mapped inside the kernel.
 from __future__ import annotations
 
 import ctypes
+import functools
 import logging
+import struct
 from dataclasses import dataclass
 
 import torch
@@ -515,67 +517,96 @@ def attention_forward_varlen(
 
 
 def _conform_operand(t: torch.Tensor) -> torch.Tensor:
-    """`_conform`, and a copy of broadcast (stride 0) dims, which a tensor map cannot describe."""
-    if any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+    """A 4-D operand a tensor map can describe: `t`, or a row-padded copy of broadcast (stride 0) or unaligned ones."""
+    sb, sh, ss, sd = t.stride()
+    if sd == 1 and not t.data_ptr() & 15:
+        B, H, S, _ = t.shape
+        per16 = 16 // t.element_size()
+        if (ss > 0 and not ss % per16 or S < 2) and (sh > 0 and not sh % per16 or H < 2) and \
+                (sb > 0 and not sb % per16 or B < 2):
+            return t
+    if 0 in (sb, sh, ss):
         t = t.contiguous()
     return _conform(t)
+
+
+# fab_attention_bwd_params as one packed record: filling its fifty-odd fields one by one costs more than the launches
+# of a short call.
+_BWD_RECORD = struct.Struct("9P27q2P9ifiPN")
+assert _BWD_RECORD.size == ctypes.sizeof(_native.FabAttentionBwdParams)
+
+
+@functools.lru_cache(maxsize=256)
+def _backward_workspace(batch, heads_q, heads_kv, seq_q, seq_k, total_q, total_k, head_dim, dtype, causal, packed) -> int:
+    """fab_attention_bwd_workspace for these sizes (pointers are only checked for alignment)."""
+    p = _native.FabAttentionBwdParams()
+    for name in ("q", "k", "v", "o", "dout", "lse", "dq", "dk", "dv"):
+        setattr(p, name, 256)
+    if packed:
+        p.cu_seqlens_q = p.cu_seqlens_k = 256
+    p.batch, p.heads_q, p.heads_kv, p.seqlen_q, p.seqlen_k = batch, heads_q, heads_kv, seq_q, seq_k
+    p.total_q, p.total_k, p.head_dim, p.dtype, p.causal, p.sm_scale = total_q, total_k, head_dim, dtype, causal, 1.0
+    need = ctypes.c_size_t(0)
+    _native.check(_native.lib.fab_attention_bwd_workspace(ctypes.byref(p), ctypes.byref(need)), "attention backward")
+    return need.value
 
 
 def _launch_attention_backward(what, dout, q, k, v, out, lse, causal, sm_scale, workspace, cu_q=None, cu_k=None,
                                max_q=0, max_k=0):
     """Validate, conform and launch one attention backward; all tensors as [B, H, S, D] views (B = 1 when packed)."""
-    named = (("dout", dout), ("q", q), ("k", k), ("v", v), ("out", out), ("lse", lse))
-    for name, t in named:
+    for name, t in (("dout", dout), ("q", q), ("k", k), ("v", v), ("out", out), ("lse", lse)):
         _require_cuda_tensor(name, t)
-    if q.dtype not in (torch.float16, torch.bfloat16):
-        raise ValueError(f"{what}: gradients are computed in float16 or bfloat16, got {q.dtype}")
-    if any(t.dtype != q.dtype for t in (dout, k, v, out)):
+    dtype, dev = q.dtype, q.device
+    if dtype is not torch.bfloat16 and dtype is not torch.float16:
+        raise ValueError(f"{what}: gradients are computed in float16 or bfloat16, got {dtype}")
+    if not dout.dtype == k.dtype == v.dtype == out.dtype == dtype:
         raise ValueError(f"{what}: dout, q, k, v and out must share one dtype")
-    if any(t.device != q.device for _, t in named):
+    if not dout.device == k.device == v.device == out.device == lse.device == dev:
         raise ValueError(f"{what}: all tensors must be on one device")
-    B, Hq, M, D = q.shape
-    Bk, Hkv, N, Dk = k.shape
-    if v.shape != k.shape or Bk != B or Dk != D or out.shape != q.shape or dout.shape != q.shape:
+    B, Hq, M, D = shape_q = q.shape
+    Bk, Hkv, N, Dk = shape_k = k.shape
+    if v.shape != shape_k or Bk != B or Dk != D or out.shape != shape_q or dout.shape != shape_q:
         raise ValueError(f"{what}: inconsistent shapes dout={tuple(dout.shape)} q={tuple(q.shape)} "
                          f"k={tuple(k.shape)} v={tuple(v.shape)} out={tuple(out.shape)}")
     if Hkv == 0 or Hq == 0 or Hq % Hkv:
         raise ValueError(f"{what}: query heads ({Hq}) must be a multiple of key/value heads ({Hkv})")
-    if lse.dtype != torch.float32 or tuple(lse.shape) != (B, Hq, M):
+    if lse.dtype is not torch.float32 or lse.shape != (B, Hq, M):
         raise ValueError(f"{what}: lse must be float32, one value per query row and head")
     if D < 1 or D > 256:
         raise ValueError(f"{what}: head_dim must be between 1 and 256, got {D}")
-    dq, dk, dv = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
-    if B == 0 or (M == 0 and N == 0):
-        return dq, dk, dv
     # Head dims off the 16-byte grid are written to padded rows first.
-    padded = D * q.element_size() % 16 != 0
-    outs = tuple(_padded_like(t) if padded else t for t in (dq, dk, dv))
-    ins = tuple(_conform_operand(t) if t.numel() else t for t in (q, k, v, out, dout))
-    p = _native.FabAttentionBwdParams()
-    for name, t in zip(("q", "k", "v", "o", "dout", "lse", "dq", "dk", "dv"), (*ins, lse, *outs)):
-        setattr(p, name, t.data_ptr())
-        for d, s in zip("bhs", t.stride()):
-            setattr(p, f"{name}_stride_{d}", s)
-    p.batch, p.heads_q, p.heads_kv, p.seqlen_q, p.seqlen_k, p.head_dim = B, Hq, Hkv, M, N, D
-    if cu_q is not None:
-        p.cu_seqlens_q, p.cu_seqlens_k = cu_q.data_ptr(), cu_k.data_ptr()
-        p.batch, p.total_q, p.total_k, p.seqlen_q, p.seqlen_k = cu_q.numel() - 1, M, N, int(max_q), int(max_k)
-    p.dtype, p.sm_scale, p.causal = _native.dtype_code(q.dtype), float(sm_scale), 1 if causal else 0
-    need = ctypes.c_size_t(0)
-    with torch.cuda.device(q.device):
-        _native.check(_native.lib.fab_attention_bwd_workspace(ctypes.byref(p), ctypes.byref(need)), what)
-        ws = workspace
-        if need.value and ws is None:
-            ws = torch.empty(need.value, device=q.device, dtype=torch.uint8)
-        if ws is not None:
-            _require_cuda_tensor("workspace", ws)
-            p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel() * ws.element_size()
-        stream = ctypes.c_void_p(_native.current_stream_handle(q.device))
-        _native.check(_native.lib.fab_attention_bwd(ctypes.byref(p), stream), what)
+    padded = D % 8 != 0
     if padded:
-        for t, buf in zip((dq, dk, dv), outs):
-            t.copy_(buf)
-    return dq, dk, dv
+        outs = tuple(_padded_like(t) for t in (q, k, v))
+    else:
+        outs = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    if B == 0 or (M == 0 and N == 0):
+        return tuple(t.contiguous() for t in outs) if padded else outs
+    ins = [_conform_operand(t) if t.numel() else t for t in (q, k, v, out, dout)]
+    code = _native.FAB_DTYPE_BF16 if dtype is torch.bfloat16 else _native.FAB_DTYPE_F16
+    causal = 1 if causal else 0
+    if cu_q is None:
+        sizes = (B, Hq, Hkv, M, N, 0, 0, D, code)
+        cu = 0, 0
+    else:
+        sizes = (cu_q.numel() - 1, Hq, Hkv, int(max_q), int(max_k), M, N, D, code)
+        cu = cu_q.data_ptr(), cu_k.data_ptr()
+    need = _backward_workspace(*sizes, causal, cu_q is not None)
+    with _native.on_device(dev):
+        ws, have = workspace, 0
+        if ws is None and need:
+            ws = torch.empty(need, device=dev, dtype=torch.uint8)
+            have = need
+        elif ws is not None:
+            _require_cuda_tensor("workspace", ws)
+            have = ws.numel() * ws.element_size()
+        strides = [s for t in ins for s in t.stride()[:3]] + list(lse.stride()) + [s for t in outs for s in t.stride()[:3]]
+        p = _native.FabAttentionBwdParams.from_buffer_copy(_BWD_RECORD.pack(
+            *[t.data_ptr() for t in ins], lse.data_ptr(), *[t.data_ptr() for t in outs], *strides, *cu, *sizes,
+            float(sm_scale), causal, ws.data_ptr() if ws is not None else 0, have))
+        rc = _native.lib.fab_attention_bwd(ctypes.byref(p), _native.current_stream_handle(dev))
+    _native.check(rc, what)
+    return tuple(t.contiguous() for t in outs) if padded else outs
 
 
 def attention_backward(
@@ -656,24 +687,16 @@ def attention_backward_varlen(
     return tuple(t.transpose(1, 2).squeeze(0) for t in grads)
 
 
-def attention_backward_workspace_bytes(q_shape, k_shape, dtype, *, packed_batch: int | None = None) -> int:
-    """Workspace bytes attention_backward needs for [B, H, S, D] shapes; with `packed_batch` sequences,
-    attention_backward_varlen for [total, H, D] shapes."""
-    p = _native.FabAttentionBwdParams()
+def attention_backward_workspace_bytes(q_shape, k_shape, dtype, *, causal: bool = False, packed_batch: int | None = None,
+                                       max_seqlen_q: int = 0, max_seqlen_k: int = 0) -> int:
+    """Workspace bytes attention_backward needs for [B, H, S, D] shapes; with `packed_batch` sequences (and their
+    longest lengths), attention_backward_varlen for [total, H, D] shapes."""
+    dt = _native.dtype_code(dtype)
     if packed_batch is None:
-        p.batch, p.heads_q, p.seqlen_q, p.head_dim = q_shape
-        _, p.heads_kv, p.seqlen_k, _ = k_shape
-    else:
-        p.batch, (p.total_q, p.heads_q, p.head_dim), (p.total_k, p.heads_kv, _) = packed_batch, q_shape, k_shape
-        p.seqlen_q, p.seqlen_k = p.total_q, p.total_k
-        p.cu_seqlens_q = p.cu_seqlens_k = 256
-    for name in ("q", "k", "v", "o", "dout", "lse", "dq", "dk", "dv"):
-        setattr(p, name, 256)  # only shapes and the type are read
-    p.dtype, p.sm_scale = _native.dtype_code(dtype), 1.0
-    need = ctypes.c_size_t(0)
-    _native.check(_native.lib.fab_attention_bwd_workspace(ctypes.byref(p), ctypes.byref(need)),
-                  "attention_backward_workspace_bytes")
-    return need.value
+        (B, Hq, M, D), (_, Hkv, N, _) = q_shape, k_shape
+        return _backward_workspace(B, Hq, Hkv, M, N, 0, 0, D, dt, int(causal), False)
+    (M, Hq, D), (N, Hkv, _) = q_shape, k_shape
+    return _backward_workspace(packed_batch, Hq, Hkv, max_seqlen_q or M, max_seqlen_k or N, M, N, D, dt, int(causal), True)
 
 
 def _host_pieces(batch: int, kv_heads: int, chunks: int) -> list[tuple[int, int, int]]:

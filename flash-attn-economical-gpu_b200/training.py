@@ -9,6 +9,8 @@ rest of the package.  No counterpart in the reference, which has no backward pas
 from __future__ import annotations
 
 import ctypes
+import functools
+import struct
 
 import torch
 
@@ -22,9 +24,13 @@ from flash_atten import (
 )
 
 
+_DTYPES = {torch.float16: _native.FAB_DTYPE_F16, torch.bfloat16: _native.FAB_DTYPE_BF16, torch.float32: _native.FAB_DTYPE_F32}
+
+
 def _rows(t: torch.Tensor, cols: int) -> torch.Tensor:
     """`t` as [rows, cols] with unit column stride (a view where its strides allow it)."""
-    t = t.reshape(-1, cols)
+    if t.ndim != 2:
+        t = t.reshape(-1, cols)
     if t.stride(1) != 1 and cols > 1:
         t = t.contiguous()
     return t
@@ -48,7 +54,8 @@ def _check_norm_input(what: str, x) -> None:
     _require_cuda_tensor("x", x)
     if x.ndim < 1 or x.shape[-1] < 1:
         raise ValueError(f"{what}: x must have at least one column")
-    _native.dtype_code(x.dtype)
+    if x.dtype not in _DTYPES:
+        raise ValueError(f"{what}: x must be float16, bfloat16 or float32, got {x.dtype}")
 
 
 def layernorm_forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *, eps: float = 1e-5,
@@ -68,21 +75,23 @@ def layernorm_forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor 
             raise ValueError(f"{what}: weight and bias must share one dtype")
     if residual is not None:
         _check_norm_tensor(what, "residual", residual, x)
-    cols = x.shape[-1]
+    shape, dev = x.shape, x.device
+    cols = shape[-1]
     x2 = _rows(x, cols)
-    r2 = _rows(residual, cols) if residual is not None else None
     rows = x2.shape[0]
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    total = torch.empty(x.shape, device=x.device, dtype=x.dtype) if residual is not None else None
-    mean, rstd = torch.empty((2, *x.shape[:-1]), device=x.device, dtype=torch.float32)
+    y = x.new_empty(shape)
+    mean, rstd = x.new_empty(shape[:-1], dtype=torch.float32), x.new_empty(shape[:-1], dtype=torch.float32)
     w, b = weight.contiguous(), bias.contiguous() if bias is not None else None
-    with torch.cuda.device(x.device):
+    if residual is not None:
+        r2, total = _rows(residual, cols), x.new_empty(shape)
+        r_ptr, r_ld, total_ptr = r2.data_ptr(), r2.stride(0), total.data_ptr()
+    else:
+        r_ptr, r_ld, total_ptr = None, 0, None
+    with _native.on_device(dev):
         rc = _native.lib.fab_layernorm(
-            x2.data_ptr(), r2.data_ptr() if r2 is not None else None, w.data_ptr(),
-            b.data_ptr() if b is not None else None, y.data_ptr(), total.data_ptr() if total is not None else None,
-            mean.data_ptr(), rstd.data_ptr(), rows, cols, x2.stride(0), r2.stride(0) if r2 is not None else 0, cols,
-            cols, float(eps), _native.dtype_code(x.dtype), _native.dtype_code(weight.dtype),
-            ctypes.c_void_p(_native.current_stream_handle(x.device)))
+            x2.data_ptr(), r_ptr, w.data_ptr(), b.data_ptr() if b is not None else None, y.data_ptr(), total_ptr,
+            mean.data_ptr(), rstd.data_ptr(), rows, cols, x2.stride(0), r_ld, cols, cols, eps, _DTYPES[x.dtype],
+            _DTYPES[weight.dtype], _native.current_stream_handle(dev))
     _native.check(rc, what)
     return (y, mean, rstd) if residual is None else (y, mean, rstd, total)
 
@@ -105,25 +114,33 @@ def layernorm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, 
         _require_cuda_tensor(name, t)
         if t.dtype != torch.float32 or t.shape != x.shape[:-1] or t.device != x.device:
             raise ValueError(f"{what}: {name} must be float32 with shape {tuple(x.shape[:-1])}")
-    cols = x.shape[-1]
+    shape, dev = x.shape, x.device
+    cols = shape[-1]
     x2, dy2 = _rows(x, cols), _rows(dy, cols)
-    r2 = _rows(dresidual, cols) if dresidual is not None else None
     rows = x2.shape[0]
-    dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    dw, db = torch.empty((2, cols), device=x.device, dtype=weight.dtype)
+    dx, dw, db = x.new_empty(shape), weight.new_empty(cols), weight.new_empty(cols)
     w, mean, rstd = weight.contiguous(), mean.contiguous(), rstd.contiguous()
-    need = ctypes.c_size_t(0)
-    _native.check(_native.lib.fab_layernorm_bwd_workspace(rows, cols, ctypes.byref(need)), what)
-    ws = torch.empty(need.value, device=x.device, dtype=torch.uint8)
-    with torch.cuda.device(x.device):
+    if dresidual is not None:
+        r2 = _rows(dresidual, cols)
+        r_ptr, r_ld = r2.data_ptr(), r2.stride(0)
+    else:
+        r_ptr, r_ld = None, 0
+    need = _norm_workspace(rows, cols)
+    ws = torch.empty(need, device=dev, dtype=torch.uint8)
+    with _native.on_device(dev):
         rc = _native.lib.fab_layernorm_bwd(
-            dy2.data_ptr(), x2.data_ptr(), w.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
-            r2.data_ptr() if r2 is not None else None, dx.data_ptr(), dw.data_ptr(), db.data_ptr(), ws.data_ptr(),
-            need.value, rows, cols, dy2.stride(0), x2.stride(0), r2.stride(0) if r2 is not None else 0, cols,
-            _native.dtype_code(x.dtype), _native.dtype_code(weight.dtype),
-            ctypes.c_void_p(_native.current_stream_handle(x.device)))
+            dy2.data_ptr(), x2.data_ptr(), w.data_ptr(), mean.data_ptr(), rstd.data_ptr(), r_ptr, dx.data_ptr(),
+            dw.data_ptr(), db.data_ptr(), ws.data_ptr(), need, rows, cols, dy2.stride(0), x2.stride(0), r_ld, cols,
+            _DTYPES[x.dtype], _DTYPES[weight.dtype], _native.current_stream_handle(dev))
     _native.check(rc, what)
     return dx, dw, db
+
+
+@functools.lru_cache(maxsize=256)
+def _norm_workspace(rows: int, cols: int) -> int:
+    need = ctypes.c_size_t(0)
+    _native.check(_native.lib.fab_layernorm_bwd_workspace(rows, cols, ctypes.byref(need)), "layernorm_backward")
+    return need.value
 
 
 def rope_multi_axis(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, cos: torch.Tensor,
@@ -159,37 +176,40 @@ def rope_multi_axis(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Te
     if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.shape != sin.shape or cos.ndim != 2 or \
             cos.shape[1] != half:
         raise ValueError(f"{what}: cos and sin must be float32 tables with {half} columns")
-    dt = _native.dtype_code(q.dtype)
+    if q.dtype not in _DTYPES:
+        raise ValueError(f"{what}: unsupported dtype {q.dtype}; expected float16, bfloat16 or float32")
     qc = q if q.stride(2) == 1 else q.contiguous()
     kc = k if k is None or k.stride(2) == 1 else k.contiguous()
     if out is None:
-        out = (torch.empty(q.shape, device=q.device, dtype=q.dtype),
-               torch.empty(k.shape, device=k.device, dtype=k.dtype) if k is not None else None)
-    for name, t, like in (("out[0]", out[0], q), ("out[1]", out[1], k)):
-        if like is None:
-            continue
-        _require_cuda_tensor(name, t)
-        if t.shape != like.shape or t.dtype != like.dtype or t.device != q.device or t.stride(2) != 1:
-            raise ValueError(f"{what}: {name} must match its input's shape, dtype and device, with unit stride along the head")
+        out = (q.new_empty(q.shape), k.new_empty(k.shape) if k is not None else None)
+    else:
+        for name, t, like in (("out[0]", out[0], q), ("out[1]", out[1], k)):
+            if like is None:
+                continue
+            _require_cuda_tensor(name, t)
+            if t.shape != like.shape or t.dtype != like.dtype or t.device != q.device or t.stride(2) != 1:
+                raise ValueError(f"{what}: {name} must match its input's shape, dtype and device, with unit stride "
+                                 "along the head")
     cos, sin = cos.contiguous(), sin.contiguous()
-    p = _native.FabRopeAxesParams()
-    p.q, p.q_out, p.positions = qc.data_ptr(), out[0].data_ptr(), positions.data_ptr()
-    p.cos, p.sin = cos.data_ptr(), sin.data_ptr()
-    p.q_stride_t, p.q_stride_h = qc.stride()[:2]
-    p.q_out_stride_t, p.q_out_stride_h = out[0].stride()[:2]
+    qo, ko = out
     if k is not None:
-        p.k, p.k_out, p.heads_k = kc.data_ptr(), out[1].data_ptr(), k.shape[1]
-        p.k_stride_t, p.k_stride_h = kc.stride()[:2]
-        p.k_out_stride_t, p.k_out_stride_h = out[1].stride()[:2]
-    p.positions_stride_axis, p.positions_stride_t = positions.stride()
-    p.tokens, p.heads_q, p.head_dim, p.axes, p.table_rows = T, Hq, D, len(sections), cos.shape[0]
-    for i, s in enumerate(sections):
-        p.sections[i] = s
-    p.positions_64bit, p.inverse, p.dtype = int(positions.dtype == torch.int64), int(bool(inverse)), dt
-    with torch.cuda.device(q.device):
-        rc = _native.lib.fab_rope_axes(ctypes.byref(p), ctypes.c_void_p(_native.current_stream_handle(q.device)))
+        k_ptrs, heads_k, k_strides = (kc.data_ptr(), ko.data_ptr()), k.shape[1], (*kc.stride()[:2], *ko.stride()[:2])
+    else:
+        k_ptrs, heads_k, k_strides = (0, 0), 0, (0, 0, 0, 0)
+    p = _native.FabRopeAxesParams.from_buffer_copy(_ROPE_RECORD.pack(
+        qc.data_ptr(), k_ptrs[0], qo.data_ptr(), k_ptrs[1], positions.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+        *qc.stride()[:2], *k_strides[:2], *qo.stride()[:2], *k_strides[2:], *positions.stride(), T, Hq, heads_k, D,
+        len(sections), *sections, *(0,) * (_native.MAX_ROPE_AXES - len(sections)), cos.shape[0],
+        positions.dtype is torch.int64, bool(inverse), _DTYPES[q.dtype]))
+    with _native.on_device(q.device):
+        rc = _native.lib.fab_rope_axes(ctypes.byref(p), _native.current_stream_handle(q.device))
     _native.check(rc, what)
     return out
+
+
+# fab_rope_axes_params as one packed record.
+_ROPE_RECORD = struct.Struct("7P10q13i4x")
+assert _ROPE_RECORD.size == ctypes.sizeof(_native.FabRopeAxesParams)
 
 
 # ---------------------------------------------------------------- autograd
