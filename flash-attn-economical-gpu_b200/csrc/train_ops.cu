@@ -1,6 +1,7 @@
 // Translation unit of the training operators around the attention: layer
 // norm and multi-axis rotary embedding (train_ops.cuh), with their C entry
 // points.  Their kernels have no device-side waits.
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 
@@ -15,9 +16,18 @@ bool aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p)
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int elt_bytes(int dtype) { return dtype == kDtypeF32 ? 4 : 2; }
 
-// Lines of partial dw/db sums: a fixed count, so that the order of the sums
-// does not depend on the device.
-constexpr int kMaxPartLines = 592;
+// CTAs of the layer norm backward kernels, which are also the lines of partial
+// dw/db sums: as many as stay resident (an SM holds 2048 16-byte vectors of
+// the rows being worked on: two stages of x, dy and dres, or three of x and a
+// residual, take 192 KB of shared memory), by sizes alone, so that the order of the sums does not
+// depend on the device.
+constexpr int kSms = 148;
+constexpr int kResidentVectors = 2048;
+// The most lines of any path.
+int64_t max_lines(int64_t rows, int cols) {
+  const int64_t per_cta = std::max<int64_t>(ceil_div(cols, 8), 64);
+  return std::min<int64_t>(rows, kSms * std::max<int64_t>(2, 2048 / per_cta));
+}
 
 int launched() { return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch; }
 
@@ -30,48 +40,113 @@ int run_fwd(const LayerNormParams& p, cudaStream_t st) {
   return launched();
 }
 
+// From this many rows per resident CTA on, the forward pass streams rows
+// through resident CTAs; below, every row has a CTA of its own.
+constexpr int64_t kStreamRows = 3;
+
+template <typename T, typename W, int NV, int kMaxThreads, int kMinCtas>
+int run_fwd_stream(const LayerNormParams& p, cudaStream_t st) {
+  constexpr int kStages = 3;
+  auto kern = layernorm_fwd_stream_kernel<T, W, NV, kMaxThreads, kMinCtas, kStages>;
+  const int threads = row_threads(p.cols, 16 / sizeof(T), NV);
+  const int64_t ctas = std::min<int64_t>(p.rows, kSms * std::max(1, kResidentVectors / (threads * NV)));
+  const size_t smem = size_t(kStages) * NV * 2 * threads * 16;
+  if (int rc = ensure_smem_attr(reinterpret_cast<const void*>(kern), 200 * 1024)) return rc;
+  kern<<<static_cast<unsigned>(ctas), threads, smem, st>>>(p);
+  return launched();
+}
+
 template <typename T, typename W>
 int fwd(const LayerNormParams& p, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
   const bool vec = p.cols % V == 0 && aligned(p.x, 16) && aligned(p.residual, 16) && aligned(p.w, 16) &&
                    aligned(p.bias, 16) && aligned(p.y, 16) && aligned(p.x_out, 16) && p.ld_x % V == 0 &&
                    p.ld_y % V == 0 && (p.residual == nullptr || (p.ld_res % V == 0 && p.ld_xo % V == 0));
+  if (vec && p.cols <= 1024 * V && p.rows >= kStreamRows * kSms * std::max(1, kResidentVectors / (p.cols / V))) {
+    if (p.cols <= 64 * V) return run_fwd_stream<T, W, 2, 32, 12>(p, st);
+    return run_fwd_stream<T, W, 4, 256, 2>(p, st);
+  }
   if (vec) {
-    // The fewest vectors per thread that keep the CTA within 256 threads,
-    // else within 1024.
-    if (p.cols <= 256 * V) return run_fwd<T, W, V, 1, 256>(p, st);
-    if (p.cols <= 512 * V) return run_fwd<T, W, V, 2, 256>(p, st);
+    // The fewest vectors per thread that keep the CTA within 512 threads, else
+    // within 1024.
+    if (p.cols <= 512 * V) return run_fwd<T, W, V, 1, 512>(p, st);
+    if (p.cols <= 1024 * V) return run_fwd<T, W, V, 2, 512>(p, st);
     if (p.cols <= 4096 * V) return run_fwd<T, W, V, 4, 1024>(p, st);
   } else {
     if (p.cols <= 1024) return run_fwd<T, W, 1, 4, 256>(p, st);
+    if (p.cols <= 4096) return run_fwd<T, W, 1, 8, 512>(p, st);
     if (p.cols <= 16384) return run_fwd<T, W, 1, 16, 1024>(p, st);
   }
   layernorm_fwd_long_kernel<T, W><<<static_cast<unsigned>(p.rows), 1024, 0, st>>>(p);
   return launched();
 }
 
-template <typename T, typename W, int V, int NV, int kMaxThreads>
-int run_bwd(const LayerNormBwdParams& p, int lines, cudaStream_t st) {
-  layernorm_bwd_kernel<T, W, V, NV, kMaxThreads><<<lines, row_threads(p.cols, V, NV), 0, st>>>(p);
+// A launch that is set up while the previous kernel of the stream runs; the
+// kernel itself waits before it reads that one's results.
+template <typename... Args, typename... Given>
+int launch_after(void (*kernel)(Args...), unsigned grid, unsigned block, cudaStream_t st, Given... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess) return kOk;
+  cudaGetLastError();
+  return kErrLaunch;
+}
+
+template <typename T, typename W, int NV, int kMaxThreads, int kMinCtas, bool kWarpRow>
+int run_bwd(const LayerNormBwdParams& p, int* lines, cudaStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  const int threads = kWarpRow ? kMaxThreads : row_threads(p.cols, V, NV);
+  // Rows on their way at once per worker, this one included.
+  constexpr int kStages = 2;
+  auto kern = layernorm_bwd_kernel<T, W, NV, kMaxThreads, kMinCtas, kWarpRow, kStages>;
+  size_t smem = size_t(kStages) * NV * 3 * threads * 16;
+  const int vectors = threads * NV;  // of one row, or of all the warps' rows
+  *lines = static_cast<int>(std::min({kWarpRow ? ceil_div(p.rows, threads / 32) : p.rows,
+                                      int64_t(kSms) * std::max(1, kResidentVectors / vectors), max_lines(p.rows, p.cols)}));
+  if (kWarpRow) smem = std::max(smem, size_t(threads / 32) * p.cols * sizeof(float));
+  if (int rc = ensure_smem_attr(reinterpret_cast<const void*>(kern), 200 * 1024)) return rc;
+  kern<<<*lines, threads, smem, st>>>(p);
+  return launched();
+}
+
+template <typename T, typename W, int NV, int kMaxThreads>
+int run_bwd_any(const LayerNormBwdParams& p, int* lines, cudaStream_t st) {
+  const int threads = row_threads(p.cols, 1, NV);
+  *lines = static_cast<int>(std::min<int64_t>(max_lines(p.rows, p.cols), kSms * std::min(16, std::max(1, 2048 / threads))));
+  layernorm_bwd_any_kernel<T, W, NV, kMaxThreads><<<*lines, threads, 0, st>>>(p);
   return launched();
 }
 
 template <typename T, typename W>
-int bwd(const LayerNormBwdParams& p, void* dw, void* db, int lines, cudaStream_t st) {
+int bwd(const LayerNormBwdParams& p, void* dw, void* db, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
   const bool vec = p.cols % V == 0 && aligned(p.x, 16) && aligned(p.dy, 16) && aligned(p.w, 16) &&
                    aligned(p.dres, 16) && aligned(p.dx, 16) && p.ld_x % V == 0 && p.ld_dy % V == 0 && p.ld_dx % V == 0 &&
                    (p.dres == nullptr || p.ld_dres % V == 0);
-  int rc;
-  if (vec && p.cols <= 256 * V) {
-    rc = run_bwd<T, W, V, 1, 256>(p, lines, st);
+  int rc, lines = 0;
+  if (vec && p.cols <= 32 * V) {
+    rc = run_bwd<T, W, 1, 256, 3, true>(p, &lines, st);
+  } else if (vec && p.cols <= 64 * V) {
+    rc = run_bwd<T, W, 2, 256, 2, true>(p, &lines, st);
+  } else if (vec && p.cols <= 256 * V) {
+    rc = run_bwd<T, W, 2, 128, 4, false>(p, &lines, st);
+  } else if (vec && p.cols <= 512 * V) {
+    rc = run_bwd<T, W, 4, 128, 4, false>(p, &lines, st);
   } else if (vec && p.cols <= 1024 * V) {
-    rc = run_bwd<T, W, V, 2, 512>(p, lines, st);
-  } else if (!vec && p.cols <= 1024) {
-    rc = run_bwd<T, W, 1, 4, 256>(p, lines, st);
+    rc = run_bwd<T, W, 4, 256, 2, false>(p, &lines, st);
+  } else if (!vec && p.cols <= 4096) {
+    rc = run_bwd_any<T, W, 8, 512>(p, &lines, st);
   } else if (!vec && p.cols <= 8192) {
-    rc = run_bwd<T, W, 1, 16, 512>(p, lines, st);
+    rc = run_bwd_any<T, W, 16, 512>(p, &lines, st);
   } else {
+    lines = static_cast<int>(max_lines(p.rows, p.cols));
     layernorm_bwd_long_kernel<T, W><<<static_cast<unsigned>(p.rows), 1024, 0, st>>>(p);
     if (p.part != nullptr)
       layernorm_bwd_long_cols_kernel<T>
@@ -79,9 +154,8 @@ int bwd(const LayerNormBwdParams& p, void* dw, void* db, int lines, cudaStream_t
     rc = launched();
   }
   if (rc || p.part == nullptr) return rc;
-  layernorm_bwd_finish_kernel<W><<<static_cast<unsigned>(ceil_div(2 * int64_t(p.cols), 32)), 256, 0, st>>>(
-      p.part, lines, p.cols, static_cast<W*>(dw), static_cast<W*>(db));
-  return launched();
+  return launch_after(layernorm_bwd_finish_kernel<W>, static_cast<unsigned>(ceil_div(2 * int64_t(p.cols), 32)), 1024u, st,
+                      static_cast<const float*>(p.part), lines, p.cols, static_cast<W*>(dw), static_cast<W*>(db));
 }
 
 // The (T, W) pairs: weights in the activations' type or fp32.
@@ -95,22 +169,25 @@ int by_types(int dtype, int w_dtype, F f) {
   return kErrUnsupported;
 }
 
-int bwd_lines(int64_t rows) { return static_cast<int>(rows < kMaxPartLines ? rows : kMaxPartLines); }
-
 template <typename T, int V>
-int run_rope(const RopeParams& p, cudaStream_t st) {
+int run_rope(RopeParams& p, cudaStream_t st) {
   const int nvec = p.half / V + (p.head_dim - 2 * p.half) / V;
-  if (nvec > 256) return kErrUnsupported;
-  rope_axes_kernel<T, V><<<dim3(static_cast<unsigned>(p.tokens), 1), 256, 0, st>>>(p);
+  p.slots = (p.heads_q + p.heads_k + kRopeHeads - 1) / kRopeHeads;
+  const int64_t blocks = ceil_div(int64_t(p.tokens) * nvec * p.slots, 256);
+  if (blocks > 0x7fffffffLL) return kErrUnsupported;
+  rope_axes_kernel<T, V><<<static_cast<unsigned>(blocks), 256, 0, st>>>(p);
   return launched();
 }
 
 template <typename T>
-int rope(const RopeParams& p, cudaStream_t st) {
+int rope(RopeParams& p, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
   auto even = [&](const void* ptr, int64_t a, int64_t b) { return aligned(ptr, 16) && a % V == 0 && b % V == 0; };
   const bool vec = p.half % V == 0 && p.head_dim % V == 0 && even(p.q, p.q_st, p.q_sh) && even(p.q_out, p.qo_st, p.qo_sh) &&
                    (p.heads_k == 0 || (even(p.k, p.k_st, p.k_sh) && even(p.k_out, p.ko_st, p.ko_sh)));
+  p.vec_table = vec && aligned(p.cos, 16) && aligned(p.sin, 16);
+  for (int i = 0; i < p.axes; ++i)
+    if (p.ends[i] % V != 0) p.vec_table = 0;
   return vec ? run_rope<T, V>(p, st) : run_rope<T, 1>(p, st);
 }
 
@@ -140,7 +217,7 @@ int fab_layernorm(const void* x, const void* residual, const void* w, const void
 
 int fab_layernorm_bwd_workspace(int64_t rows, int cols, size_t* bytes) {
   if (bytes == nullptr || rows < 0 || cols <= 0) return kErrInvalidArg;
-  *bytes = size_t(bwd_lines(rows)) * 2 * size_t(cols) * sizeof(float);
+  *bytes = size_t(max_lines(rows, cols)) * 2 * size_t(cols) * sizeof(float);
   return kOk;
 }
 
@@ -162,15 +239,14 @@ int fab_layernorm_bwd(const void* dy, const void* x, const void* w, const float*
   if (!aligned(dy, e) || !aligned(x, e) || !aligned(dresidual, e) || !aligned(dx, e) || !aligned(w, we) ||
       !aligned(mean, 4) || !aligned(rstd, 4))
     return kErrInvalidArg;
-  const int lines = bwd_lines(rows);
   const bool sums = dw != nullptr || db != nullptr;
   if (sums && (workspace == nullptr || !aligned(workspace, 16) ||
-               workspace_bytes < size_t(lines) * 2 * size_t(cols) * sizeof(float)))
+               workspace_bytes < size_t(max_lines(rows, cols)) * 2 * size_t(cols) * sizeof(float)))
     return kErrWorkspace;
   LayerNormBwdParams p{dy, x, w, mean, rstd, dresidual, dx, sums ? static_cast<float*>(workspace) : nullptr,
                        ld_dy, ld_x, ld_dres, ld_dx, rows, cols};
   return by_types(dtype, w_dtype,
-                  [&](auto t, auto wt) { return bwd<decltype(t), decltype(wt)>(p, dw, db, lines, st); });
+                  [&](auto t, auto wt) { return bwd<decltype(t), decltype(wt)>(p, dw, db, st); });
 }
 
 int fab_rope_axes(const fab_rope_axes_params* a, void* stream) {

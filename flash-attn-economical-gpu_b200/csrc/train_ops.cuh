@@ -33,39 +33,157 @@ template <typename T, int V>
 struct alignas(V * sizeof(T) < 16 ? V * sizeof(T) : 16) Vec {
   T e[V];
 };
+// Two 16-bit values of one word, converted together.
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t w);
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename T, int V>
+__device__ __forceinline__ void to_floats(const Vec<T, V>& v, float (&f)[V]) {
+  if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&v);
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      const float2 x = unpack2<T>(w[i]);
+      f[2 * i] = x.x;
+      f[2 * i + 1] = x.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = to_float<T>(v.e[i]);
+  }
+}
 template <typename T, int V>
 __device__ __forceinline__ void load_vec(const T* p, float (&f)[V]) {
-  const Vec<T, V> v = *reinterpret_cast<const Vec<T, V>*>(p);
-#pragma unroll
-  for (int i = 0; i < V; ++i) f[i] = to_float<T>(v.e[i]);
+  if constexpr (V * sizeof(T) == 16) {
+    const uint4 w = *reinterpret_cast<const uint4*>(p);
+    to_floats<T, V>(*reinterpret_cast<const Vec<T, V>*>(&w), f);
+  } else if constexpr (V * sizeof(T) == 32) {
+    const uint4 w[2] = {reinterpret_cast<const uint4*>(p)[0], reinterpret_cast<const uint4*>(p)[1]};
+    to_floats<T, V>(*reinterpret_cast<const Vec<T, V>*>(w), f);
+  } else {
+    to_floats<T, V>(*reinterpret_cast<const Vec<T, V>*>(p), f);
+  }
 }
 template <typename T, int V>
 __device__ __forceinline__ void store_vec(T* p, const float (&f)[V]) {
   Vec<T, V> v;
+  if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(&v);
 #pragma unroll
-  for (int i = 0; i < V; ++i) v.e[i] = from_float<T>(f[i]);
-  *reinterpret_cast<Vec<T, V>*>(p) = v;
+    for (int i = 0; i < V / 2; ++i) w[i] = pack2<T>(f[2 * i], f[2 * i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v.e[i] = from_float<T>(f[i]);
+  }
+  if constexpr (V * sizeof(T) == 16)
+    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(&v);
+  else
+    *reinterpret_cast<Vec<T, V>*>(p) = v;
 }
+
+// The 16-byte vectors of the kernels below, worked on in pairs (two fp32
+// operations per instruction).
+template <typename T>
+struct Pairs {
+  static constexpr int kN = 8 / sizeof(T);  // pairs in 16 bytes
+};
+template <typename T>
+__device__ __forceinline__ void to_pairs(const uint4& w, float2 (&f)[Pairs<T>::kN]) {
+  if constexpr (sizeof(T) == 2) {
+    f[0] = unpack2<T>(w.x), f[1] = unpack2<T>(w.y), f[2] = unpack2<T>(w.z), f[3] = unpack2<T>(w.w);
+  } else {
+    f[0] = make_float2(__uint_as_float(w.x), __uint_as_float(w.y));
+    f[1] = make_float2(__uint_as_float(w.z), __uint_as_float(w.w));
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint4 from_pairs(const float2 (&f)[Pairs<T>::kN]) {
+  if constexpr (sizeof(T) == 2)
+    return make_uint4(pack2<T>(f[0].x, f[0].y), pack2<T>(f[1].x, f[1].y), pack2<T>(f[2].x, f[2].y), pack2<T>(f[3].x, f[3].y));
+  else
+    return make_uint4(__float_as_uint(f[0].x), __float_as_uint(f[0].y), __float_as_uint(f[1].x), __float_as_uint(f[1].y));
+}
+// 2 * N weights of type W (N pairs), 16-byte aligned for N * 2 * sizeof(W) >= 16.
+template <typename W, int N>
+__device__ __forceinline__ void load_pairs(const W* p, float2 (&f)[N]) {
+  if constexpr (sizeof(W) == 4) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const float4 v = *reinterpret_cast<const float4*>(p + 2 * i);
+      f[i] = make_float2(v.x, v.y);
+      f[i + 1] = make_float2(v.z, v.w);
+    }
+  } else {
+    static_assert(N == 4, "16-bit weights go with 16-bit rows");
+    to_pairs<W>(*reinterpret_cast<const uint4*>(p), f);
+  }
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
 // Sum over the CTA of K values at once, the result in every thread.  `red`
 // holds K * 32 floats; a caller that reduces again synchronises in between.
 template <int K>
+__device__ __forceinline__ void warp_sum(float (&v)[K]) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1)
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], off);
+}
+template <int K>
 __device__ __forceinline__ void block_sum(float (&v)[K], float* red) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = (blockDim.x + 31) >> 5;
-#pragma unroll
-  for (int k = 0; k < K; ++k)
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], off);
+  warp_sum<K>(v);
   if (lane == 0)
 #pragma unroll
     for (int k = 0; k < K; ++k) red[k * 32 + warp] = v[k];
   __syncthreads();
+  if (warps <= 8) {
+    // Every thread adds the few warps' sums itself, in warp order.
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = red[k * 32];
+    for (int w = 1; w < warps; ++w)
+#pragma unroll
+      for (int k = 0; k < K; ++k) v[k] += red[k * 32 + w];
+  } else {
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = lane < warps ? red[k * 32 + lane] : 0.f;
+    warp_sum<K>(v);
+  }
+}
+
+// block_sum for CTAs of at most eight warps that reduce once per row: `red`
+// holds K * 8 floats, zero where there is no warp, and every thread adds the
+// eight itself (two 16-byte reads), in warp order.
+template <int K>
+__device__ __forceinline__ void few_warps_sum(float (&v)[K], float* red) {
+  warp_sum<K>(v);
+  if ((threadIdx.x & 31) == 0)
+#pragma unroll
+    for (int k = 0; k < K; ++k) red[k * 8 + (threadIdx.x >> 5)] = v[k];
+  __syncthreads();
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    float s = lane < warps ? red[k * 32 + lane] : 0.f;
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    v[k] = s;
+    const float4 a = *reinterpret_cast<const float4*>(red + k * 8), b = *reinterpret_cast<const float4*>(red + k * 8 + 4);
+    v[k] = ((a.x + a.y) + (a.z + a.w)) + ((b.x + b.y) + (b.z + b.w));
   }
 }
 
@@ -106,8 +224,14 @@ __global__ void __launch_bounds__(kMaxThreads) layernorm_fwd_kernel(const LayerN
         float r[V];
         load_vec<T, V>(res + row * p.ld_res + c, r);
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[k][e] = to_float<T>(from_float<T>(v[k][e] + r[e]));
-        store_vec<T, V>(reinterpret_cast<T*>(p.x_out) + row * p.ld_xo + c, v[k]);
+        for (int e = 0; e < V; ++e) v[k][e] += r[e];
+        T* xo = reinterpret_cast<T*>(p.x_out) + row * p.ld_xo + c;
+        store_vec<T, V>(xo, v[k]);
+        // The norm is of the rounded sum.
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) v[k][e] = to_float<T>(from_float<T>(v[k][e]));
+        }
       }
 #pragma unroll
       for (int e = 0; e < V; ++e) sum[0] += v[k][e];
@@ -147,6 +271,143 @@ __global__ void __launch_bounds__(kMaxThreads) layernorm_fwd_kernel(const LayerN
       store_vec<T, V>(reinterpret_cast<T*>(p.y) + row * p.ld_y + c, o);
     }
   }
+}
+
+// Asynchronous 16-byte copies into shared memory that the copying thread
+// alone reads back: it waits for its own groups, no barrier is needed.
+__device__ __forceinline__ void copy16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
+               "l"(src)
+               : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
+}
+
+// A shared-memory read that the compiler may not merge with an earlier one.
+__device__ __forceinline__ uint4 read_again(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p)))
+               : "memory");
+  return v;
+}
+
+// The rows of a launch, streamed: each CTA takes rows blockIdx.x, + gridDim.x,
+// ... and has the next kStages - 1 of them on their way into shared memory
+// while it works on one, so that the memory stays busy across a row's two
+// reductions; weight and bias wait in registers for all of them (read anew for
+// every row they were the larger part of what L1 had to deliver).  16-byte
+// rows, NV vectors per thread.
+template <typename T, typename W, int NV, int kMaxThreads, int kMinCtas, int kStages>
+__global__ void __launch_bounds__(kMaxThreads, kMinCtas) layernorm_fwd_stream_kernel(const LayerNormParams p) {
+  constexpr int N = Pairs<T>::kN, V = 2 * N;
+  extern __shared__ __align__(16) uint8_t smem_copies[];
+  __shared__ __align__(16) float red[2][16];
+  const bool summed = p.residual != nullptr;
+  const int threads = blockDim.x;
+  const int c0 = threadIdx.x * V, step = threads * V;  // first column, columns between vectors
+  if (threadIdx.x < 32) red[threadIdx.x >> 4][threadIdx.x & 15] = 0.f;
+  __syncthreads();
+  float2 w[NV][N], b[NV][N];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = c0 + k * step;
+#pragma unroll
+    for (int e = 0; e < N; ++e) w[k][e] = b[k][e] = both(0.f);
+    if (c < p.cols) {
+      load_pairs<W, N>(reinterpret_cast<const W*>(p.w) + c, w[k]);
+      if (p.bias != nullptr) load_pairs<W, N>(reinterpret_cast<const W*>(p.bias) + c, b[k]);
+    }
+  }
+  // Pointers to this thread's first column of the row being fetched and of the
+  // one being worked on, moved from row to row.
+  const int64_t rows_apart = gridDim.x;
+  const T* fx = reinterpret_cast<const T*>(p.x) + blockIdx.x * p.ld_x + c0;
+  const T* fr = reinterpret_cast<const T*>(p.residual) + blockIdx.x * p.ld_res + c0;
+  T* y = reinterpret_cast<T*>(p.y) + blockIdx.x * p.ld_y + c0;
+  T* xo = reinterpret_cast<T*>(p.x_out) + blockIdx.x * p.ld_xo + c0;
+  const int64_t dx = rows_apart * p.ld_x, dr = rows_apart * p.ld_res, dy = rows_apart * p.ld_y, dxo = rows_apart * p.ld_xo;
+  // This thread's vectors of a stage: x at [k], the residual at [NV + k].
+  uint4* const mine = reinterpret_cast<uint4*>(smem_copies) + threadIdx.x;
+  const int stage_size = 2 * NV * threads;
+  int64_t fetch_row = blockIdx.x;
+  auto fetch = [&](uint4* to) {
+    if (fetch_row < p.rows) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+        if (c0 + k * step < p.cols) {
+          copy16(to + k * threads, fx + k * step);
+          if (summed) copy16(to + (NV + k) * threads, fr + k * step);
+        }
+    }
+    copy_commit();
+    fetch_row += rows_apart;
+    fx += dx;
+    fr += dr;
+  };
+  const float inv = 1.f / static_cast<float>(p.cols);
+  uint4* to = mine;
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s, to += stage_size) fetch(to);
+  const uint4* from = mine;
+  uint4* const end = mine + kStages * stage_size;
+  for (int64_t row = blockIdx.x; row < p.rows; row += rows_apart, y += dy, xo += dxo) {
+    fetch(to);
+    if ((to += stage_size) == end) to = mine;
+    copy_wait<kStages - 1>();
+    float2 f[NV][N];
+    float2 sum2 = both(0.f);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if (c0 + k * step < p.cols) {
+        to_pairs<T>(from[k * threads], f[k]);
+        if (summed) {
+          float2 r[N];
+          to_pairs<T>(from[(NV + k) * threads], r);
+#pragma unroll
+          for (int e = 0; e < N; ++e) r[e] = __fadd2_rn(f[k][e], r[e]);
+          const uint4 raw = from_pairs<T>(r);
+          *reinterpret_cast<uint4*>(xo + k * step) = raw;
+          to_pairs<T>(raw, f[k]);  // the norm is of the rounded sum
+        }
+#pragma unroll
+        for (int e = 0; e < N; ++e) sum2 = __fadd2_rn(sum2, f[k][e]);
+      }
+    }
+    if ((from += stage_size) == end) from = mine;
+    float sum[1] = {sum2.x + sum2.y};
+    few_warps_sum<1>(sum, red[0]);
+    const float mean = sum[0] * inv;
+    float2 sq2 = both(0.f);
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if (c0 + k * step < p.cols)
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          f[k][e] = __fadd2_rn(f[k][e], both(-mean));
+          sq2 = __ffma2_rn(f[k][e], f[k][e], sq2);
+        }
+    float sq[1] = {sq2.x + sq2.y};
+    // Each reduction's barrier also frees the other's buffer.
+    few_warps_sum<1>(sq, red[1]);
+    const float rstd = rsqrtf(sq[0] * inv + p.eps);
+    if (threadIdx.x == 0 && p.mean != nullptr) {
+      p.mean[row] = mean;
+      p.rstd[row] = rstd;
+    }
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if (c0 + k * step < p.cols) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[k][e] = __ffma2_rn(__fmul2_rn(f[k][e], both(rstd)), w[k][e], b[k][e]);
+        *reinterpret_cast<uint4*>(y + k * step) = from_pairs<T>(f[k]);
+      }
+  }
+  copy_wait<0>();
 }
 
 // Rows too long for the registers of one CTA: the same sums over three reads
@@ -207,75 +468,225 @@ struct LayerNormBwdParams {
 // With xhat = (x - mean) * rstd and g = dy * w:
 //   dx = rstd * (g - mean(g) - xhat * mean(g * xhat)) + dres
 //   dw = sum_rows dy * xhat,  db = sum_rows dy
-// CTA i takes rows i, i + gridDim.x, ...; a thread keeps the same columns for
-// all of them, so its share of dw and db stays in registers and leaves once
-// per CTA.
-template <typename T, typename W, int V, int NV, int kMaxThreads>
-__global__ void __launch_bounds__(kMaxThreads) layernorm_bwd_kernel(const LayerNormBwdParams p) {
-  __shared__ float red[2][64];
-  float dw[NV][V], db[NV][V];
+// Memory-bound: dy, x (and dres) in, dx out, each once.  A row belongs to one
+// warp (kWarpRow, short rows: no barrier at all) or to the whole CTA; a
+// "worker" (warp or CTA) i takes rows i, i + workers, ...  A thread keeps the
+// same columns for all of them, so its share of dw and db stays in registers
+// and leaves once.  The next kStages - 1 rows are on their way into shared
+// memory while one is worked on, which keeps the memory busy across the
+// reduction that every row has in its middle; the weight waits in registers.
+template <typename T, typename W, int NV, int kMaxThreads, int kMinCtas, bool kWarpRow, int kStages>
+__global__ void __launch_bounds__(kMaxThreads, kMinCtas) layernorm_bwd_kernel(const LayerNormBwdParams p) {
+  constexpr int N = Pairs<T>::kN, V = 2 * N;
+  extern __shared__ __align__(16) uint8_t smem_copies[];
+  __shared__ __align__(16) float red[2][16];
+  const int threads = blockDim.x;
+  const int lanes = kWarpRow ? 32 : threads;  // threads of a row
+  const int me = kWarpRow ? threadIdx.x & 31 : threadIdx.x;
+  const int64_t worker = kWarpRow ? static_cast<int64_t>(blockIdx.x) * (threads >> 5) + (threadIdx.x >> 5) : blockIdx.x;
+  const int64_t workers = kWarpRow ? static_cast<int64_t>(gridDim.x) * (threads >> 5) : gridDim.x;
+  const int c0 = me * V, step = lanes * V;  // first column, columns between vectors
+  const bool summed = p.dres != nullptr;
+  if (threadIdx.x < 32) red[threadIdx.x >> 4][threadIdx.x & 15] = 0.f;
+  __syncthreads();
+  float2 w[NV][N], dw[NV][N], db[NV][N];
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
+    const int c = c0 + k * step;
 #pragma unroll
-    for (int e = 0; e < V; ++e) dw[k][e] = db[k][e] = 0.f;
+    for (int e = 0; e < N; ++e) w[k][e] = dw[k][e] = db[k][e] = both(0.f);
+    if (c < p.cols) load_pairs<W, N>(reinterpret_cast<const W*>(p.w) + c, w[k]);
   }
+  const float inv = 1.f / static_cast<float>(p.cols);
+  // Pointers to this thread's first column of the row being fetched and of the
+  // one being worked on, moved from row to row.
+  const T* fx = reinterpret_cast<const T*>(p.x) + worker * p.ld_x + c0;
+  const T* fg = reinterpret_cast<const T*>(p.dy) + worker * p.ld_dy + c0;
+  const T* fr = reinterpret_cast<const T*>(p.dres) + worker * p.ld_dres + c0;
+  T* out = reinterpret_cast<T*>(p.dx) + worker * p.ld_dx + c0;
+  const int64_t ax = workers * p.ld_x, ag = workers * p.ld_dy, ar = workers * p.ld_dres, ao = workers * p.ld_dx;
+  // This thread's vectors of a stage: x at [k], dy at [NV + k], dres after.
+  uint4* const mine = reinterpret_cast<uint4*>(smem_copies) + threadIdx.x;
+  const int stage_size = 3 * NV * threads;
+  int64_t fetch_row = worker;
+  auto fetch = [&](uint4* to) {
+    if (fetch_row < p.rows) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+        if (c0 + k * step < p.cols) {
+          copy16(to + k * threads, fx + k * step);
+          copy16(to + (NV + k) * threads, fg + k * step);
+          if (summed) copy16(to + (2 * NV + k) * threads, fr + k * step);
+        }
+    }
+    copy_commit();
+    fetch_row += workers;
+    fx += ax;
+    fg += ag;
+    fr += ar;
+  };
+  uint4* to = mine;
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s, to += stage_size) fetch(to);
+  const uint4* from = mine;
+  uint4* const end = mine + kStages * stage_size;
+  int turn = 0;
+  float next_mean = 0.f, next_rstd = 0.f;
+  if (worker < p.rows) {
+    next_mean = p.mean[worker];
+    next_rstd = p.rstd[worker];
+  }
+  for (int64_t row = worker; row < p.rows; row += workers, turn ^= 1, out += ao) {
+    fetch(to);
+    if ((to += stage_size) == end) to = mine;
+    const float2 scale = both(next_rstd), less = both(-next_mean);
+    if (row + workers < p.rows) {  // the next row's, a row ahead of their use
+      next_mean = p.mean[row + workers];
+      next_rstd = p.rstd[row + workers];
+    }
+    copy_wait<kStages - 1>();
+    float2 s0 = both(0.f), s1 = both(0.f);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if (c0 + k * step < p.cols) {
+        // Read again after the reduction rather than held across it: the
+        // registers buy another resident CTA.
+        float2 h[N], g[N];
+        to_pairs<T>(from[k * threads], h);
+        to_pairs<T>(from[(NV + k) * threads], g);
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          h[e] = __fmul2_rn(__fadd2_rn(h[e], less), scale);
+          dw[k][e] = __ffma2_rn(g[e], h[e], dw[k][e]);
+          db[k][e] = __fadd2_rn(db[k][e], g[e]);
+          g[e] = __fmul2_rn(g[e], w[k][e]);
+          s0 = __fadd2_rn(s0, g[e]);
+          s1 = __ffma2_rn(g[e], h[e], s1);
+        }
+      }
+    }
+    float s[2] = {s0.x + s0.y, s1.x + s1.y};
+    if constexpr (kWarpRow)
+      warp_sum<2>(s);
+    else
+      few_warps_sum<2>(s, red[turn]);  // the other buffer is free again: every thread has passed this row's barrier
+    const float2 na = both(-s[0] * inv), nb = both(-s[1] * inv);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if (c0 + k * step < p.cols) {
+        float2 h[N], g[N];
+        to_pairs<T>(read_again(from + k * threads), h);
+        to_pairs<T>(read_again(from + (NV + k) * threads), g);
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          h[e] = __fmul2_rn(__fadd2_rn(h[e], less), scale);
+          g[e] = __ffma2_rn(g[e], w[k][e], __ffma2_rn(h[e], nb, na));
+          g[e] = __fmul2_rn(g[e], scale);
+        }
+        if (summed) {
+          float2 r[N];
+          to_pairs<T>(from[(2 * NV + k) * threads], r);
+#pragma unroll
+          for (int e = 0; e < N; ++e) g[e] = __fadd2_rn(g[e], r[e]);
+        }
+        *reinterpret_cast<uint4*>(out + k * step) = from_pairs<T>(g);
+      }
+    }
+    if ((from += stage_size) == end) from = mine;
+  }
+  copy_wait<0>();
+  if (p.part == nullptr) return;
+  float* part = p.part + static_cast<int64_t>(blockIdx.x) * 2 * p.cols;
+  if constexpr (kWarpRow) {
+    // The warps' sums meet in shared memory, in warp order.
+    __syncthreads();
+    float* sums = reinterpret_cast<float*>(smem_copies);
+    const int warps = threads >> 5;
+    for (int which = 0; which < 2; ++which) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+        if (c0 + k * step < p.cols)
+#pragma unroll
+          for (int e = 0; e < N; ++e)
+            *reinterpret_cast<float2*>(sums + (threadIdx.x >> 5) * p.cols + c0 + k * step + 2 * e) = which ? db[k][e] : dw[k][e];
+      __syncthreads();
+      for (int c = threadIdx.x; c < p.cols; c += threads) {
+        float v = sums[c];
+        for (int x = 1; x < warps; ++x) v += sums[x * p.cols + c];
+        part[which * p.cols + c] = v;
+      }
+      __syncthreads();
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = c0 + k * step;
+      if (c < p.cols)
+#pragma unroll
+        for (int e = 0; e < N; e += 2) {
+          *reinterpret_cast<float4*>(part + c + 2 * e) = make_float4(dw[k][e].x, dw[k][e].y, dw[k][e + 1].x, dw[k][e + 1].y);
+          *reinterpret_cast<float4*>(part + p.cols + c + 2 * e) =
+              make_float4(db[k][e].x, db[k][e].y, db[k][e + 1].x, db[k][e + 1].y);
+        }
+    }
+  }
+}
+
+// The same for rows off the 16-byte grid, one value per access, a CTA per row.
+template <typename T, typename W, int NV, int kMaxThreads>
+__global__ void __launch_bounds__(kMaxThreads) layernorm_bwd_any_kernel(const LayerNormBwdParams p) {
+  __shared__ float red[2][64];
+  float dw[NV], db[NV];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) dw[k] = db[k] = 0.f;
   const float inv = 1.f / static_cast<float>(p.cols);
   int turn = 0;
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
     const T* x = reinterpret_cast<const T*>(p.x) + row * p.ld_x;
     const T* dy = reinterpret_cast<const T*>(p.dy) + row * p.ld_dy;
+    const T* res = reinterpret_cast<const T*>(p.dres) + row * p.ld_dres;
     const float mean = p.mean[row], rstd = p.rstd[row];
-    float h[NV][V], g[NV][V];
+    float h[NV], g[NV], r[NV];
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int c = (threadIdx.x + k * blockDim.x) * V;
+      const int c = threadIdx.x + k * blockDim.x;
+      h[k] = g[k] = r[k] = 0.f;
       if (c < p.cols) {
-        load_vec<T, V>(x + c, h[k]);
-        load_vec<T, V>(dy + c, g[k]);
-        float w[V];
-        load_vec<W, V>(reinterpret_cast<const W*>(p.w) + c, w);
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          h[k][e] = (h[k][e] - mean) * rstd;
-          dw[k][e] = fmaf(g[k][e], h[k][e], dw[k][e]);
-          db[k][e] += g[k][e];
-          g[k][e] *= w[e];
-          s[0] += g[k][e];
-          s[1] = fmaf(g[k][e], h[k][e], s[1]);
-        }
+        h[k] = to_float<T>(x[c]);
+        g[k] = to_float<T>(dy[c]);
+        if (p.dres != nullptr) r[k] = to_float<T>(res[c]);
       }
     }
-    block_sum<2>(s, red[turn]);  // the other buffer is free again: every thread has passed this row's barrier
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = threadIdx.x + k * blockDim.x;
+      if (c < p.cols) {
+        h[k] = (h[k] - mean) * rstd;
+        dw[k] = fmaf(g[k], h[k], dw[k]);
+        db[k] += g[k];
+        g[k] *= to_float<W>(reinterpret_cast<const W*>(p.w)[c]);
+        s[0] += g[k];
+        s[1] = fmaf(g[k], h[k], s[1]);
+      }
+    }
+    block_sum<2>(s, red[turn]);
     const float a = s[0] * inv, b = s[1] * inv;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int c = (threadIdx.x + k * blockDim.x) * V;
-      if (c < p.cols) {
-        float o[V];
-#pragma unroll
-        for (int e = 0; e < V; ++e) o[e] = rstd * (g[k][e] - fmaf(h[k][e], b, a));
-        if (p.dres != nullptr) {
-          float r[V];
-          load_vec<T, V>(reinterpret_cast<const T*>(p.dres) + row * p.ld_dres + c, r);
-#pragma unroll
-          for (int e = 0; e < V; ++e) o[e] += r[e];
-        }
-        store_vec<T, V>(reinterpret_cast<T*>(p.dx) + row * p.ld_dx + c, o);
-      }
+      const int c = threadIdx.x + k * blockDim.x;
+      if (c < p.cols)
+        reinterpret_cast<T*>(p.dx)[row * p.ld_dx + c] = from_float<T>(rstd * (g[k] - fmaf(h[k], b, a)) + r[k]);
     }
   }
-  if (p.part != nullptr) {
-    float* out = p.part + static_cast<int64_t>(blockIdx.x) * 2 * p.cols;
+  if (p.part == nullptr) return;
+  float* out = p.part + static_cast<int64_t>(blockIdx.x) * 2 * p.cols;
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int c = (threadIdx.x + k * blockDim.x) * V;
-      if (c < p.cols)
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          out[c + e] = dw[k][e];
-          out[p.cols + c + e] = db[k][e];
-        }
+  for (int k = 0; k < NV; ++k) {
+    const int c = threadIdx.x + k * blockDim.x;
+    if (c < p.cols) {
+      out[c] = dw[k];
+      out[p.cols + c] = db[k];
     }
   }
 }
@@ -324,23 +735,23 @@ __global__ void __launch_bounds__(1024) layernorm_bwd_long_cols_kernel(const Lay
 }
 
 // dw[c] = sum_i part[i][0][c], db[c] = sum_i part[i][1][c], in a fixed order:
-// 32 columns per CTA, eight warps take every eighth line, their sums are added
-// in warp order.
+// 32 columns per CTA, warp x takes lines x, x + 32, ... (its loads all under
+// way together), the warps' sums are added in warp order.
 template <typename W>
-__global__ void __launch_bounds__(256) layernorm_bwd_finish_kernel(const float* __restrict__ part, int lines, int cols,
-                                                                   W* dw, W* db) {
-  __shared__ float sums[8][32];
+__global__ void __launch_bounds__(1024) layernorm_bwd_finish_kernel(const float* part, int lines, int cols, W* dw, W* db) {
+  __shared__ float sums[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int j = blockIdx.x * 32 + lane;  // column of [dw | db]
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   float s = 0.f;
   if (j < 2 * cols)
-#pragma unroll 4
-    for (int i = warp; i < lines; i += 8) s += part[static_cast<int64_t>(i) * 2 * cols + j];
+#pragma unroll 8
+    for (int i = warp; i < lines; i += 32) s += part[static_cast<int64_t>(i) * 2 * cols + j];
   sums[warp][lane] = s;
   __syncthreads();
   if (warp == 0 && j < 2 * cols) {
 #pragma unroll
-    for (int k = 1; k < 8; ++k) s += sums[k][lane];
+    for (int k = 1; k < 32; ++k) s += sums[k][lane];
     W* out = j < cols ? dw : db;
     if (out != nullptr) out[j < cols ? j : j - cols] = from_float<W>(s);
   }
@@ -365,6 +776,8 @@ struct RopeParams {
   int table_rows;
   float sin_sign;  // -1: the inverse rotation
   int pos64;
+  int vec_table;  // every V pairs of a thread follow one axis and lie 16-byte aligned in the tables
+  int slots;      // threads that share a token's heads
 };
 
 __device__ __forceinline__ int rope_axis(const RopeParams& p, int i) {
@@ -381,55 +794,90 @@ __device__ __forceinline__ int rope_row(const RopeParams& p, int axis, int64_t t
   return r >= 0 && r < p.table_rows ? static_cast<int>(r) : -1;
 }
 
-// One CTA per token (and per gridDim.y share of its heads).  Thread vi of a
-// head slot owns V pairs of every head of the slot: their cosines and sines
-// are read once and used for all of them.  A position outside the table makes
-// its pairs NaN; nothing is read out of bounds.
+// Thread (token, slot, vi) owns V pairs of kRopeHeads heads (slot, slot +
+// slots, ...): their cosines and sines are read once for all of them, and all
+// of their loads are under way before the first is used.  Memory-bound: q and
+// k in and out once; the table rows stay in L1 and L2.  A position outside the
+// table makes its pairs NaN; nothing is read out of bounds.
+constexpr int kRopeHeads = 2;
 template <typename T, int V>
-__global__ void __launch_bounds__(256) rope_axes_kernel(const RopeParams p) {
-  const int64_t t = blockIdx.x;
-  const int rot = p.half / V;                         // vectors of pairs
+__global__ void __launch_bounds__(256, 4) rope_axes_kernel(const RopeParams p) {
+  const int rot = p.half / V;                            // vectors of pairs
   const int nvec = rot + (p.head_dim - 2 * p.half) / V;  // and of columns to copy
-  const int slots = blockDim.x / nvec;
-  const int vi = threadIdx.x % nvec;
-  const int slot = threadIdx.x / nvec;
-  if (slot >= slots) return;
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  const int per_token = nvec * p.slots;
+  const int64_t t = id / per_token;
+  if (t >= p.tokens) return;
+  const int in_token = static_cast<int>(id - t * per_token);
+  const int slot = in_token / nvec, vi = in_token - slot * nvec;
+  const int heads = p.heads_q + p.heads_k;
+  const bool turns = vi < rot;
+  const int c0 = turns ? vi * V : 2 * p.half + (vi - rot) * V;
+  // Loads of every head first.
+  Vec<T, V> lo[kRopeHeads], hi[kRopeHeads];
+  T* out[kRopeHeads];
+#pragma unroll
+  for (int j = 0; j < kRopeHeads; ++j) {
+    const int h = slot + j * p.slots;
+    if (h >= heads) continue;
+    const bool is_k = h >= p.heads_q;
+    const int hh = is_k ? h - p.heads_q : h;
+    const T* in = reinterpret_cast<const T*>(is_k ? p.k : p.q) + t * (is_k ? p.k_st : p.q_st) + hh * (is_k ? p.k_sh : p.q_sh) + c0;
+    out[j] = reinterpret_cast<T*>(is_k ? p.k_out : p.q_out) + t * (is_k ? p.ko_st : p.qo_st) + hh * (is_k ? p.ko_sh : p.qo_sh) + c0;
+    lo[j] = *reinterpret_cast<const Vec<T, V>*>(in);
+    if (turns) hi[j] = *reinterpret_cast<const Vec<T, V>*>(in + p.half);
+  }
+  if (!turns) {
+#pragma unroll
+    for (int j = 0; j < kRopeHeads; ++j)
+      if (slot + j * p.slots < heads) *reinterpret_cast<Vec<T, V>*>(out[j]) = lo[j];
+    return;
+  }
   float c[V], s[V];
-  if (vi < rot) {
+  if (V >= 4 && p.vec_table) {
+    const int row = rope_row(p, rope_axis(p, c0), t);
+#pragma unroll
+    for (int e = 0; e < V; e += 4) {
+      const int64_t at = static_cast<int64_t>(row < 0 ? 0 : row) * p.half + c0 + e;
+      float4 cv = make_float4(NAN, NAN, NAN, NAN), sv = cv;
+      if (row >= 0) {
+        cv = *reinterpret_cast<const float4*>(p.cos + at);
+        sv = *reinterpret_cast<const float4*>(p.sin + at);
+      }
+      c[e] = cv.x, s[e] = sv.x;
+      if constexpr (V >= 4) {
+        c[e + 1] = cv.y, c[e + 2] = cv.z, c[e + 3] = cv.w;
+        s[e + 1] = sv.y, s[e + 2] = sv.z, s[e + 3] = sv.w;
+      }
+    }
+  } else {
     int last_axis = -1, row = -1;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const int i = vi * V + e;
-      const int a = rope_axis(p, i);
+      const int a = rope_axis(p, c0 + e);
       if (a != last_axis) {
         row = rope_row(p, a, t);
         last_axis = a;
       }
-      c[e] = row < 0 ? NAN : p.cos[static_cast<int64_t>(row) * p.half + i];
-      s[e] = row < 0 ? NAN : p.sin[static_cast<int64_t>(row) * p.half + i] * p.sin_sign;
+      c[e] = row < 0 ? NAN : p.cos[static_cast<int64_t>(row) * p.half + c0 + e];
+      s[e] = row < 0 ? NAN : p.sin[static_cast<int64_t>(row) * p.half + c0 + e];
     }
   }
-  for (int h = blockIdx.y * slots + slot; h < p.heads_q + p.heads_k; h += slots * gridDim.y) {
-    const bool is_k = h >= p.heads_q;
-    const int hh = is_k ? h - p.heads_q : h;
-    const T* in = reinterpret_cast<const T*>(is_k ? p.k : p.q) + t * (is_k ? p.k_st : p.q_st) + hh * (is_k ? p.k_sh : p.q_sh);
-    T* out = reinterpret_cast<T*>(is_k ? p.k_out : p.q_out) + t * (is_k ? p.ko_st : p.qo_st) + hh * (is_k ? p.ko_sh : p.qo_sh);
-    if (vi < rot) {
-      const int i = vi * V;
-      float lo[V], hi[V], a[V], b[V];
-      load_vec<T, V>(in + i, lo);
-      load_vec<T, V>(in + p.half + i, hi);
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        a[e] = lo[e] * c[e] - hi[e] * s[e];
-        b[e] = hi[e] * c[e] + lo[e] * s[e];
-      }
-      store_vec<T, V>(out + i, a);
-      store_vec<T, V>(out + p.half + i, b);
-    } else {
-      const int i = 2 * p.half + (vi - rot) * V;
-      *reinterpret_cast<Vec<T, V>*>(out + i) = *reinterpret_cast<const Vec<T, V>*>(in + i);
+  for (int e = 0; e < V; ++e) s[e] *= p.sin_sign;
+#pragma unroll
+  for (int j = 0; j < kRopeHeads; ++j) {
+    if (slot + j * p.slots >= heads) continue;
+    float l[V], u[V], a[V], b[V];
+    to_floats<T, V>(lo[j], l);
+    to_floats<T, V>(hi[j], u);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      a[e] = l[e] * c[e] - u[e] * s[e];
+      b[e] = u[e] * c[e] + l[e] * s[e];
     }
+    store_vec<T, V>(out[j], a);
+    store_vec<T, V>(out[j] + p.half, b);
   }
 }
 

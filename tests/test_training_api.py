@@ -128,7 +128,7 @@ def test_layernorm_backward_refuses_before_any_launch():
     assert call(dtype=1, w_dtype=0) == _native.FAB_ERR_UNSUPPORTED
     assert call(rows=0, dw=None, db=None) == _native.FAB_OK
     need = ctypes.c_size_t(0)
-    assert _native.lib.fab_layernorm_bwd_workspace(1 << 20, 1 << 20, ctypes.byref(need)) == _native.FAB_OK
+    assert _native.lib.fab_layernorm_bwd_workspace(1 << 20, 1 << 21, ctypes.byref(need)) == _native.FAB_OK
     assert need.value > 1 << 31  # counted in 64 bits
 
 
