@@ -325,6 +325,8 @@ __device__ __forceinline__ void bwd_store_chunk(int64_t row, int64_t stride, int
 // warp leaves its code in the abort flag and unwinds.
 constexpr uint32_t kWaitTries = 4000000;
 __device__ __forceinline__ bool bwd_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int code) {
+  // Usually complete already: one test, no loop.
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
   uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t.reg .u32 n, a;\n\t"
@@ -771,24 +773,6 @@ __device__ __forceinline__ bool bwd_issue(const BwdCta<kDP>& c, uint32_t tmem, b
 }
 
 // ----------------------------------------------------------------- softmax
-// Sets columns outside [lo, hi) of this lane's kCols columns to `value`, in
-// TMEM: the few tiles that the mask's edge crosses are prepared with this, so
-// that one copy of the code below serves all.
-template <int kCols>
-__device__ __forceinline__ void bwd_mask(uint32_t addr, int lo, int hi, uint32_t value) {
-#pragma unroll 1
-  for (int cc = 0; cc < kCols; cc += 32) {
-    uint32_t rr[32];
-    tmem_ld32(addr + cc, rr);
-    tmem_wait_ld();
-#pragma unroll
-    for (int e = 0; e < 32; ++e)
-      if (cc + e < lo || cc + e >= hi) rr[e] = value;
-    tmem_st32(addr + cc, rr);
-  }
-  tmem_wait_st();
-}
-
 struct BwdSoftmax {
   BwdPos it, item, stat;
 };
@@ -823,7 +807,6 @@ __device__ __forceinline__ bool bwd_tiles(const FaBwdParams& p, const BwdCta<kDP
     if (kDkv && !bwd_wait(c.st_full + n.stat.slot, n.stat.phase, c.abort_flag, kDevTimeoutKV)) return false;
     if (!bwd_wait(c.s, n.it.phase, c.abort_flag, kDevTimeoutS)) return false;
     tc_fence_after();
-    if (need_mask) bwd_mask<kCols>(tS, lo, hi, out);
     // Chunks of 32 columns; the next one's load is under way while one is
     // worked on.
     float pr[kCols];
@@ -841,6 +824,11 @@ __device__ __forceinline__ bool bwd_tiles(const FaBwdParams& p, const BwdCta<kDP
       if (kDkv && C::kHalves && cc == 1) {
         tmem_wait_st();
         arrive(c.pr);
+      }
+      if (need_mask) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          if (cc * 32 + e < lo || cc * 32 + e >= hi) rr[cc][e] = out;
       }
       [[maybe_unused]] uint32_t pk[16];
 #pragma unroll
@@ -870,8 +858,6 @@ __device__ __forceinline__ bool bwd_tiles(const FaBwdParams& p, const BwdCta<kDP
     }
     if (!bwd_wait(c.dp, n.it.phase, c.abort_flag, kDevTimeoutS)) return false;
     tc_fence_after();
-    // P is 0 where nothing is visible, but dP may be infinite or NaN.
-    if (need_mask) bwd_mask<kCols>(tP, lo, hi, 0u);
     tmem_ld32(tP, rr[0]);
 #pragma unroll
     for (int cc = 0; cc < kChunks; ++cc) {
