@@ -34,7 +34,7 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 size_t round256(size_t x) { return (x + 255) / 256 * 256; }
 
 // A slice no shorter than this is worth its own read-out (see choose_slices).
-constexpr int64_t kMinSliceTiles = 4;
+constexpr int64_t kMinSliceTiles = 6;
 constexpr int kSms = 148;  // plans depend on sizes only, so that results do not depend on the device at hand
 
 // What a call launches and how its workspace is laid out (byte offsets).
@@ -61,9 +61,16 @@ int64_t streamed_tiles(int64_t tiles, int64_t other_rows, int bs, bool causal, b
 }
 
 // Slices of the longest tile's `longest` streamed tiles when an SM's share of
-// the whole work is `share` of them.  Measured on B200: FILL IN.
+// the whole work is `share` of them: a tile half as long again as 5/4 of the
+// share would finish last, alone.  A slice costs a round of fp32 sums and the
+// join kernel.  Measured on B200, sliced and unsliced: 28 heads over 4, S 2048
+// causal 114 against 183 us; 4 over 1, S 4096, D 256 causal 200 against 359;
+// 8 heads, 1 query, 32768 keys 124 against 364; one head, S 1024 causal, 41
+// against 59.  Slices of half the share cost 8 to 50 % more than these, of
+// 3/2 of it up to 14 % (one head, S 8192, causal); a minimum of 4 tiles 20 %
+// more at one head, S 1024.
 void choose_slices(int64_t longest, double share, int* len, int* slices) {
-  const int64_t want = std::max<int64_t>(kMinSliceTiles, static_cast<int64_t>(share / 2 + 0.5));
+  const int64_t want = std::max<int64_t>(kMinSliceTiles, static_cast<int64_t>(share * 1.25 + 0.5));
   *len = static_cast<int>(std::min<int64_t>(longest < 1 ? 1 : longest, want));
   *slices = 1;
   if (longest * 2 >= want * 3) *slices = static_cast<int>(std::min<int64_t>(ceil_div(longest, want), 1 << 15));

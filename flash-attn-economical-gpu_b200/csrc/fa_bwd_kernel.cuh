@@ -93,15 +93,6 @@ struct BwdElem<__half> {
 // S(i) and again by dK(i) or dQ(i), a whole tile's time later, and its next
 // load has only until S two tiles on to land; the second (dO, or V) is done
 // with half a tile after it is first read.  So the first ring is the longer.
-#ifndef FAB_BWD_HALVES
-#define FAB_BWD_HALVES 1
-#endif
-#ifndef FAB_BWD_TURNS
-#define FAB_BWD_TURNS 1
-#endif
-#ifndef FAB_BWD_PASS
-#define FAB_BWD_PASS (kDP / 32)
-#endif
 template <int kDP_>
 struct BwdCfg {
   static constexpr int kDP = kDP_;
@@ -125,7 +116,7 @@ struct BwdCfg {
       2 * kABytes + (kRing0 + kRing1) * kBBytes + 2 * kStatBytes + kNumBars * 8 + kTailBytes;
   // P and dS are handed to the tensor core in two halves where a warp works
   // through two 32-column chunks.
-  static constexpr bool kHalves = kBS == 128 && FAB_BWD_HALVES;
+  static constexpr bool kHalves = kBS == 128;
   static constexpr int kThreads = 384;
   // Launched with 168 registers a thread; the load/MMA warpgroup hands some
   // to the two softmax warpgroups, which hold a 64-column row of P across

@@ -126,6 +126,56 @@ def test_any_softmax_scale(scale, cuda_device):
     _assert_within(got, *_reference(dout, q, k, v, o, lse, False, scale))
 
 
+@pytest.mark.parametrize("scale", [-0.2, 0.0])
+def test_causal_with_any_softmax_scale(scale, cuda_device):
+    """Masked pairs stay out whatever the sign of the scale."""
+    dout, q, k, v = _inputs(1, 2, 1, 200, 170, 64, torch.bfloat16, cuda_device, 4)
+    o, lse = attention_forward(q, k, v, causal=True, sm_scale=scale, return_lse=True)
+    got = attention_backward(dout, q, k, v, o, lse, causal=True, sm_scale=scale)
+    _assert_within(got, *_reference(dout, q, k, v, o, lse, True, scale))
+
+
+SLICED = [
+    # few tiles of long sums, in parts that are joined; then many short items for each SM
+    (1, 1, 1, 40, 5000, 64, torch.bfloat16, False),
+    (1, 1, 1, 5000, 40, 128, torch.float16, False),
+    (1, 2, 1, 2500, 2500, 128, torch.bfloat16, True),
+    (1, 7, 1, 1100, 1100, 128, torch.bfloat16, True),
+    (1, 1, 1, 1700, 1300, 256, torch.float16, True),
+    (1, 2, 1, 90, 3333, 256, torch.bfloat16, False),
+    (1, 1, 1, 2049, 2049, 96, torch.float16, False),
+    (40, 24, 12, 130, 130, 64, torch.bfloat16, True),
+    (24, 16, 16, 70, 200, 128, torch.float16, False),
+    (17, 9, 3, 150, 129, 256, torch.bfloat16, True),
+]
+
+
+@pytest.mark.parametrize("case", SLICED, ids=lambda c: f"B{c[0]}H{c[1]}/{c[2]}M{c[3]}N{c[4]}D{c[5]}{str(c[6])[6:]}{'c' if c[7] else ''}")
+def test_long_sums_and_many_items(case, cuda_device):
+    B, Hq, Hkv, M, N, D, dtype, causal = case
+    dout, q, k, v = _inputs(B, Hq, Hkv, M, N, D, dtype, cuda_device, M * N + D)
+    o, lse = attention_forward(q, k, v, causal=causal, return_lse=True)
+    got = attention_backward(dout, q, k, v, o, lse, causal=causal)
+    _assert_within(got, *_reference(dout, q, k, v, o, lse, causal, D ** -0.5))
+    again = attention_backward(dout, q, k, v, o, lse, causal=causal)
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
+
+
+def test_offsets_past_32_bits(cuda_device):
+    """Heads and rows that lie more than 2^31 elements into their tensors, inputs and gradients alike."""
+    S, D, step = 150, 64, 1 << 30
+    base = torch.zeros(2 * step + S * D + 64, device=cuda_device, dtype=torch.bfloat16)
+    dout, q, k, v = _inputs(1, 3, 3, S, S, D, torch.bfloat16, cuda_device, 13)
+    far = base.as_strided((1, 3, S, D), (step, step, D, 1))
+    o, lse = attention_forward(q, k, v, causal=True, return_lse=True)
+    want = attention_backward(dout, q, k, v, o, lse, causal=True)
+    ok = dict(dout=dout, q=q, k=k, v=v, out=o)
+    for name in ok:
+        far.copy_(ok[name])
+        got = attention_backward(**{**ok, name: far}, lse=lse, causal=True)
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), name
+
+
 def test_strided_and_broadcast_inputs(cuda_device):
     """Column views of one packed projection, [B, S, H, D] outputs, a key/value head shared by expand, a dout of one
     repeated value."""
@@ -225,6 +275,9 @@ PACKED = [
     ((70, 33, 128), (99, 45, 128), 2, 2, 80, torch.bfloat16, True),
     ((3, 40, 4), (0, 40, 10), 2, 2, 64, torch.bfloat16, False),              # queries with no keys
     ((37, 1), (200, 129), 7, 1, 33, torch.float16, True),
+    (tuple(1 + 37 * i % 200 for i in range(60)), tuple(1 + 37 * i % 200 for i in range(60)), 3, 1, 64, torch.bfloat16, True),
+    ((1, 2000, 3), (2500, 2, 1), 1, 1, 128, torch.bfloat16, False),          # long sums of one sequence, in parts
+    ((1300, 1, 40), (1300, 1, 40), 2, 1, 256, torch.float16, True),
 ]
 
 
@@ -236,7 +289,7 @@ def _packed_inputs(lq, lk, Hq, Hkv, D, dtype, dev, seed):
     return dout, q, k, v, cu_q, cu_k
 
 
-@pytest.mark.parametrize("case", PACKED, ids=lambda c: f"q{c[0]}k{c[1]}H{c[2]}/{c[3]}D{c[4]}{str(c[5])[6:]}{'c' if c[6] else ''}")
+@pytest.mark.parametrize("case", PACKED, ids=lambda c: f"q{str(c[0])[:20]}k{str(c[1])[:20]}H{c[2]}/{c[3]}D{c[4]}{str(c[5])[6:]}{'c' if c[6] else ''}")
 def test_packed_matches_the_formula_per_sequence(case, cuda_device):
     lq, lk, Hq, Hkv, D, dtype, causal = case
     dout, q, k, v, cu_q, cu_k = _packed_inputs(lq, lk, Hq, Hkv, D, dtype, cuda_device, sum(lq))
