@@ -254,7 +254,7 @@ DEVICE_WAITS = {1: "a Q tile's load", 2: "a K/V tile's load", 3: "an S product",
                 5: "O's last product", 6: "a free K/V or stage slot", 7: "a GEMM accumulator",
                 8: "the drain at teardown", 9: "a peer rank's partial tile", 10: "a peer owner's reduced tile",
                 11: "a stream-K piece from another CTA pair", 12: "the CTA-pair GEMM's next tile from its scheduler",
-                13: "the split-KV merge's copies"}
+                13: "the split-KV merge's copies", 14: "the layer norm's row sums"}
 
 
 def raise_on_device_error() -> None:

@@ -953,7 +953,10 @@ int fab_get_device_error(int* code) {
   int w = 0;
   rc = fa_bwd_take_device_error(&w);
   if (rc) return rc;
-  *code = v != 0 ? v : g != 0 ? g : w;
+  int t = 0;
+  rc = train_ops_take_device_error(&t);
+  if (rc) return rc;
+  *code = v != 0 ? v : g != 0 ? g : w != 0 ? w : t;
   return kOk;
 }
 

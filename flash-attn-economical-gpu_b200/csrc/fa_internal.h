@@ -268,6 +268,8 @@ int gemm_kernel_attrs(int in_dtype, int* regs, int* smem, int* threads);
 int gemm_take_device_error(int* code);
 // The same for the attention backward's unit.
 int fa_bwd_take_device_error(int* code);
+// And for the training operators' unit.
+int train_ops_take_device_error(int* code);
 
 // Helpers implemented in capi.cu.
 int ensure_smem_attr(const void* kernel, int bytes);

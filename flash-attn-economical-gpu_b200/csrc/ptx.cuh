@@ -29,6 +29,7 @@ enum DeviceError : int {
   kDevTimeoutPartial = 11,   // a stream-K partial tile from another CTA pair never arrived
   kDevTimeoutSched = 12,     // the next tile from the cluster scheduler, or its slot's release, never came
   kDevTimeoutMerge = 13,     // the split-KV merge's copies of the partial rows never landed
+  kDevTimeoutRowSum = 14,    // a row's sums from another CTA of its cluster never came
 };
 
 // Device-global status word of the kernels of one translation unit (internal

@@ -1,6 +1,6 @@
 // Translation unit of the training operators around the attention: layer
 // norm and multi-axis rotary embedding (train_ops.cuh), with their C entry
-// points.  Their kernels have no device-side waits.
+// points.  The unit has its own copy of the device status word.
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
@@ -10,6 +10,18 @@
 #include "train_ops.cuh"
 
 namespace fab {
+
+int train_ops_take_device_error(int* code) {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_fab_device_error, sizeof(int)) != cudaSuccess) return kErrCuda;
+  if (v != 0) {
+    const int zero = 0;
+    if (cudaMemcpyToSymbol(g_fab_device_error, &zero, sizeof(int)) != cudaSuccess) return kErrCuda;
+  }
+  *code = v;
+  return kOk;
+}
+
 namespace {
 
 bool aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
@@ -44,40 +56,103 @@ int run_fwd(const LayerNormParams& p, cudaStream_t st) {
 // through resident CTAs; below, every row has a CTA of its own.
 constexpr int64_t kStreamRows = 3;
 
-template <typename T, typename W, int NV, int kMaxThreads, int kMinCtas>
-int run_fwd_stream(const LayerNormParams& p, cudaStream_t st) {
-  constexpr int kStages = 3;
-  auto kern = layernorm_fwd_stream_kernel<T, W, NV, kMaxThreads, kMinCtas, kStages>;
-  const int threads = row_threads(p.cols, 16 / sizeof(T), NV);
-  const int64_t ctas = std::min<int64_t>(p.rows, kSms * std::max(1, kResidentVectors / (threads * NV)));
-  const size_t smem = size_t(kStages) * NV * 2 * threads * 16;
-  if (int rc = ensure_smem_attr(reinterpret_cast<const void*>(kern), 200 * 1024)) return rc;
-  kern<<<static_cast<unsigned>(ctas), threads, smem, st>>>(p);
-  return launched();
+// Clusters of `ctas` CTAs that are resident together: all that the SMs have
+// room for, but the GPU's processing clusters are not a multiple of four CTAs
+// each.  (Measured: of the clusters of 4 and 8 that fill every SM some had to
+// wait for a second round; 4096 x 16384 fp32 backward 246 against 174 us.)
+int64_t resident(int64_t per_sm, int ctas) { return kSms * per_sm * (ctas > 2 ? 7 : 8) / (8 * ctas); }
+
+// How rows of `places` places (columns, and in front of them those of a cut
+// 16-byte piece) are shared out, `per_cta` at most to a CTA: the CTAs of a row
+// (a cluster where there are several), and each one's places.
+struct Spread {
+  int ctas, span;
+};
+Spread spread_row(int places, int per_cta, int unit) {
+  int ctas = 1;
+  while (int64_t(ctas) * per_cta < places) ctas *= 2;
+  return {ctas, static_cast<int>(ceil_div(ceil_div(places, ctas), unit) * unit)};
 }
+
+// Rows whose 16-byte pieces do not start where the rows do: workable all the
+// same where a row starts at the same place of a piece in every tensor.  Each
+// worker then takes every 8th row or a multiple of that, which start alike.
+enum class Rows { kEven, kOdd, kAny };
+struct RowTensor {
+  const void* p;  // or null
+  int64_t ld;
+};
+template <int N>
+Rows rows_kind(const RowTensor (&t)[N], int cols, int v, bool even_weights) {
+  bool even = even_weights && cols % v == 0, alike = true;
+  for (const RowTensor& x : t) {
+    if (x.p == nullptr) continue;
+    even = even && aligned(x.p, 16) && x.ld % v == 0;
+    alike = alike && (reinterpret_cast<uintptr_t>(x.p) - reinterpret_cast<uintptr_t>(t[0].p)) % 16 == 0 &&
+            (x.ld - t[0].ld) % v == 0 && x.ld >= 0;
+  }
+  return even ? Rows::kEven : alike ? Rows::kOdd : Rows::kAny;
+}
+int64_t like_workers(int64_t workers, int64_t rows, bool odd) {
+  return !odd || workers >= rows || workers < 8 ? std::min(workers, rows) : workers / 8 * 8;
+}
+
+// `workers` rows at a time, each on `ctas` CTAs.
+template <typename P>
+int launch_rows(void (*kern)(P), const P& p, int64_t workers, int ctas, int threads, size_t smem, cudaStream_t st) {
+  if (int rc = ensure_smem_attr(reinterpret_cast<const void*>(kern), 200 * 1024)) return rc;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(workers * ctas));
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = ctas;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = ctas > 1 ? 1 : 0;
+  if (cudaLaunchKernelEx(&cfg, kern, p) == cudaSuccess) return kOk;
+  cudaGetLastError();
+  return kErrLaunch;
+}
+
+template <typename T, typename W, int NV, int kMaxThreads, int kMinCtas, bool kWide, bool kOdd>
+int run_fwd_stream(LayerNormParams p, cudaStream_t st) {
+  constexpr int kStages = 3, V = 16 / sizeof(T);
+  const int places = p.cols + (kOdd ? V - 1 : 0);
+  const Spread row = spread_row(places, kWide ? 1024 * V : places, 32 * V);
+  p.span = row.span;
+  const int threads = row_threads(kWide ? row.span : places, V, NV);
+  const int64_t workers = like_workers(resident(std::max(1, kResidentVectors / (threads * NV)), row.ctas), p.rows, kOdd);
+  return launch_rows(layernorm_fwd_stream_kernel<T, W, NV, kMaxThreads, kMinCtas, kStages, kWide, kOdd>, p, workers, row.ctas,
+                     threads, size_t(kStages) * NV * 2 * threads * 16, st);
+}
+
+// Rows of any length and place.
+int long_threads(int cols) { return static_cast<int>(std::min<int64_t>(1024, ceil_div(cols, 32) * 32)); }
 
 template <typename T, typename W>
 int fwd(const LayerNormParams& p, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
-  const bool vec = p.cols % V == 0 && aligned(p.x, 16) && aligned(p.residual, 16) && aligned(p.w, 16) &&
-                   aligned(p.bias, 16) && aligned(p.y, 16) && aligned(p.x_out, 16) && p.ld_x % V == 0 &&
-                   p.ld_y % V == 0 && (p.residual == nullptr || (p.ld_res % V == 0 && p.ld_xo % V == 0));
-  if (vec && p.cols <= 1024 * V && p.rows >= kStreamRows * kSms * std::max(1, kResidentVectors / (p.cols / V))) {
-    if (p.cols <= 64 * V) return run_fwd_stream<T, W, 2, 32, 12>(p, st);
-    return run_fwd_stream<T, W, 4, 256, 2>(p, st);
+  const RowTensor rows[] = {{p.x, p.ld_x}, {p.y, p.ld_y}, {p.residual, p.ld_res}, {p.residual ? p.x_out : nullptr, p.ld_xo}};
+  const Rows kind = rows_kind(rows, p.cols, V, aligned(p.w, 16) && aligned(p.bias, 16));
+  if (kind == Rows::kOdd && p.cols + V - 1 <= 1024 * V) return run_fwd_stream<T, W, 4, 256, 2, false, true>(p, st);
+  if (kind == Rows::kOdd && p.cols + V - 1 <= kMaxCluster * 1024 * V) return run_fwd_stream<T, W, 4, 256, 2, true, true>(p, st);
+  if (kind == Rows::kEven && p.cols <= kMaxCluster * 1024 * V &&
+      p.rows >= kStreamRows * kSms * kResidentVectors / (p.cols / V)) {
+    if (p.cols <= 64 * V) return run_fwd_stream<T, W, 2, 32, 12, false, false>(p, st);
+    if (p.cols <= 1024 * V) return run_fwd_stream<T, W, 4, 256, 2, false, false>(p, st);
+    return run_fwd_stream<T, W, 4, 256, 2, true, false>(p, st);
   }
-  if (vec) {
+  if (kind == Rows::kEven) {
     // The fewest vectors per thread that keep the CTA within 512 threads, else
     // within 1024.
     if (p.cols <= 512 * V) return run_fwd<T, W, V, 1, 512>(p, st);
     if (p.cols <= 1024 * V) return run_fwd<T, W, V, 2, 512>(p, st);
     if (p.cols <= 4096 * V) return run_fwd<T, W, V, 4, 1024>(p, st);
-  } else {
-    if (p.cols <= 1024) return run_fwd<T, W, 1, 4, 256>(p, st);
-    if (p.cols <= 4096) return run_fwd<T, W, 1, 8, 512>(p, st);
-    if (p.cols <= 16384) return run_fwd<T, W, 1, 16, 1024>(p, st);
   }
-  layernorm_fwd_long_kernel<T, W><<<static_cast<unsigned>(p.rows), 1024, 0, st>>>(p);
+  layernorm_fwd_long_kernel<T, W><<<static_cast<unsigned>(p.rows), long_threads(p.cols), 0, st>>>(p);
   return launched();
 }
 
@@ -99,59 +174,57 @@ int launch_after(void (*kernel)(Args...), unsigned grid, unsigned block, cudaStr
   return kErrLaunch;
 }
 
-template <typename T, typename W, int NV, int kMaxThreads, int kMinCtas, bool kWarpRow>
-int run_bwd(const LayerNormBwdParams& p, int* lines, cudaStream_t st) {
+template <typename T, typename W, int NV, int kMaxThreads, int kMinCtas, bool kWarpRow, bool kWide, bool kOdd>
+int run_bwd(LayerNormBwdParams p, int* lines, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
-  const int threads = kWarpRow ? kMaxThreads : row_threads(p.cols, V, NV);
+  const int places = p.cols + (kOdd ? V - 1 : 0);
+  const Spread row = spread_row(places, kWide ? 1024 * V : places, 32 * V);
+  p.span = row.span;
+  const int threads = kWarpRow ? kMaxThreads : row_threads(kWide ? row.span : places, V, NV);
   // Rows on their way at once per worker, this one included.
   constexpr int kStages = 2;
-  auto kern = layernorm_bwd_kernel<T, W, NV, kMaxThreads, kMinCtas, kWarpRow, kStages>;
   size_t smem = size_t(kStages) * NV * 3 * threads * 16;
   const int vectors = threads * NV;  // of one row, or of all the warps' rows
-  *lines = static_cast<int>(std::min({kWarpRow ? ceil_div(p.rows, threads / 32) : p.rows,
-                                      int64_t(kSms) * std::max(1, kResidentVectors / vectors), max_lines(p.rows, p.cols)}));
+  const int64_t most = std::min(resident(std::max(1, kResidentVectors / vectors), row.ctas), max_lines(p.rows, p.cols));
+  *lines = static_cast<int>(like_workers(most, kWarpRow ? ceil_div(p.rows, threads / 32) : p.rows, kOdd && !kWarpRow));
   if (kWarpRow) smem = std::max(smem, size_t(threads / 32) * p.cols * sizeof(float));
-  if (int rc = ensure_smem_attr(reinterpret_cast<const void*>(kern), 200 * 1024)) return rc;
-  kern<<<*lines, threads, smem, st>>>(p);
-  return launched();
-}
-
-template <typename T, typename W, int NV, int kMaxThreads>
-int run_bwd_any(const LayerNormBwdParams& p, int* lines, cudaStream_t st) {
-  const int threads = row_threads(p.cols, 1, NV);
-  *lines = static_cast<int>(std::min<int64_t>(max_lines(p.rows, p.cols), kSms * std::min(16, std::max(1, 2048 / threads))));
-  layernorm_bwd_any_kernel<T, W, NV, kMaxThreads><<<*lines, threads, 0, st>>>(p);
-  return launched();
+  return launch_rows(layernorm_bwd_kernel<T, W, NV, kMaxThreads, kMinCtas, kWarpRow, kWide, kOdd, kStages>, p, *lines,
+                     row.ctas, threads, smem, st);
 }
 
 template <typename T, typename W>
 int bwd(const LayerNormBwdParams& p, void* dw, void* db, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
-  const bool vec = p.cols % V == 0 && aligned(p.x, 16) && aligned(p.dy, 16) && aligned(p.w, 16) &&
-                   aligned(p.dres, 16) && aligned(p.dx, 16) && p.ld_x % V == 0 && p.ld_dy % V == 0 && p.ld_dx % V == 0 &&
-                   (p.dres == nullptr || p.ld_dres % V == 0);
+  const RowTensor rows[] = {{p.x, p.ld_x}, {p.dy, p.ld_dy}, {p.dx, p.ld_dx}, {p.dres, p.ld_dres}};
+  const Rows kind = rows_kind(rows, p.cols, V, aligned(p.w, 16));
+  const int places = p.cols + (kind == Rows::kOdd ? V - 1 : 0);
   int rc, lines = 0;
-  if (vec && p.cols <= 32 * V) {
-    rc = run_bwd<T, W, 1, 256, 3, true>(p, &lines, st);
-  } else if (vec && p.cols <= 64 * V) {
-    rc = run_bwd<T, W, 2, 256, 2, true>(p, &lines, st);
-  } else if (vec && p.cols <= 256 * V) {
-    rc = run_bwd<T, W, 2, 128, 4, false>(p, &lines, st);
-  } else if (vec && p.cols <= 512 * V) {
-    rc = run_bwd<T, W, 4, 128, 4, false>(p, &lines, st);
-  } else if (vec && p.cols <= 1024 * V) {
-    rc = run_bwd<T, W, 4, 256, 2, false>(p, &lines, st);
-  } else if (!vec && p.cols <= 4096) {
-    rc = run_bwd_any<T, W, 8, 512>(p, &lines, st);
-  } else if (!vec && p.cols <= 8192) {
-    rc = run_bwd_any<T, W, 16, 512>(p, &lines, st);
-  } else {
+  if (kind == Rows::kAny || places > kMaxCluster * 1024 * V) {
     lines = static_cast<int>(max_lines(p.rows, p.cols));
-    layernorm_bwd_long_kernel<T, W><<<static_cast<unsigned>(p.rows), 1024, 0, st>>>(p);
+    layernorm_bwd_long_kernel<T, W><<<static_cast<unsigned>(p.rows), long_threads(p.cols), 0, st>>>(p);
     if (p.part != nullptr)
       layernorm_bwd_long_cols_kernel<T>
-          <<<dim3(static_cast<unsigned>(ceil_div(p.cols, 1024)), static_cast<unsigned>(lines)), 1024, 0, st>>>(p);
+          <<<dim3(static_cast<unsigned>(ceil_div(p.cols, 1024)), static_cast<unsigned>(lines)), long_threads(p.cols), 0, st>>>(p);
     rc = launched();
+  } else if (kind == Rows::kOdd) {
+    if (places <= 64 * V)
+      rc = run_bwd<T, W, 2, 256, 2, true, false, true>(p, &lines, st);
+    else if (places <= 1024 * V)
+      rc = run_bwd<T, W, 4, 256, 2, false, false, true>(p, &lines, st);
+    else
+      rc = run_bwd<T, W, 4, 256, 2, false, true, true>(p, &lines, st);
+  } else if (p.cols <= 32 * V) {
+    rc = run_bwd<T, W, 1, 256, 3, true, false, false>(p, &lines, st);
+  } else if (p.cols <= 64 * V) {
+    rc = run_bwd<T, W, 2, 256, 2, true, false, false>(p, &lines, st);
+  } else if (p.cols <= 256 * V) {
+    rc = run_bwd<T, W, 2, 128, 4, false, false, false>(p, &lines, st);
+  } else if (p.cols <= 512 * V) {
+    rc = run_bwd<T, W, 4, 128, 4, false, false, false>(p, &lines, st);
+  } else if (p.cols <= 1024 * V) {
+    rc = run_bwd<T, W, 4, 256, 2, false, false, false>(p, &lines, st);
+  } else {
+    rc = run_bwd<T, W, 4, 256, 2, false, true, false>(p, &lines, st);
   }
   if (rc || p.part == nullptr) return rc;
   return launch_after(layernorm_bwd_finish_kernel<W>, static_cast<unsigned>(ceil_div(2 * int64_t(p.cols), 32)), 1024u, st,
@@ -210,7 +283,7 @@ int fab_layernorm(const void* x, const void* residual, const void* w, const void
   if (!aligned(x, e) || !aligned(residual, e) || !aligned(y, e) || !aligned(x_out, e) || !aligned(w, we) ||
       !aligned(bias, we) || !aligned(mean, 4) || !aligned(rstd, 4))
     return kErrInvalidArg;
-  LayerNormParams p{x, residual, w, bias, y, x_out, mean, rstd, ld_x, ld_res, ld_y, ld_xo, rows, cols, eps};
+  LayerNormParams p{x, residual, w, bias, y, x_out, mean, rstd, ld_x, ld_res, ld_y, ld_xo, rows, cols, eps, 0};
   auto st = static_cast<cudaStream_t>(stream);
   return by_types(dtype, w_dtype, [&](auto t, auto wt) { return fwd<decltype(t), decltype(wt)>(p, st); });
 }
@@ -244,7 +317,7 @@ int fab_layernorm_bwd(const void* dy, const void* x, const void* w, const float*
                workspace_bytes < size_t(max_lines(rows, cols)) * 2 * size_t(cols) * sizeof(float)))
     return kErrWorkspace;
   LayerNormBwdParams p{dy, x, w, mean, rstd, dresidual, dx, sums ? static_cast<float*>(workspace) : nullptr,
-                       ld_dy, ld_x, ld_dres, ld_dx, rows, cols};
+                       ld_dy, ld_x, ld_dres, ld_dx, rows, cols, 0};
   return by_types(dtype, w_dtype,
                   [&](auto t, auto wt) { return bwd<decltype(t), decltype(wt)>(p, dw, db, st); });
 }

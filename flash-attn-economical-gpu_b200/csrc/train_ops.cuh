@@ -9,6 +9,8 @@
 
 #include <cstdint>
 
+#include "ptx.cuh"
+
 namespace fab {
 
 template <typename T>
@@ -187,6 +189,145 @@ __device__ __forceinline__ void few_warps_sum(float (&v)[K], float* red) {
   }
 }
 
+// Rows wider than a CTA's share of shared memory belong to a cluster of CTAs,
+// each with its columns.  A CTA's columns are counted in places: column c is
+// place c + shift, where the row starts `shift` elements past a 16-byte
+// boundary, so that places 0, V, 2V, ... lie on boundaries.  (V values are 16
+// bytes.)
+constexpr int kMaxCluster = 8;
+struct RowShare {
+  int rank, ctas;      // place in the cluster
+  int first, places;   // first place, places of this CTA
+  int lo, hi;          // this CTA's places that are columns
+};
+template <bool kWide>
+__device__ __forceinline__ RowShare row_share(int cols, int shift, int span) {
+  RowShare r{0, 1, 0, cols + shift, shift, cols + shift};
+  if constexpr (kWide) {
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r.rank));
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r.ctas));
+    r.first = r.rank * span;
+    r.places = max(0, min(span, r.hi - r.first));
+    r.lo -= r.first;
+    r.hi -= r.first;
+  }
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile(
+      "barrier.cluster.arrive.release.aligned;\n\t"
+      "barrier.cluster.wait.acquire.aligned;" ::
+          : "memory");
+}
+
+// The sums over a row of K values at a time, in one of two buffers in turn:
+// every thread has left a buffer for good when the other one's sums are
+// complete.  A CTA alone: few_warps_sum.  A cluster: each warp's sum goes to
+// every CTA, and its bytes complete that CTA's barrier.  (A barrier of the
+// cluster, which also waits for the row's stores to global memory, took longer:
+// 4096 x 12288 bf16 forward 104 us against 78.)  The kernels hold
+//   float red[2][kSumFloats<kWide, K>], RowBars bars  in shared memory
+// as variables of their own: through a reference the reads of a lone CTA's
+// sums became generic ones, 4 % of the backward's time.
+template <bool kWide, int K>
+constexpr int kSumFloats = K * 8 * (kWide ? kMaxCluster : 1);
+struct RowBars {
+  uint64_t bar[2];
+  int abort;
+};
+template <bool kWide, int kFloats>
+__device__ __forceinline__ void init_sums(float (&red)[2][kFloats], RowBars& bars) {
+  for (int i = threadIdx.x; i < 2 * kFloats; i += blockDim.x) red[i / kFloats][i % kFloats] = 0.f;
+  if constexpr (kWide) {
+    if (threadIdx.x == 0) {
+      mbar_init(bars.bar, 1);
+      mbar_init(bars.bar + 1, 1);
+      mbar_fence_init();
+      bars.abort = 0;
+    }
+    cluster_sync();
+  } else {
+    __syncthreads();
+  }
+}
+// K sums over the cluster; false when a peer's never came.
+template <int K>
+__device__ __forceinline__ bool cluster_sum(float (&v)[K], float* red, uint64_t* bar, uint32_t parity, RowBars& bars,
+                                            const RowShare& r) {
+  const int lane = threadIdx.x & 31;
+  warp_sum<K>(v);
+  if (threadIdx.x == 0) mbar_arrive_expect_tx(bar, K * 4 * (blockDim.x >> 5) * r.ctas);
+  if (lane < r.ctas) {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      asm volatile(
+          "{\n\t.reg .u32 to, bar;\n\t"
+          "mapa.shared::cluster.u32 to, %0, %2;\n\t"
+          "mapa.shared::cluster.u32 bar, %1, %2;\n\t"
+          "st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [to], %3, [bar];\n\t}" ::"r"(
+              smem_u32(red + (k * kMaxCluster + r.rank) * 8 + (threadIdx.x >> 5))),
+          "r"(smem_u32(bar)), "r"(lane), "r"(__float_as_uint(v[k]))
+          : "memory");
+  }
+  __syncwarp();
+  const bool ok = __all_sync(0xffffffffu, mbar_wait_cluster(bar, parity, &bars.abort, kDevTimeoutRowSum));
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    v[k] = 0.f;
+    for (int x = 0; x < 2 * r.ctas; ++x) {
+      const float4 a = *reinterpret_cast<const float4*>(red + k * kMaxCluster * 8 + x * 4);
+      v[k] += (a.x + a.y) + (a.z + a.w);
+    }
+  }
+  return ok;
+}
+
+// A row whose ends lie inside 16-byte pieces (kOdd): those pieces' places that
+// are no columns.
+template <typename T>
+struct RowEnds {
+  static constexpr int V = 16 / sizeof(T);
+  int lo, hi;  // columns are places [lo, hi)
+  __device__ __forceinline__ bool cut(int c) const { return c < lo || c + V > hi; }
+  __device__ __forceinline__ bool in(int c) const { return c >= lo && c < hi; }
+  // Values at no column become 0.
+  __device__ __forceinline__ void clip(int c, float2 (&f)[V / 2]) const {
+#pragma unroll
+    for (int e = 0; e < V / 2; ++e) {
+      if (!in(c + 2 * e)) f[e].x = 0.f;
+      if (!in(c + 2 * e + 1)) f[e].y = 0.f;
+    }
+  }
+  __device__ __forceinline__ void copy(T* to, const T* from, int c) const {
+#pragma unroll 1
+    for (int e = 0; e < V; ++e)
+      if (in(c + e)) to[e] = from[e];
+  }
+  __device__ __forceinline__ void store(T* to, const uint4& v, int c) const {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (in(c + e)) {
+        if constexpr (sizeof(T) == 2)
+          reinterpret_cast<uint16_t*>(to)[e] = static_cast<uint16_t>(e & 1 ? w[e / 2] >> 16 : w[e / 2]);
+        else
+          reinterpret_cast<uint32_t*>(to)[e] = w[e];
+      }
+  }
+  // Weights of the places from c on, 0 at no column.
+  template <typename W>
+  __device__ __forceinline__ void weights(const W* w, int c, float2 (&f)[V / 2]) const {
+#pragma unroll
+    for (int e = 0; e < V / 2; ++e)
+      f[e] = make_float2(in(c + 2 * e) ? to_float<W>(w[c + 2 * e]) : 0.f, in(c + 2 * e + 1) ? to_float<W>(w[c + 2 * e + 1]) : 0.f);
+  }
+};
+// Elements from the 16-byte boundary at or before p.
+template <typename T>
+__device__ __forceinline__ int past_boundary(const T* p) {
+  return static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15u) / static_cast<int>(sizeof(T));
+}
+
 // ------------------------------------------------------------ layer norm ---
 struct LayerNormParams {
   const void* x;
@@ -201,6 +342,7 @@ struct LayerNormParams {
   int64_t rows;
   int cols;
   float eps;
+  int span;  // columns of a CTA where a cluster shares a row
 };
 
 // y = (x' - mean) * rsqrt(var + eps) * w + b per row, x' = x or round(x + residual).
@@ -276,9 +418,7 @@ __global__ void __launch_bounds__(kMaxThreads) layernorm_fwd_kernel(const LayerN
 // Asynchronous 16-byte copies into shared memory that the copying thread
 // alone reads back: it waits for its own groups, no barrier is needed.
 __device__ __forceinline__ void copy16(void* dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
-               "l"(src)
-               : "memory");
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int kPending>
@@ -291,7 +431,7 @@ __device__ __forceinline__ uint4 read_again(const uint4* p) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p)))
+               : "r"(smem_u32(p))
                : "memory");
   return v;
 }
@@ -300,46 +440,70 @@ __device__ __forceinline__ uint4 read_again(const uint4* p) {
 // ... and has the next kStages - 1 of them on their way into shared memory
 // while it works on one, so that the memory stays busy across a row's two
 // reductions; weight and bias wait in registers for all of them (read anew for
-// every row they were the larger part of what L1 had to deliver).  16-byte
-// rows, NV vectors per thread.
-template <typename T, typename W, int NV, int kMaxThreads, int kMinCtas, int kStages>
+// every row they were the larger part of what L1 had to deliver).  NV 16-byte
+// vectors per thread.  kOdd: rows off the 16-byte grid, of which every CTA
+// takes some that start at the same offset (gridDim.x / ctas is a multiple of
+// 8, or there is one row each); the pieces at their ends are cut to the row.
+template <typename T, typename W, int NV, int kMaxThreads, int kMinCtas, int kStages, bool kWide, bool kOdd>
 __global__ void __launch_bounds__(kMaxThreads, kMinCtas) layernorm_fwd_stream_kernel(const LayerNormParams p) {
   constexpr int N = Pairs<T>::kN, V = 2 * N;
   extern __shared__ __align__(16) uint8_t smem_copies[];
-  __shared__ __align__(16) float red[2][16];
+  __shared__ __align__(16) float red[2][kSumFloats<kWide, 1>];
+  __shared__ RowBars bars;
+  uint32_t ctas = 1;
+  if constexpr (kWide) asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
+  const int64_t row0 = blockIdx.x / ctas;
+  const int shift = kOdd ? past_boundary(reinterpret_cast<const T*>(p.x) + row0 * p.ld_x) : 0;
+  const RowShare share = row_share<kWide>(p.cols, shift, p.span);
+  const int cols = share.places, col0 = share.first - shift;
+  [[maybe_unused]] const RowEnds<T> ends{share.lo, share.hi};
   const bool summed = p.residual != nullptr;
   const int threads = blockDim.x;
   const int c0 = threadIdx.x * V, step = threads * V;  // first column, columns between vectors
-  if (threadIdx.x < 32) red[threadIdx.x >> 4][threadIdx.x & 15] = 0.f;
-  __syncthreads();
+  init_sums<kWide>(red, bars);
+  [[maybe_unused]] uint32_t parity = 0;
   float2 w[NV][N], b[NV][N];
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     const int c = c0 + k * step;
 #pragma unroll
     for (int e = 0; e < N; ++e) w[k][e] = b[k][e] = both(0.f);
-    if (c < p.cols) {
-      load_pairs<W, N>(reinterpret_cast<const W*>(p.w) + c, w[k]);
-      if (p.bias != nullptr) load_pairs<W, N>(reinterpret_cast<const W*>(p.bias) + c, b[k]);
+    if (c < cols) {
+      const W* pw = reinterpret_cast<const W*>(p.w) + col0;
+      const W* pb = reinterpret_cast<const W*>(p.bias) + col0;
+      if constexpr (kOdd) {
+        ends.weights(pw, c, w[k]);
+        if (p.bias != nullptr) ends.weights(pb, c, b[k]);
+      } else {
+        load_pairs<W, N>(pw + c, w[k]);
+        if (p.bias != nullptr) load_pairs<W, N>(pb + c, b[k]);
+      }
     }
   }
   // Pointers to this thread's first column of the row being fetched and of the
   // one being worked on, moved from row to row.
-  const int64_t rows_apart = gridDim.x;
-  const T* fx = reinterpret_cast<const T*>(p.x) + blockIdx.x * p.ld_x + c0;
-  const T* fr = reinterpret_cast<const T*>(p.residual) + blockIdx.x * p.ld_res + c0;
-  T* y = reinterpret_cast<T*>(p.y) + blockIdx.x * p.ld_y + c0;
-  T* xo = reinterpret_cast<T*>(p.x_out) + blockIdx.x * p.ld_xo + c0;
+  const int64_t rows_apart = gridDim.x / ctas;
+  const T* fx = reinterpret_cast<const T*>(p.x) + row0 * p.ld_x + col0 + c0;
+  const T* fr = reinterpret_cast<const T*>(p.residual) + row0 * p.ld_res + col0 + c0;
+  T* y = reinterpret_cast<T*>(p.y) + row0 * p.ld_y + col0 + c0;
+  T* xo = reinterpret_cast<T*>(p.x_out) + row0 * p.ld_xo + col0 + c0;
   const int64_t dx = rows_apart * p.ld_x, dr = rows_apart * p.ld_res, dy = rows_apart * p.ld_y, dxo = rows_apart * p.ld_xo;
   // This thread's vectors of a stage: x at [k], the residual at [NV + k].
   uint4* const mine = reinterpret_cast<uint4*>(smem_copies) + threadIdx.x;
   const int stage_size = 2 * NV * threads;
-  int64_t fetch_row = blockIdx.x;
+  int64_t fetch_row = row0;
+  [[maybe_unused]] const bool close = p.ld_x < V || (summed && p.ld_res < V);  // rows nearer than a piece
   auto fetch = [&](uint4* to) {
     if (fetch_row < p.rows) {
 #pragma unroll
       for (int k = 0; k < NV; ++k)
-        if (c0 + k * step < p.cols) {
+        if (c0 + k * step < cols) {
+          // The first and last row's cut pieces are not all inside the tensor.
+          if (kOdd && ends.cut(c0 + k * step) && (fetch_row == 0 || fetch_row + 1 == p.rows || close)) {
+            ends.copy(reinterpret_cast<T*>(to + k * threads), fx + k * step, c0 + k * step);
+            if (summed) ends.copy(reinterpret_cast<T*>(to + (NV + k) * threads), fr + k * step, c0 + k * step);
+            continue;
+          }
           copy16(to + k * threads, fx + k * step);
           if (summed) copy16(to + (NV + k) * threads, fr + k * step);
         }
@@ -355,7 +519,7 @@ __global__ void __launch_bounds__(kMaxThreads, kMinCtas) layernorm_fwd_stream_ke
   for (int s = 0; s < kStages - 1; ++s, to += stage_size) fetch(to);
   const uint4* from = mine;
   uint4* const end = mine + kStages * stage_size;
-  for (int64_t row = blockIdx.x; row < p.rows; row += rows_apart, y += dy, xo += dxo) {
+  for (int64_t row = row0; row < p.rows; row += rows_apart, y += dy, xo += dxo) {
     fetch(to);
     if ((to += stage_size) == end) to = mine;
     copy_wait<kStages - 1>();
@@ -363,7 +527,7 @@ __global__ void __launch_bounds__(kMaxThreads, kMinCtas) layernorm_fwd_stream_ke
     float2 sum2 = both(0.f);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      if (c0 + k * step < p.cols) {
+      if (c0 + k * step < cols) {
         to_pairs<T>(from[k * threads], f[k]);
         if (summed) {
           float2 r[N];
@@ -371,43 +535,61 @@ __global__ void __launch_bounds__(kMaxThreads, kMinCtas) layernorm_fwd_stream_ke
 #pragma unroll
           for (int e = 0; e < N; ++e) r[e] = __fadd2_rn(f[k][e], r[e]);
           const uint4 raw = from_pairs<T>(r);
-          *reinterpret_cast<uint4*>(xo + k * step) = raw;
+          if (kOdd && ends.cut(c0 + k * step))
+            ends.store(xo + k * step, raw, c0 + k * step);
+          else
+            *reinterpret_cast<uint4*>(xo + k * step) = raw;
           to_pairs<T>(raw, f[k]);  // the norm is of the rounded sum
         }
+        if (kOdd && ends.cut(c0 + k * step)) ends.clip(c0 + k * step, f[k]);
 #pragma unroll
         for (int e = 0; e < N; ++e) sum2 = __fadd2_rn(sum2, f[k][e]);
       }
     }
     if ((from += stage_size) == end) from = mine;
     float sum[1] = {sum2.x + sum2.y};
-    few_warps_sum<1>(sum, red[0]);
+    if constexpr (kWide) {
+      if (!cluster_sum<1>(sum, red[0], bars.bar, parity, bars, share)) break;
+    } else {
+      few_warps_sum<1>(sum, red[0]);
+    }
     const float mean = sum[0] * inv;
     float2 sq2 = both(0.f);
 #pragma unroll
     for (int k = 0; k < NV; ++k)
-      if (c0 + k * step < p.cols)
+      if (c0 + k * step < cols) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          f[k][e] = __fadd2_rn(f[k][e], both(-mean));
-          sq2 = __ffma2_rn(f[k][e], f[k][e], sq2);
-        }
+        for (int e = 0; e < N; ++e) f[k][e] = __fadd2_rn(f[k][e], both(-mean));
+        if (kOdd && ends.cut(c0 + k * step)) ends.clip(c0 + k * step, f[k]);
+#pragma unroll
+        for (int e = 0; e < N; ++e) sq2 = __ffma2_rn(f[k][e], f[k][e], sq2);
+      }
     float sq[1] = {sq2.x + sq2.y};
-    // Each reduction's barrier also frees the other's buffer.
-    few_warps_sum<1>(sq, red[1]);
+    // Each of the two sums also frees the other's buffer.
+    if constexpr (kWide) {
+      if (!cluster_sum<1>(sq, red[1], bars.bar + 1, parity, bars, share)) break;
+      parity ^= 1u;
+    } else {
+      few_warps_sum<1>(sq, red[1]);
+    }
     const float rstd = rsqrtf(sq[0] * inv + p.eps);
-    if (threadIdx.x == 0 && p.mean != nullptr) {
+    if (threadIdx.x == 0 && share.rank == 0 && p.mean != nullptr) {
       p.mean[row] = mean;
       p.rstd[row] = rstd;
     }
 #pragma unroll
     for (int k = 0; k < NV; ++k)
-      if (c0 + k * step < p.cols) {
+      if (c0 + k * step < cols) {
 #pragma unroll
         for (int e = 0; e < N; ++e) f[k][e] = __ffma2_rn(__fmul2_rn(f[k][e], both(rstd)), w[k][e], b[k][e]);
-        *reinterpret_cast<uint4*>(y + k * step) = from_pairs<T>(f[k]);
+        if (kOdd && ends.cut(c0 + k * step))
+          ends.store(y + k * step, from_pairs<T>(f[k]), c0 + k * step);
+        else
+          *reinterpret_cast<uint4*>(y + k * step) = from_pairs<T>(f[k]);
       }
   }
   copy_wait<0>();
+  if constexpr (kWide) cluster_sync();  // the others may still write their sums here
 }
 
 // Rows too long for the registers of one CTA: the same sums over three reads
@@ -463,6 +645,7 @@ struct LayerNormBwdParams {
   int64_t ld_dy, ld_x, ld_dres, ld_dx;
   int64_t rows;
   int cols;
+  int span;  // columns of a CTA where a cluster shares a row
 };
 
 // With xhat = (x - mean) * rstd and g = dy * w:
@@ -475,45 +658,73 @@ struct LayerNormBwdParams {
 // and leaves once.  The next kStages - 1 rows are on their way into shared
 // memory while one is worked on, which keeps the memory busy across the
 // reduction that every row has in its middle; the weight waits in registers.
-template <typename T, typename W, int NV, int kMaxThreads, int kMinCtas, bool kWarpRow, int kStages>
+template <typename T, typename W, int NV, int kMaxThreads, int kMinCtas, bool kWarpRow, bool kWide, bool kOdd, int kStages>
 __global__ void __launch_bounds__(kMaxThreads, kMinCtas) layernorm_bwd_kernel(const LayerNormBwdParams p) {
   constexpr int N = Pairs<T>::kN, V = 2 * N;
   extern __shared__ __align__(16) uint8_t smem_copies[];
-  __shared__ __align__(16) float red[2][16];
+  __shared__ __align__(16) float red[2][kSumFloats<kWide, 2>];
+  __shared__ RowBars bars;
+  uint32_t ctas = 1;
+  if constexpr (kWide) asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
   const int threads = blockDim.x;
   const int lanes = kWarpRow ? 32 : threads;  // threads of a row
   const int me = kWarpRow ? threadIdx.x & 31 : threadIdx.x;
-  const int64_t worker = kWarpRow ? static_cast<int64_t>(blockIdx.x) * (threads >> 5) + (threadIdx.x >> 5) : blockIdx.x;
-  const int64_t workers = kWarpRow ? static_cast<int64_t>(gridDim.x) * (threads >> 5) : gridDim.x;
+  const int64_t worker = kWarpRow ? static_cast<int64_t>(blockIdx.x) * (threads >> 5) + (threadIdx.x >> 5) : blockIdx.x / ctas;
+  const int64_t workers = kWarpRow ? static_cast<int64_t>(gridDim.x) * (threads >> 5) : gridDim.x / ctas;
+  const int shift = kOdd ? past_boundary(reinterpret_cast<const T*>(p.x) + worker * p.ld_x) : 0;
+  const RowShare share = row_share<kWide>(p.cols, shift, p.span);
+  const int cols = share.places, col0 = share.first - shift;
+  [[maybe_unused]] const RowEnds<T> ends{share.lo, share.hi};
   const int c0 = me * V, step = lanes * V;  // first column, columns between vectors
   const bool summed = p.dres != nullptr;
-  if (threadIdx.x < 32) red[threadIdx.x >> 4][threadIdx.x & 15] = 0.f;
-  __syncthreads();
+  init_sums<kWide>(red, bars);
+  [[maybe_unused]] uint32_t parity = 0;
   float2 w[NV][N], dw[NV][N], db[NV][N];
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     const int c = c0 + k * step;
 #pragma unroll
     for (int e = 0; e < N; ++e) w[k][e] = dw[k][e] = db[k][e] = both(0.f);
-    if (c < p.cols) load_pairs<W, N>(reinterpret_cast<const W*>(p.w) + c, w[k]);
+    if (c < cols) {
+      if constexpr (kOdd)
+        ends.weights(reinterpret_cast<const W*>(p.w) + col0, c, w[k]);
+      else
+        load_pairs<W, N>(reinterpret_cast<const W*>(p.w) + col0 + c, w[k]);
+    }
   }
   const float inv = 1.f / static_cast<float>(p.cols);
-  // Pointers to this thread's first column of the row being fetched and of the
-  // one being worked on, moved from row to row.
-  const T* fx = reinterpret_cast<const T*>(p.x) + worker * p.ld_x + c0;
-  const T* fg = reinterpret_cast<const T*>(p.dy) + worker * p.ld_dy + c0;
-  const T* fr = reinterpret_cast<const T*>(p.dres) + worker * p.ld_dres + c0;
-  T* out = reinterpret_cast<T*>(p.dx) + worker * p.ld_dx + c0;
+  // This thread's first column of the row being fetched and of the one being
+  // worked on.  Moved from row to row; where a cluster or cut pieces need the
+  // registers, formed anew (kFresh: 4096 x 12288 bf16 110 against 128 us, but
+  // one CTA's rows, 8192 x 8192, 126 against 116).
+  constexpr bool kFresh = kWide || kOdd;
+  const T* fx = reinterpret_cast<const T*>(p.x) + worker * p.ld_x + col0 + c0;
+  const T* fg = reinterpret_cast<const T*>(p.dy) + worker * p.ld_dy + col0 + c0;
+  const T* fr = reinterpret_cast<const T*>(p.dres) + worker * p.ld_dres + col0 + c0;
+  T* out = reinterpret_cast<T*>(p.dx) + worker * p.ld_dx + col0 + c0;
   const int64_t ax = workers * p.ld_x, ag = workers * p.ld_dy, ar = workers * p.ld_dres, ao = workers * p.ld_dx;
   // This thread's vectors of a stage: x at [k], dy at [NV + k], dres after.
   uint4* const mine = reinterpret_cast<uint4*>(smem_copies) + threadIdx.x;
   const int stage_size = 3 * NV * threads;
+  [[maybe_unused]] const bool close = p.ld_x < V || p.ld_dy < V || (summed && p.ld_dres < V);  // rows nearer than a piece
   int64_t fetch_row = worker;
   auto fetch = [&](uint4* to) {
     if (fetch_row < p.rows) {
+      if constexpr (kFresh) {
+        fx = reinterpret_cast<const T*>(p.x) + fetch_row * p.ld_x + col0 + c0;
+        fg = reinterpret_cast<const T*>(p.dy) + fetch_row * p.ld_dy + col0 + c0;
+        fr = reinterpret_cast<const T*>(p.dres) + fetch_row * p.ld_dres + col0 + c0;
+      }
 #pragma unroll
       for (int k = 0; k < NV; ++k)
-        if (c0 + k * step < p.cols) {
+        if (c0 + k * step < cols) {
+          // The first and last row's cut pieces are not all inside the tensor.
+          if (kOdd && ends.cut(c0 + k * step) && (fetch_row == 0 || fetch_row + 1 == p.rows || close)) {
+            ends.copy(reinterpret_cast<T*>(to + k * threads), fx + k * step, c0 + k * step);
+            ends.copy(reinterpret_cast<T*>(to + (NV + k) * threads), fg + k * step, c0 + k * step);
+            if (summed) ends.copy(reinterpret_cast<T*>(to + (2 * NV + k) * threads), fr + k * step, c0 + k * step);
+            continue;
+          }
           copy16(to + k * threads, fx + k * step);
           copy16(to + (NV + k) * threads, fg + k * step);
           if (summed) copy16(to + (2 * NV + k) * threads, fr + k * step);
@@ -521,9 +732,11 @@ __global__ void __launch_bounds__(kMaxThreads, kMinCtas) layernorm_bwd_kernel(co
     }
     copy_commit();
     fetch_row += workers;
-    fx += ax;
-    fg += ag;
-    fr += ar;
+    if constexpr (!kFresh) {
+      fx += ax;
+      fg += ag;
+      fr += ar;
+    }
   };
   uint4* to = mine;
 #pragma unroll
@@ -536,7 +749,7 @@ __global__ void __launch_bounds__(kMaxThreads, kMinCtas) layernorm_bwd_kernel(co
     next_mean = p.mean[worker];
     next_rstd = p.rstd[worker];
   }
-  for (int64_t row = worker; row < p.rows; row += workers, turn ^= 1, out += ao) {
+  for (int64_t row = worker; row < p.rows; row += workers, turn ^= 1) {
     fetch(to);
     if ((to += stage_size) == end) to = mine;
     const float2 scale = both(next_rstd), less = both(-next_mean);
@@ -548,12 +761,16 @@ __global__ void __launch_bounds__(kMaxThreads, kMinCtas) layernorm_bwd_kernel(co
     float2 s0 = both(0.f), s1 = both(0.f);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      if (c0 + k * step < p.cols) {
+      if (c0 + k * step < cols) {
         // Read again after the reduction rather than held across it: the
         // registers buy another resident CTA.
         float2 h[N], g[N];
         to_pairs<T>(from[k * threads], h);
         to_pairs<T>(from[(NV + k) * threads], g);
+        if (kOdd && ends.cut(c0 + k * step)) {
+          ends.clip(c0 + k * step, h);
+          ends.clip(c0 + k * step, g);
+        }
 #pragma unroll
         for (int e = 0; e < N; ++e) {
           h[e] = __fmul2_rn(__fadd2_rn(h[e], less), scale);
@@ -566,14 +783,19 @@ __global__ void __launch_bounds__(kMaxThreads, kMinCtas) layernorm_bwd_kernel(co
       }
     }
     float s[2] = {s0.x + s0.y, s1.x + s1.y};
-    if constexpr (kWarpRow)
+    if constexpr (kWarpRow) {
       warp_sum<2>(s);
-    else
+    } else if constexpr (kWide) {
+      if (!cluster_sum<2>(s, red[turn], bars.bar + turn, parity, bars, share)) break;
+      parity ^= static_cast<uint32_t>(turn);
+    } else {
       few_warps_sum<2>(s, red[turn]);  // the other buffer is free again: every thread has passed this row's barrier
+    }
     const float2 na = both(-s[0] * inv), nb = both(-s[1] * inv);
+    if constexpr (kFresh) out = reinterpret_cast<T*>(p.dx) + row * p.ld_dx + col0 + c0;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      if (c0 + k * step < p.cols) {
+      if (c0 + k * step < cols) {
         float2 h[N], g[N];
         to_pairs<T>(read_again(from + k * threads), h);
         to_pairs<T>(read_again(from + (NV + k) * threads), g);
@@ -589,14 +811,19 @@ __global__ void __launch_bounds__(kMaxThreads, kMinCtas) layernorm_bwd_kernel(co
 #pragma unroll
           for (int e = 0; e < N; ++e) g[e] = __fadd2_rn(g[e], r[e]);
         }
-        *reinterpret_cast<uint4*>(out + k * step) = from_pairs<T>(g);
+        if (kOdd && ends.cut(c0 + k * step))
+          ends.store(out + k * step, from_pairs<T>(g), c0 + k * step);
+        else
+          *reinterpret_cast<uint4*>(out + k * step) = from_pairs<T>(g);
       }
     }
     if ((from += stage_size) == end) from = mine;
+    if constexpr (!kFresh) out += ao;
   }
   copy_wait<0>();
+  if constexpr (kWide) cluster_sync();  // the others may still write their sums here
   if (p.part == nullptr) return;
-  float* part = p.part + static_cast<int64_t>(blockIdx.x) * 2 * p.cols;
+  float* part = p.part + static_cast<int64_t>(kWide ? worker : blockIdx.x) * 2 * p.cols;
   if constexpr (kWarpRow) {
     // The warps' sums meet in shared memory, in warp order.
     __syncthreads();
@@ -605,10 +832,19 @@ __global__ void __launch_bounds__(kMaxThreads, kMinCtas) layernorm_bwd_kernel(co
     for (int which = 0; which < 2; ++which) {
 #pragma unroll
       for (int k = 0; k < NV; ++k)
-        if (c0 + k * step < p.cols)
+        if (c0 + k * step < cols)
 #pragma unroll
-          for (int e = 0; e < N; ++e)
-            *reinterpret_cast<float2*>(sums + (threadIdx.x >> 5) * p.cols + c0 + k * step + 2 * e) = which ? db[k][e] : dw[k][e];
+          for (int e = 0; e < N; ++e) {
+            const float2 v = which ? db[k][e] : dw[k][e];
+            const int c = c0 + k * step + 2 * e;
+            float* to = sums + (threadIdx.x >> 5) * p.cols + col0 + c;
+            if constexpr (kOdd) {
+              if (ends.in(c)) to[0] = v.x;
+              if (ends.in(c + 1)) to[1] = v.y;
+            } else {
+              *reinterpret_cast<float2*>(to) = v;
+            }
+          }
       __syncthreads();
       for (int c = threadIdx.x; c < p.cols; c += threads) {
         float v = sums[c];
@@ -621,72 +857,22 @@ __global__ void __launch_bounds__(kMaxThreads, kMinCtas) layernorm_bwd_kernel(co
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int c = c0 + k * step;
-      if (c < p.cols)
+      if (c >= cols) continue;
+      float* const to = part + col0 + c;
 #pragma unroll
-        for (int e = 0; e < N; e += 2) {
-          *reinterpret_cast<float4*>(part + c + 2 * e) = make_float4(dw[k][e].x, dw[k][e].y, dw[k][e + 1].x, dw[k][e + 1].y);
-          *reinterpret_cast<float4*>(part + p.cols + c + 2 * e) =
-              make_float4(db[k][e].x, db[k][e].y, db[k][e + 1].x, db[k][e + 1].y);
+      for (int e = 0; e < N; e += 2) {
+        if constexpr (kOdd) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int d = 2 * (e + x);
+            if (ends.in(c + d)) to[d] = dw[k][e + x].x, to[p.cols + d] = db[k][e + x].x;
+            if (ends.in(c + d + 1)) to[d + 1] = dw[k][e + x].y, to[p.cols + d + 1] = db[k][e + x].y;
+          }
+        } else {
+          *reinterpret_cast<float4*>(to + 2 * e) = make_float4(dw[k][e].x, dw[k][e].y, dw[k][e + 1].x, dw[k][e + 1].y);
+          *reinterpret_cast<float4*>(to + p.cols + 2 * e) = make_float4(db[k][e].x, db[k][e].y, db[k][e + 1].x, db[k][e + 1].y);
         }
-    }
-  }
-}
-
-// The same for rows off the 16-byte grid, one value per access, a CTA per row.
-template <typename T, typename W, int NV, int kMaxThreads>
-__global__ void __launch_bounds__(kMaxThreads) layernorm_bwd_any_kernel(const LayerNormBwdParams p) {
-  __shared__ float red[2][64];
-  float dw[NV], db[NV];
-#pragma unroll
-  for (int k = 0; k < NV; ++k) dw[k] = db[k] = 0.f;
-  const float inv = 1.f / static_cast<float>(p.cols);
-  int turn = 0;
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
-    const T* x = reinterpret_cast<const T*>(p.x) + row * p.ld_x;
-    const T* dy = reinterpret_cast<const T*>(p.dy) + row * p.ld_dy;
-    const T* res = reinterpret_cast<const T*>(p.dres) + row * p.ld_dres;
-    const float mean = p.mean[row], rstd = p.rstd[row];
-    float h[NV], g[NV], r[NV];
-    float s[2] = {0.f, 0.f};
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int c = threadIdx.x + k * blockDim.x;
-      h[k] = g[k] = r[k] = 0.f;
-      if (c < p.cols) {
-        h[k] = to_float<T>(x[c]);
-        g[k] = to_float<T>(dy[c]);
-        if (p.dres != nullptr) r[k] = to_float<T>(res[c]);
       }
-    }
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int c = threadIdx.x + k * blockDim.x;
-      if (c < p.cols) {
-        h[k] = (h[k] - mean) * rstd;
-        dw[k] = fmaf(g[k], h[k], dw[k]);
-        db[k] += g[k];
-        g[k] *= to_float<W>(reinterpret_cast<const W*>(p.w)[c]);
-        s[0] += g[k];
-        s[1] = fmaf(g[k], h[k], s[1]);
-      }
-    }
-    block_sum<2>(s, red[turn]);
-    const float a = s[0] * inv, b = s[1] * inv;
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int c = threadIdx.x + k * blockDim.x;
-      if (c < p.cols)
-        reinterpret_cast<T*>(p.dx)[row * p.ld_dx + c] = from_float<T>(rstd * (g[k] - fmaf(h[k], b, a)) + r[k]);
-    }
-  }
-  if (p.part == nullptr) return;
-  float* out = p.part + static_cast<int64_t>(blockIdx.x) * 2 * p.cols;
-#pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int c = threadIdx.x + k * blockDim.x;
-    if (c < p.cols) {
-      out[c] = dw[k];
-      out[p.cols + c] = db[k];
     }
   }
 }

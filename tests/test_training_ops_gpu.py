@@ -101,6 +101,20 @@ NORMS = [
     (2, 40000, torch.float16, torch.float16, True),      # past what a CTA's registers hold
     (603, 33000, torch.bfloat16, torch.bfloat16, False),
     (4099, 64, torch.bfloat16, torch.float32, True),
+    # many rows for each worker, every way a row is shared out: by a warp, a CTA, a cluster; rows off the 16-byte grid
+    (9001, 136, torch.float16, torch.float16, False),
+    (9001, 509, torch.bfloat16, torch.bfloat16, True),
+    (9000, 63, torch.float32, torch.float32, True),
+    (3100, 1023, torch.bfloat16, torch.float32, True),
+    (2777, 4104, torch.bfloat16, torch.bfloat16, True),
+    (2500, 4095, torch.float32, torch.float32, False),
+    (1501, 6001, torch.float16, torch.float32, True),
+    (999, 12288, torch.bfloat16, torch.bfloat16, True),
+    (999, 12289, torch.bfloat16, torch.bfloat16, True),
+    (777, 16388, torch.float32, torch.float32, True),
+    (160, 65528, torch.float16, torch.float16, False),
+    (90, 65529, torch.bfloat16, torch.float32, True),
+    (40, 32761, torch.float32, torch.float32, True),
 ]
 
 
@@ -159,6 +173,53 @@ def test_layernorm_rows_are_independent_of_bad_ones(cuda_device):
     got = training.layernorm_forward(bad, w, b)
     keep = [0, 1, 2, 3, 5, 6, 8]
     assert torch.equal(got[0][keep], clean[0][keep]) and torch.isnan(got[0][4]).all() and torch.isnan(got[0][7]).all()
+
+
+@pytest.mark.parametrize("cols", [640, 641, 83, 9001])
+def test_layernorm_gradients_are_independent_of_bad_rows(cols, cuda_device):
+    """Where 16-byte pieces reach into the rows before and after, nothing of them gets in."""
+    for rows in (9, 700):
+        x, w, b, res, dy = _norm_inputs(rows, cols, torch.bfloat16, torch.bfloat16, cuda_device, 3)
+        _, mean, rstd = training.layernorm_forward(x, w, b)
+        clean = training.layernorm_backward(dy, x, w, mean, rstd, dresidual=res)[0]
+        bad_x, bad_dy = x.clone(), dy.clone()
+        bad_x[1::2], bad_dy[1::2] = float("nan"), float("inf")
+        y, m, r = training.layernorm_forward(bad_x, w, b)
+        assert torch.equal(y[::2], training.layernorm_forward(x, w, b)[0][::2])
+        got = training.layernorm_backward(bad_dy, bad_x, w, mean, rstd, dresidual=res)[0]
+        assert torch.equal(got[::2], clean[::2])
+
+
+@pytest.mark.parametrize("lead", [0, 1, 5])
+def test_layernorm_writes_no_neighbour(lead, cuda_device):
+    """Rows with gaps between them and around them, through the C ABI: the gaps keep their bits."""
+    rows, cols, ld = 700, 333, 341
+    x, w, b, res, dy = _norm_inputs(rows, cols, torch.bfloat16, torch.bfloat16, cuda_device, 9)
+
+    def padded(t=None):
+        store = torch.full((rows * ld + 16,), 7.0, device=cuda_device, dtype=torch.bfloat16)
+        view = store.as_strided((rows, cols), (ld, 1), lead)
+        if t is not None:
+            view.copy_(t)
+        return store, view
+
+    ins = [padded(t) for t in (x, res, dy)]
+    (ys, y), (xos, xo), (dxs, dx) = (padded() for _ in range(3))
+    mean, rstd = (torch.empty(rows, device=cuda_device) for _ in range(2))
+    stream = _native.current_stream_handle(cuda_device)
+    ptr = torch.Tensor.data_ptr
+    dt = _native.dtype_code(torch.bfloat16)
+    _native.check(_native.lib.fab_layernorm(
+        ptr(ins[0][1]), ptr(ins[1][1]), ptr(w), ptr(b), ptr(y), ptr(xo), ptr(mean), ptr(rstd), rows, cols, ld, ld, ld, ld,
+        EPS, dt, dt, stream), "fab_layernorm")
+    _native.check(_native.lib.fab_layernorm_bwd(
+        ptr(ins[2][1]), ptr(xo), ptr(w), ptr(mean), ptr(rstd), ptr(ins[1][1]), ptr(dx), None, None, None, 0, rows, cols, ld,
+        ld, ld, ld, dt, dt, stream), "fab_layernorm_bwd")
+    _check_forward(x, w, b, (y, mean, rstd, xo), res)
+    _check_backward(dy, xo, w, mean, rstd, (dx,), res, with_sums=False)
+    for store, view in ((ys, y), (xos, xo), (dxs, dx)):
+        view.fill_(7.0)
+        assert (store == 7.0).all()
 
 
 def test_layernorm_without_rows(cuda_device):
