@@ -254,12 +254,15 @@ class _LayerNorm(torch.autograd.Function):
         y, mean, rstd, *total = layernorm_forward(x, weight, bias, eps=eps, residual=residual)
         ctx.save_for_backward(total[0] if total else x, weight, mean, rstd)
         ctx.has_bias, ctx.has_residual = bias is not None, residual is not None
+        ctx.set_materialize_grads(False)  # an unused sum costs no pass over zeros
         return (y, total[0]) if total else y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dtotal=None):
         x, weight, mean, rstd = ctx.saved_tensors
+        if dy is None:
+            dy = torch.zeros_like(x)
         dx, dw, db = layernorm_backward(dy, x, weight, mean, rstd, dresidual=dtotal)
         return dx, dw, db if ctx.has_bias else None, None, dx if ctx.has_residual else None
 
@@ -278,9 +281,17 @@ class _Rope(torch.autograd.Function):
         return dq, dk, None, None, None, None
 
 
+def _check_trainable(what: str, q) -> None:
+    # The forward pass also takes float32, which the backward pass does not.
+    _require_cuda_tensor("q", q)
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"{what}: q, k and v must be float16 or bfloat16, got {q.dtype}")
+
+
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool = False,
               sm_scale: float | None = None) -> torch.Tensor:
     """Differentiable flash_atten.attention_forward (float16 or bfloat16)."""
+    _check_trainable("attention", q)
     return _Attention.apply(q, k, v, causal, sm_scale)
 
 
@@ -288,6 +299,7 @@ def attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
                      cu_seqlens_k: torch.Tensor, max_seqlen_q: int, max_seqlen_k: int, *, causal: bool = False,
                      sm_scale: float | None = None) -> torch.Tensor:
     """Differentiable flash_atten.attention_forward_varlen (float16 or bfloat16)."""
+    _check_trainable("attention_varlen", q)
     return _AttentionVarlen.apply(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, causal, sm_scale)
 
 

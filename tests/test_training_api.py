@@ -152,3 +152,24 @@ def test_rope_refuses_before_any_launch():
                    dict(dtype=9), dict(tokens=-1), dict(head_dim=0), dict(positions=4100, positions_64bit=1)):
         assert call(**change) == _native.FAB_ERR_INVALID_ARG, change
     assert call(tokens=0) == _native.FAB_OK
+
+
+def test_autograd_attention_refuses_what_has_no_gradient():
+    x = torch.zeros(1, 1, 4, 64)
+    with pytest.raises(ValueError, match="CUDA"):
+        training.attention(x, x, x)
+
+
+def test_example_positions_and_batches():
+    import train_block
+
+    pos = train_block.rope_positions(2, 2, 3)
+    assert pos.tolist() == [[0, 1, 2, 2, 2, 2, 2, 2], [0, 1, 2, 2, 2, 3, 3, 3], [0, 1, 2, 3, 4, 2, 3, 4]]
+    g = torch.Generator().manual_seed(1)
+    words = torch.arange(14).view(2, 7)
+    tokens, batch = train_block.make_batch(((3, 2, 2), (1, 1, 4)), words, (2, 1, 1), g, "cpu")
+    assert batch["cu"].tolist() == [0, 7, 12] and batch["longest"] == 7 and batch["positions"].shape == (3, 12)
+    assert batch["cos"].shape == (int(batch["positions"].max()) + 1, 4)
+    assert tokens[0] == tokens[7] % 7 + tokens[0] // 7 * 7
+    loss = train_block.next_token_loss(torch.zeros(12, 14), tokens, batch["cu"])
+    assert abs(loss.item() - torch.tensor(14.0).log().item()) < 1e-5
