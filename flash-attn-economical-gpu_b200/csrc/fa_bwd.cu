@@ -185,10 +185,10 @@ void launch_stats(const FaBwdParams& kp, cudaStream_t stream) {
   }
 }
 
-template <typename T, int kDP>
+template <typename T, int kDP, bool kTwo>
 int launch(const fab_attention_bwd_params* p, FaBwdParams& kp, cudaStream_t stream) {
   using C = BwdCfg<kDP>;
-  auto kern = fa_bwd_kernel<T, kDP>;
+  auto kern = fa_bwd_kernel<T, kDP, kTwo>;
   int rc = ensure_smem_attr(reinterpret_cast<const void*>(kern), C::kSmemBytes);
   if (rc) return rc;
   // The kernel's register split was sized for this launch allocation; a build
@@ -263,15 +263,21 @@ int launch(const fab_attention_bwd_params* p, FaBwdParams& kp, cudaStream_t stre
   return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
 }
 
+template <typename T, int kDP>
+int launch_parts(const fab_attention_bwd_params* p, FaBwdParams& kp, cudaStream_t stream) {
+  const bool two = kp.few_rows || kp.cu_q != nullptr || std::min(kp.M, kp.N) <= kTwoPartLength;
+  return two ? launch<T, kDP, true>(p, kp, stream) : launch<T, kDP, false>(p, kp, stream);
+}
+
 template <typename T>
 int launch_dim(const fab_attention_bwd_params* p, FaBwdParams& kp, cudaStream_t stream) {
   switch (padded_head_dim(kp.D)) {
     case 64:
-      return launch<T, 64>(p, kp, stream);
+      return launch_parts<T, 64>(p, kp, stream);
     case 128:
-      return launch<T, 128>(p, kp, stream);
+      return launch_parts<T, 128>(p, kp, stream);
     default:
-      return launch<T, 256>(p, kp, stream);
+      return launch_parts<T, 256>(p, kp, stream);
   }
 }
 
@@ -343,6 +349,7 @@ int fab_attention_bwd(const fab_attention_bwd_params* p, void* stream) {
   // vanishing one does the same and keeps masked scores masked.
   kp.scale_log2 = (p->sm_scale == 0.f ? 1e-30f : p->sm_scale) * 1.4426950408889634f;
   kp.causal = p->causal ? 1 : 0;
+  kp.few_rows = int64_t(p->heads_q) * (p->cu_seqlens_q != nullptr ? p->total_q : int64_t(p->batch) * p->seqlen_q) <= kTwoPartRows;
   kp.cu_q = p->cu_seqlens_q;
   kp.cu_k = p->cu_seqlens_k;
   kp.total_q = p->total_q;

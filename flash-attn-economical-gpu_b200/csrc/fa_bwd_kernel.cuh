@@ -62,6 +62,7 @@ struct BwdElem<__nv_bfloat16> {
     __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<uint32_t*>(&h);
   }
+  __device__ static float2 unpack2(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
   __device__ static float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
 };
 template <>
@@ -80,6 +81,7 @@ struct BwdElem<__half> {
     __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<uint32_t*>(&h);
   }
+  __device__ static float2 unpack2(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
   __device__ static float to_f(__half x) { return __half2float(x); }
 };
 
@@ -353,6 +355,7 @@ struct BwdItem {
   int begin, nt;           // this slice: streamed tiles begin .. begin + nt of all heads'
   int begin_head, begin_tile;  // begin / per_head, begin % per_head
   int slice, slices;
+  int two;                 // P and dS as two 16-bit parts each
   // The tile's first row in dK or dQ [0] and in dV [1], the bytes between
   // rows, and the slice's sums where there are several slices.
   int64_t out[2], stride[2], part;
@@ -367,6 +370,16 @@ __device__ __forceinline__ void bwd_slices(int total, int slice_len, int max_sli
   slices = min(max_slices, max(1, (total + slice_len - 1) / slice_len));
   share = (total + slices - 1) / slices;
 }
+
+// P and dS are rounded to 16 bits as operands.  Over many rows that adds as
+// much error to a gradient as its own rounding does (together 1.4 times), but
+// where few rows or keys are summed a handful of values decides, and whole
+// gradients were up to 1.8 times as far off as by their rounding alone.  Short
+// sequences, and all sequences of a call with few query rows (over its heads),
+// take each value as two 16-bit parts with a product for each.  Measured: 4
+// heads of 300 tokens, one of 1024 and 4 of 500 by 700 (D 256) take the same
+// time within 2 %; 8 heads of 1 query and 32768 keys 156 instead of 129 us.
+constexpr int kTwoPartLength = 128, kTwoPartRows = 2048;
 
 // False: nothing to do (a tile or slice that this sequence does not have).
 template <int kDP, bool kDkv>
@@ -404,6 +417,7 @@ __device__ __forceinline__ bool bwd_item(const FaBwdParams& p, int index, BwdIte
   if (w.slice >= w.slices) return false;
   w.begin = w.slice * share;
   w.nt = max(0, min(share, total - w.begin));
+  w.two = p.few_rows || min(w.M, w.N) <= kTwoPartLength;
   w.begin_head = w.per_head > 0 ? w.begin / w.per_head : 0;
   w.begin_tile = w.begin - w.begin_head * w.per_head;
   w.kind = kDkv ? kItemDkv : kItemDq;
@@ -642,7 +656,7 @@ struct BwdIssuer {
   BwdPos item, it;  // items, streamed tiles
 };
 
-template <typename T, int kDP>
+template <typename T, int kDP, bool kTwo>
 __device__ __forceinline__ bool bwd_issue(const BwdCta<kDP>& c, uint32_t tmem, bool leader, int role, const BwdItem& w,
                                           BwdIssuer& n) {
   using C = BwdCfg<kDP>;
@@ -683,10 +697,11 @@ __device__ __forceinline__ bool bwd_issue(const BwdCta<kDP>& c, uint32_t tmem, b
   };
   // D[128 x kOut] += A (TMEM, kBS wide) x B(slot).  Each softmax warpgroup's
   // half of A starts at its half of the fp32 columns; `part` 0 takes the first
-  // half of each warpgroup's columns, 1 the rest.
-  auto second_product = [&](bool acc, int part) {
+  // half of each warpgroup's columns, 1 the rest.  `rest`: the second part of
+  // values in two parts.
+  auto second_product = [&](bool acc, int part, bool rest = false) {
     uint32_t vb = bn_lo + n.o.slot * (C::kBBytes >> 4) + part * ((kBS / 64 * 16 * 128) >> 4);
-    uint32_t at = tBuf + part * (kBS / 8);
+    uint32_t at = tBuf + part * (kBS / 8) + (rest ? kBS / 4 : 0);
     asm volatile("" : "+r"(vb), "+r"(at));
 #pragma unroll
     for (int x = 0; x < kBS / 32; ++x) {
@@ -726,6 +741,9 @@ __device__ __forceinline__ bool bwd_issue(const BwdCta<kDP>& c, uint32_t tmem, b
       if (sum) {
         if (!C::kHalves) second_product(i > 0, 0);
         second_product(true, 1);
+        if (kTwo && w.two)
+#pragma unroll 1
+          for (int part = 0; part < 2; ++part) second_product(true, part, true);
         commit(empty_o + n.o.slot);
       }
       n.o.next(size_o);
@@ -768,8 +786,18 @@ struct BwdSoftmax {
   BwdPos it, item, stat;
 };
 
+// What packing 32 values left of them, packed in turn.
+template <typename T>
+__device__ __forceinline__ void bwd_rest(const float* x, const uint32_t (&pk)[16], uint32_t (&rest)[16]) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const float2 f = BwdElem<T>::unpack2(pk[e]);
+    rest[e] = BwdElem<T>::pack2(x[2 * e] - f.x, x[2 * e + 1] - f.y);
+  }
+}
+
 // The streamed tiles of one item.
-template <typename T, int kDP, bool kDkv>
+template <typename T, int kDP, bool kTwo, bool kDkv>
 __device__ __forceinline__ bool bwd_tiles(const FaBwdParams& p, const BwdCta<kDP>& c, uint32_t tS, uint32_t tP, int half,
                                           int r, float row_nl, float row_nd, float cta_scale, const BwdItem& w,
                                           BwdSoftmax& n) {
@@ -841,7 +869,15 @@ __device__ __forceinline__ bool bwd_tiles(const FaBwdParams& p, const BwdCta<kDP
         }
       }
       // P of 32 columns takes 16 of them: columns that are in registers.
-      if constexpr (kDkv) tmem_st16(tS + cc * 16, pk);
+      if constexpr (kDkv) {
+        tmem_st16(tS + cc * 16, pk);
+        if (kTwo && w.two) {
+          tmem_wait_ld();  // the second parts go where the last chunks of S were
+          uint32_t rest[16];
+          bwd_rest<T>(pr + cc * 32, pk, rest);
+          tmem_st16(tS + kCols / 2 + cc * 16, rest);
+        }
+      }
     }
     if constexpr (kDkv) {
       tmem_wait_st();
@@ -859,6 +895,7 @@ __device__ __forceinline__ bool bwd_tiles(const FaBwdParams& p, const BwdCta<kDP
         arrive(c.ds);
       }
       uint32_t pk[16];
+      float value[32];
 #pragma unroll
       for (int e = 0; e < 32; e += 4) {
         const int x = cc * 32 + e;
@@ -876,8 +913,15 @@ __device__ __forceinline__ bool bwd_tiles(const FaBwdParams& p, const BwdCta<kDP
         }
         pk[e / 2] = BwdElem<T>::pack2(d0.x, d0.y);
         pk[e / 2 + 1] = BwdElem<T>::pack2(d1.x, d1.y);
+        value[e] = d0.x, value[e + 1] = d0.y, value[e + 2] = d1.x, value[e + 3] = d1.y;
       }
       tmem_st16(tP + cc * 16, pk);
+      if (kTwo && w.two) {
+        tmem_wait_ld();
+        uint32_t rest[16];
+        bwd_rest<T>(value, pk, rest);
+        tmem_st16(tP + kCols / 2 + cc * 16, rest);
+      }
     }
     tmem_wait_st();
     arrive(c.ds + 1);
@@ -891,7 +935,7 @@ __device__ __forceinline__ bool bwd_tiles(const FaBwdParams& p, const BwdCta<kDP
   return true;
 }
 
-template <typename T, int kDP>
+template <typename T, int kDP, bool kTwo>
 __device__ __forceinline__ bool bwd_softmax(const FaBwdParams& p, const BwdCta<kDP>& c, uint32_t tmem, const BwdItem& w,
                                             BwdSoftmax& n) {
   using C = BwdCfg<kDP>;
@@ -921,7 +965,7 @@ __device__ __forceinline__ bool bwd_softmax(const FaBwdParams& p, const BwdCta<k
         cta_scale = exp2f(-e - BwdElem<T>::kPExp);
         unscale = exp2f(e);
       }
-      if (!bwd_tiles<T, kDP, true>(p, c, tS, tP, half, r, 0.f, 0.f, cta_scale, w, n)) return false;
+      if (!bwd_tiles<T, kDP, kTwo, true>(p, c, tS, tP, half, r, 0.f, 0.f, cta_scale, w, n)) return false;
     } else {
       float row_nl = 0.f, row_nd = 0.f;
       const int my = w.row0 + r;
@@ -935,7 +979,7 @@ __device__ __forceinline__ bool bwd_softmax(const FaBwdParams& p, const BwdCta<k
           unscale = exp2f(-e);
         }
       }
-      if (!bwd_tiles<T, kDP, false>(p, c, tS, tP, half, r, row_nl, row_nd, 1.f, w, n)) return false;
+      if (!bwd_tiles<T, kDP, kTwo, false>(p, c, tS, tP, half, r, row_nl, row_nd, 1.f, w, n)) return false;
     }
     if (!bwd_wait(c.done + (dkv ? half : 0), n.item.phase, c.abort_flag, kDevTimeoutO)) return false;
     tc_fence_after();
@@ -974,7 +1018,9 @@ __device__ __forceinline__ bool bwd_softmax(const FaBwdParams& p, const BwdCta<k
 // blocks that have not started, which it takes from the hardware scheduler
 // (cluster launch control).  Loads, products and softmax run ahead into the
 // next item, so only the accumulators' read-out separates two items.
-template <typename T, int kDP>
+// kTwo: items may have P and dS in two parts (a kernel of its own: as a branch
+// in the one for all calls it cost the others 2 to 5 %).
+template <typename T, int kDP, bool kTwo>
 __global__ void __launch_bounds__(384, 1)
     fa_bwd_kernel(const __grid_constant__ FaBwdParams p, const __grid_constant__ CUtensorMap k_a,
                   const __grid_constant__ CUtensorMap v_a, const __grid_constant__ CUtensorMap q_b,
@@ -1122,7 +1168,7 @@ __global__ void __launch_bounds__(384, 1)
 #pragma unroll 1
       for (int q = 0;; ++q) {
         get_item(q, w);
-        if (w.kind == kItemEnd || !bwd_issue<T, kDP>(c, tmem, leader, role, w, n)) break;
+        if (w.kind == kItemEnd || !bwd_issue<T, kDP, kTwo>(c, tmem, leader, role, w, n)) break;
       }
       // Drain the tensor pipe before TMEM is released.
       if (leader) mma_commit(c.drained + role);
@@ -1137,7 +1183,7 @@ __global__ void __launch_bounds__(384, 1)
 #pragma unroll 1
       for (int q = 0;; ++q) {
         get_item(q, w);
-        if (w.kind == kItemEnd || !bwd_softmax<T, kDP>(p, c, tmem, w, n)) break;
+        if (w.kind == kItemEnd || !bwd_softmax<T, kDP, kTwo>(p, c, tmem, w, n)) break;
       }
     }
   }

@@ -118,6 +118,7 @@ struct FaBwdParams {
   float scale;
   float scale_log2;
   int causal;
+  int few_rows;  // of queries, over all heads: P and dS in two parts
   int q_tiles, k_tiles;  // 128-row tiles of the longest sequence
   int num_dkv;           // items below this index form dK and dV, the others dQ
   // Slices of a tile's work (see bwd_slices): their length in streamed tiles
