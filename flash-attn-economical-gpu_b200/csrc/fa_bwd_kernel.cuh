@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(256) fa_bwd_zero_rest_kernel(const FaBwdParams
 // largest |dO|.  One CTA per kBS-row tile; kLanes lanes share a row, eight
 // columns each, so a warp reads whole 128-byte lines.
 template <typename T, int kBS, int kLanes>
-__global__ void __launch_bounds__(256) fa_bwd_stats_kernel(const FaBwdParams p) {
+__global__ void __launch_bounds__(256, 2) fa_bwd_stats_kernel(const FaBwdParams p) {
   // The main kernel may be set up meanwhile; it waits before it reads.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int bh = blockIdx.y;
@@ -206,30 +206,45 @@ __global__ void __launch_bounds__(256) fa_bwd_stats_kernel(const FaBwdParams p) 
   const int sub = threadIdx.x % kLanes, r0 = threadIdx.x / kLanes;
   const int col = sub * 8;
   float amax = 0.f;
-#pragma unroll 4
-  for (int r = r0; r < kBS; r += kRows) {
-    const int m = m0 + r;
-    float dot = 0.f, big = 0.f;
-    if (m < M && col < p.D) {
+  // All of a thread's loads are under way before the first is used: the
+  // kernel's time is one trip to memory where there are few rows.
+  constexpr int kSteps = kBS / kRows;
+  uint4 ow[kSteps], gw[kSteps];
+  float l[kSteps];
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    const int m = m0 + r0 + i * kRows;
+    ow[i] = gw[i] = make_uint4(0, 0, 0, 0);
+    l[i] = -INFINITY;
+    if (m < M) {
       const T* orow = o + m * p.o_ss + col;
       const T* grow = g + m * p.g_ss + col;
       if (col + 8 <= p.D) {
-        const uint4 ow = *reinterpret_cast<const uint4*>(orow), gw = *reinterpret_cast<const uint4*>(grow);
-        const T* oe = reinterpret_cast<const T*>(&ow);
-        const T* ge = reinterpret_cast<const T*>(&gw);
+        ow[i] = *reinterpret_cast<const uint4*>(orow);
+        gw[i] = *reinterpret_cast<const uint4*>(grow);
+      } else if (col < p.D) {
+        alignas(16) T part[2][8] = {};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float gv = BwdElem<T>::to_f(ge[e]);
-          dot = fmaf(BwdElem<T>::to_f(oe[e]), gv, dot);
-          big = fmaxf(big, fabsf(gv));
-        }
-      } else {
-        for (int e = 0; col + e < p.D; ++e) {
-          const float gv = BwdElem<T>::to_f(grow[e]);
-          dot = fmaf(BwdElem<T>::to_f(orow[e]), gv, dot);
-          big = fmaxf(big, fabsf(gv));
-        }
+        for (int e = 0; e < 8; ++e)
+          if (col + e < p.D) part[0][e] = orow[e], part[1][e] = grow[e];
+        ow[i] = *reinterpret_cast<const uint4*>(part[0]);
+        gw[i] = *reinterpret_cast<const uint4*>(part[1]);
       }
+      if (sub == 0) l[i] = lse[m * p.l_ss];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    const int r = r0 + i * kRows;
+    float dot = 0.f, big = 0.f;
+    const uint32_t* ov = reinterpret_cast<const uint32_t*>(&ow[i]);
+    const uint32_t* gv = reinterpret_cast<const uint32_t*>(&gw[i]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 of = BwdElem<T>::unpack2(ov[e]), gf = BwdElem<T>::unpack2(gv[e]);
+      dot = fmaf(of.x, gf.x, dot);
+      dot = fmaf(of.y, gf.y, dot);
+      big = fmaxf(big, fmaxf(fabsf(gf.x), fabsf(gf.y)));
     }
 #pragma unroll
     for (int off = kLanes / 2; off > 0; off >>= 1) {
@@ -237,9 +252,8 @@ __global__ void __launch_bounds__(256) fa_bwd_stats_kernel(const FaBwdParams p) 
       if constexpr (BwdElem<T>::kScaled) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
     }
     if (sub == 0) {
-      const float l = m < M ? lse[m * p.l_ss] : -INFINITY;
-      const bool none = l == -INFINITY;
-      st[r] = none ? -INFINITY : fmaf(-l, 1.4426950408889634f, BwdElem<T>::kPExp);
+      const bool none = l[i] == -INFINITY;
+      st[r] = none ? -INFINITY : fmaf(-l[i], 1.4426950408889634f, BwdElem<T>::kPExp);
       st[kBS + r] = none ? 0.f : -dot;
       if constexpr (BwdElem<T>::kScaled) {
         // 2^e * big in [1, 2); rows of zeros (and of infinities) keep their scale.
