@@ -176,12 +176,12 @@ void launch_stats(const FaBwdParams& kp, cudaStream_t stream) {
                   static_cast<unsigned>(kp.B * kp.Hq + (kp.cu_q != nullptr ? 3 : 0)));
   // Lanes per row: eight columns each.
   if constexpr (kBS == 64) {
-    fa_bwd_stats_kernel<T, 64, 32><<<grid, 256, 0, stream>>>(kp);
+    fa_bwd_stats_kernel<T, 64, 32><<<grid, kStatThreads, 0, stream>>>(kp);
   } else {
     if (kp.D <= 64)
-      fa_bwd_stats_kernel<T, 128, 8><<<grid, 256, 0, stream>>>(kp);
+      fa_bwd_stats_kernel<T, 128, 8><<<grid, kStatThreads, 0, stream>>>(kp);
     else
-      fa_bwd_stats_kernel<T, 128, 16><<<grid, 256, 0, stream>>>(kp);
+      fa_bwd_stats_kernel<T, 128, 16><<<grid, kStatThreads, 0, stream>>>(kp);
   }
 }
 
