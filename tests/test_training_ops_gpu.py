@@ -288,6 +288,8 @@ ROPES = [
     (18, 5, 0, 256, (0, 100, 28), torch.float16, torch.int32),     # an axis without pairs, no key heads
     (6, 1, 1, 2, (1,), torch.float32, torch.int64),
     (11, 33, 7, 96, (8, 16, 8), torch.bfloat16, torch.int32),
+    (70, 4, 2, 80, (8, 12), torch.float16, torch.int32),           # 20 pairs: 8-byte pieces
+    (70, 3, 1, 80, (7, 13), torch.bfloat16, torch.int64),          # and sections that cut them
 ]
 
 
