@@ -52,10 +52,6 @@ int run_fwd(const LayerNormParams& p, cudaStream_t st) {
   return launched();
 }
 
-// From this many rows per resident CTA on, the forward pass streams rows
-// through resident CTAs; below, every row has a CTA of its own.
-constexpr int64_t kStreamRows = 3;
-
 // Clusters of `ctas` CTAs that are resident together: all that the SMs have
 // room for, but the GPU's processing clusters are not a multiple of four CTAs
 // each.  (Measured: of the clusters of 4 and 8 that fill every SM some had to
@@ -117,6 +113,13 @@ int launch_rows(void (*kern)(P), const P& p, int64_t workers, int ctas, int thre
   return kErrLaunch;
 }
 
+// Rows stream through resident CTAs where each gets at least this many (kFewRows
+// otherwise: nothing was launched).  Measured, streamed against a CTA for every
+// row: 8192 x 3584 bf16 with a residual 47.8 against 57.3 us, 1200 x 3584 15.9
+// against 16.4, 148 x 3584 10.2 against 8.2; 32768 x 256 20.5 against 25.8.
+constexpr int64_t kStreamRows = 2;
+constexpr int kFewRows = -1;
+
 template <typename T, typename W, int NV, int kMaxThreads, int kMinCtas, bool kWide, bool kOdd>
 int run_fwd_stream(LayerNormParams p, cudaStream_t st) {
   constexpr int kStages = 3, V = 16 / sizeof(T);
@@ -124,7 +127,9 @@ int run_fwd_stream(LayerNormParams p, cudaStream_t st) {
   const Spread row = spread_row(places, kWide ? 1024 * V : places, 32 * V);
   p.span = row.span;
   const int threads = row_threads(kWide ? row.span : places, V, NV);
-  const int64_t workers = like_workers(resident(std::max(1, kResidentVectors / (threads * NV)), row.ctas), p.rows, kOdd);
+  const int64_t most = resident(std::max(1, kResidentVectors / (threads * NV)), row.ctas);
+  if (!kOdd && p.rows < kStreamRows * most) return kFewRows;
+  const int64_t workers = like_workers(most, p.rows, kOdd);
   return launch_rows(layernorm_fwd_stream_kernel<T, W, NV, kMaxThreads, kMinCtas, kStages, kWide, kOdd>, p, workers, row.ctas,
                      threads, size_t(kStages) * NV * 2 * threads * 16, st);
 }
@@ -139,15 +144,20 @@ int fwd(const LayerNormParams& p, cudaStream_t st) {
   const Rows kind = rows_kind(rows, p.cols, V, aligned(p.w, 16) && aligned(p.bias, 16));
   if (kind == Rows::kOdd && p.cols + V - 1 <= 1024 * V) return run_fwd_stream<T, W, 4, 256, 2, false, true>(p, st);
   if (kind == Rows::kOdd && p.cols + V - 1 <= kMaxCluster * 1024 * V) return run_fwd_stream<T, W, 4, 256, 2, true, true>(p, st);
-  if (kind == Rows::kEven && p.cols <= kMaxCluster * 1024 * V &&
-      p.rows >= kStreamRows * kSms * kResidentVectors / (p.cols / V)) {
-    if (p.cols <= 64 * V) return run_fwd_stream<T, W, 2, 32, 12, false, false>(p, st);
-    if (p.cols <= 1024 * V) return run_fwd_stream<T, W, 4, 256, 2, false, false>(p, st);
-    return run_fwd_stream<T, W, 4, 256, 2, true, false>(p, st);
-  }
   if (kind == Rows::kEven) {
-    // The fewest vectors per thread that keep the CTA within 512 threads, else
-    // within 1024.
+    // Up to 64 vectors a warp is a CTA: at 32768 x 256 20.5 us against 24.2
+    // with the wider form.
+    int rc = kFewRows;
+    if (p.cols <= 64 * V)
+      rc = run_fwd_stream<T, W, 2, 32, 12, false, false>(p, st);
+    else if (p.cols <= 1024 * V)
+      rc = run_fwd_stream<T, W, 4, 256, 2, false, false>(p, st);
+    else if (p.cols <= kMaxCluster * 1024 * V)
+      rc = run_fwd_stream<T, W, 4, 256, 2, true, false>(p, st);
+    if (rc != kFewRows) return rc;
+    // One vector per thread up to 512 threads, the quickest for one row's
+    // latency (148 x 3584 8.2 us against 10.2 with two); two up to there,
+    // then four (148 x 8192 10.2 us with two, 16.3 with four).
     if (p.cols <= 512 * V) return run_fwd<T, W, V, 1, 512>(p, st);
     if (p.cols <= 1024 * V) return run_fwd<T, W, V, 2, 512>(p, st);
     if (p.cols <= 4096 * V) return run_fwd<T, W, V, 4, 1024>(p, st);
@@ -213,11 +223,12 @@ int bwd(const LayerNormBwdParams& p, void* dw, void* db, cudaStream_t st) {
       rc = run_bwd<T, W, 4, 256, 2, false, false, true>(p, &lines, st);
     else
       rc = run_bwd<T, W, 4, 256, 2, false, true, true>(p, &lines, st);
-  } else if (p.cols <= 32 * V) {
-    rc = run_bwd<T, W, 1, 256, 3, true, false, false>(p, &lines, st);
   } else if (p.cols <= 64 * V) {
+    // A warp for each row (32768 x 512 bf16: 37.9 us against 50.2 with a CTA).
     rc = run_bwd<T, W, 2, 256, 2, true, false, false>(p, &lines, st);
   } else if (p.cols <= 256 * V) {
+    // Two vectors per thread while that leaves four warps or more for a row
+    // (8192 x 2048 bf16: 39.9 us against 44.0 with four).
     rc = run_bwd<T, W, 2, 128, 4, false, false, false>(p, &lines, st);
   } else if (p.cols <= 512 * V) {
     rc = run_bwd<T, W, 4, 128, 4, false, false, false>(p, &lines, st);
