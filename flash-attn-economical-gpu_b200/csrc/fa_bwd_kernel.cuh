@@ -24,19 +24,39 @@
 //
 // A CTA stays on its SM and takes item after item (a tile, or a slice of one
 // when there are few).  Warps 0 and 3 load (TMA; one operand each), warps 1
-// and 2 issue tcgen05.mma, warps 4-11 are two softmax warpgroups: each covers the 128 lanes and one half of
-// the streamed tile's columns.  Per streamed tile i
+// and 2 issue tcgen05.mma, warps 4-11 are two softmax warpgroups: each covers
+// the 128 lanes and one half of the streamed tile's columns.  Per streamed
+// tile i
 //   warp 1 issues  [dV(i)] S(i+1)      once P(i) is stored (dQ: S(i) read)
 //   warp 2 issues  dK(i)/dQ(i) dP(i+1) once dS(i) is stored
 // Each pair shares one TMEM buffer (P overwrites S, dS overwrites dP), whose
-// products its warp keeps in order; the two pairs touch different buffers and
-// need no order between them.  One issuing warp for all four left the tensor
-// core idle for the few hundred cycles that a warp's first wait after a burst
-// of products takes (measured: twice per tile, of some 3300 cycles); with two,
-// the other's products run meanwhile.  While the softmax warps turn S(i+1)
+// products its warp keeps in order; the two pairs touch different buffers, and
+// their bursts take turns, so that neither's products queue behind a second
+// burst of the other's.  One issuing warp for all four left the tensor core
+// idle for the few hundred cycles that a warp's first wait after a burst of
+// products takes (twice per tile, of some 3300 cycles then); with two, the
+// other's products run meanwhile.  While the softmax warps turn S(i+1)
 // into P the tensor core runs dK(i) and dP(i+1), and while they turn dP into
 // dS it runs dV(i) and S(i+1).  P overwrites its own half of S, dS its own
 // half of dP, so no warp writes columns another still has to read.
+//
+// What bounds it.  B1 H16 S4096 D128 (bf16, all pairs) takes 353 us, 973 TF/s
+// of the five products that the formula needs and 1360 TF/s of the seven that
+// run: the rate a plain GEMM sustains here under the power limit.  A tile of a
+// dK/dV item is 2048 tensor-core cycles against some 2400 of the softmax warps'
+// chain (S's wait, 64 exponentials a lane, P's store, dP's wait, dS's store).
+// Causal 4 x 32 heads of S 1024 (184 us, 467 TF/s) spends a further 15 % on the
+// accumulators' read-out and stores, which nothing overlaps (the stores alone
+// 3 %), and 15 us on the statistics.  At head dim 64 the same exponentials stand
+// against half the products: 32 heads S 4096 566 us, 607 TF/s.  At 256, 2 x 16
+// heads S 4096 causal 1170 us, 590 TF/s: products of 64 streamed rows read each
+// stationary operand from shared memory for half the work, some 2250 cycles of
+// its bandwidth against 1536 of the tensor core's; a second half-tile slot for
+// dO in place of its single one changed nothing.
+//
+// P and dS are handed on in halves (kHalves): B1 H16 S4096 353 us against 365
+// in one piece.  16 softmax warps (32 columns each) and exponentials by
+// polynomial on the FMA pipe were slower or no faster.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -1219,7 +1239,8 @@ __global__ void __launch_bounds__(384, 1)
 
 // Adds the slices of every tile that has more than one, in slice order, and
 // stores the result.  blockIdx.x: tile (as an item without its slice),
-// blockIdx.y: 32-column chunk of a thread's columns.
+// blockIdx.y: 32-column chunk of a thread's columns.  28 heads over 4, S 2048:
+// 8.4 us for the 64 key tiles' dK and dV.
 template <typename T, int kDP, bool kDkv>
 __global__ void __launch_bounds__(256) fa_bwd_join_kernel(const FaBwdParams p) {
   const int max_slices = kDkv ? p.dkv_slices : p.dq_slices;

@@ -348,7 +348,8 @@ struct LayerNormParams {
 // y = (x' - mean) * rsqrt(var + eps) * w + b per row, x' = x or round(x + residual).
 // One CTA per row; the row stays in registers (NV vectors of V per thread), so
 // it is read once, and the variance is the mean of squared distances from the
-// mean, not a difference of sums.
+// mean, not a difference of sums.  For calls of few rows, where one row's
+// latency is the time (1 x 3584 bf16 4.3 us).
 template <typename T, typename W, int V, int NV, int kMaxThreads>
 __global__ void __launch_bounds__(kMaxThreads) layernorm_fwd_kernel(const LayerNormParams p) {
   __shared__ float red[64];
@@ -444,6 +445,9 @@ __device__ __forceinline__ uint4 read_again(const uint4* p) {
 // vectors per thread.  kOdd: rows off the 16-byte grid, of which every CTA
 // takes some that start at the same offset (gridDim.x / ctas is a multiple of
 // 8, or there is one row each); the pieces at their ends are cut to the row.
+// Bound by memory: 8192 x 3584 bf16 with a residual moves 235 MB in 34.5 us,
+// 6.8 TB/s; 8192 x 3585 takes 71 us a call against 48 (its edges' values come
+// and go one by one), a cluster's 4096 x 16384 fp32 181 us for 1.07 GB.
 template <typename T, typename W, int NV, int kMaxThreads, int kMinCtas, int kStages, bool kWide, bool kOdd>
 __global__ void __launch_bounds__(kMaxThreads, kMinCtas) layernorm_fwd_stream_kernel(const LayerNormParams p) {
   constexpr int N = Pairs<T>::kN, V = 2 * N;
@@ -592,8 +596,9 @@ __global__ void __launch_bounds__(kMaxThreads, kMinCtas) layernorm_fwd_stream_ke
   if constexpr (kWide) cluster_sync();  // the others may still write their sums here
 }
 
-// Rows too long for the registers of one CTA: the same sums over three reads
-// of the row (the later ones from L2).
+// Rows too long for a cluster, or that lie at different places of a 16-byte
+// piece in different tensors: the same sums over three reads of the row (the
+// later ones from L2).  Rare, and 2 to 4 times the streamed kernels' time.
 template <typename T, typename W>
 __global__ void __launch_bounds__(1024) layernorm_fwd_long_kernel(const LayerNormParams p) {
   __shared__ float red[64];
@@ -658,6 +663,13 @@ struct LayerNormBwdParams {
 // and leaves once.  The next kStages - 1 rows are on their way into shared
 // memory while one is worked on, which keeps the memory busy across the
 // reduction that every row has in its middle; the weight waits in registers.
+// Wider than 1024 vectors, a row is shared by a cluster (kWide), and rows off
+// the 16-byte grid are taken in whole pieces (kOdd), as in the forward kernel.
+// Measured: 8192 x 3584 bf16 with dres 235 MB in 50 us, 4.7 TB/s, a third of
+// the issue slots: what bounds it is the latency of a row's two passes over
+// shared memory with the sum in between, at the 16 warps that the sums leave
+// registers for.  Three stages (one CTA less), 16 warps in one CTA, and dy and
+// xhat held in registers across the sum were all slower.
 template <typename T, typename W, int NV, int kMaxThreads, int kMinCtas, bool kWarpRow, bool kWide, bool kOdd, int kStages>
 __global__ void __launch_bounds__(kMaxThreads, kMinCtas) layernorm_bwd_kernel(const LayerNormBwdParams p) {
   constexpr int N = Pairs<T>::kN, V = 2 * N;
@@ -877,7 +889,8 @@ __global__ void __launch_bounds__(kMaxThreads, kMinCtas) layernorm_bwd_kernel(co
   }
 }
 
-// Rows too long for the registers: dx only, two reads of the row.
+// Rows too long for a cluster, or of unlike places: dx only, two reads of the
+// row; the column sums are left to the next kernel, which reads it again.
 template <typename T, typename W>
 __global__ void __launch_bounds__(1024) layernorm_bwd_long_kernel(const LayerNormBwdParams p) {
   __shared__ float red[64];
@@ -922,7 +935,9 @@ __global__ void __launch_bounds__(1024) layernorm_bwd_long_cols_kernel(const Lay
 
 // dw[c] = sum_i part[i][0][c], db[c] = sum_i part[i][1][c], in a fixed order:
 // 32 columns per CTA, warp x takes lines x, x + 32, ... (its loads all under
-// way together), the warps' sums are added in warp order.
+// way together), the warps' sums are added in warp order.  592 lines of 3584
+// columns, 17 MB mostly from L2: 7 us, of which setting it up under the
+// backward kernel (programmatic launch) hides a part.
 template <typename W>
 __global__ void __launch_bounds__(1024) layernorm_bwd_finish_kernel(const float* part, int lines, int cols, W* dw, W* db) {
   __shared__ float sums[32][33];
@@ -984,10 +999,12 @@ __device__ __forceinline__ int rope_row(const RopeParams& p, int axis, int64_t t
 // slots, ...): their cosines and sines are read once for all of them, and all
 // of their loads are under way before the first is used.  Memory-bound: q and
 // k in and out once; the table rows stay in L1 and L2.  A position outside the
-// table makes its pairs NaN; nothing is read out of bounds.
-constexpr int kRopeHeads = 2;
+// table makes its pairs NaN; nothing is read out of bounds.  Measured: a call of
+// 16384 tokens, 28 + 4 heads of 128, bf16, 268 MB, takes 53 us with a cold L2
+// (5.1 TB/s); two heads per thread 59, one 69, six 67, eight 55.
+constexpr int kRopeHeads = 4;
 template <typename T, int V>
-__global__ void __launch_bounds__(256, 4) rope_axes_kernel(const RopeParams p) {
+__global__ void __launch_bounds__(256, 3) rope_axes_kernel(const RopeParams p) {
   const int rot = p.half / V;                            // vectors of pairs
   const int nvec = rot + (p.head_dim - 2 * p.half) / V;  // and of columns to copy
   const int64_t id = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
