@@ -44,7 +44,8 @@ struct BwdPlan {
   int64_t stat_tiles;
   int dkv_slice_len, dkv_slices, dq_slice_len, dq_slices;
   int64_t part_k_tiles, part_q_tiles;
-  size_t row_exp, tile_max, dkv_part, dq_part, bytes;
+  int64_t key_tiles;
+  size_t row_norm, tile_max, key_max, dkv_part, dq_part, bytes;
 };
 
 // Streamed tiles a tile works through, summed over the tiles of one head (of
@@ -104,10 +105,13 @@ BwdPlan make_plan(const fab_attention_bwd_params* p) {
   choose_slices(ceil_div(N, bs), share / 3, &w.dq_slice_len, &w.dq_slices);
   const int64_t tiles = w.stat_tiles * per_q;
   size_t at = round256(size_t(tiles) * 2 * bs * sizeof(float));
-  w.row_exp = at;
+  w.row_norm = at;
   if (p->dtype == kDtypeF16) at += round256(size_t(tiles) * bs * sizeof(float));
   w.tile_max = at;
   if (p->dtype == kDtypeF16) at += round256(size_t(tiles) * sizeof(float));
+  w.key_max = at;
+  w.key_tiles = packed ? p->total_k / bs + int64_t(p->batch) + 1 : ceil_div(N, bs);
+  if (p->dtype == kDtypeF16) at += round256(size_t(w.key_tiles) * per_kv * sizeof(float));
   const int dp = padded_head_dim(p->head_dim);
   w.dkv_part = at;
   if (w.dkv_slices > 1) at += size_t(w.part_k_tiles) * per_kv * w.dkv_slices * 2 * dp * 128 * sizeof(float);
@@ -172,8 +176,9 @@ int validate(const fab_attention_bwd_params* p, bool* empty) {
 
 template <typename T, int kBS>
 void launch_stats(const FaBwdParams& kp, cudaStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(ceil_div(kp.M, kBS)),
-                  static_cast<unsigned>(kp.B * kp.Hq + (kp.cu_q != nullptr ? 3 : 0)));
+  constexpr bool kKeys = BwdElem<T>::kScaled;
+  const dim3 grid(static_cast<unsigned>(ceil_div(kKeys ? std::max(kp.M, kp.N) : kp.M, kBS)),
+                  static_cast<unsigned>(kp.B * (kp.Hq + (kKeys ? kp.Hkv : 0)) + (kp.cu_q != nullptr ? 3 : 0)));
   // Lanes per row: eight columns each.
   if constexpr (kBS == 64) {
     fa_bwd_stats_kernel<T, 64, 32><<<grid, kStatThreads, 0, stream>>>(kp);
@@ -222,7 +227,7 @@ int launch(const fab_attention_bwd_params* p, FaBwdParams& kp, cudaStream_t stre
       if ((rc = map(&kb, p->k, k_rows, kp.Hkv, p->k_stride_s, p->k_stride_h, p->k_stride_b, C::kBS))) return rc;
       if ((rc = map(&vb, p->v, k_rows, kp.Hkv, p->v_stride_s, p->v_stride_h, p->v_stride_b, C::kBS))) return rc;
     }
-    if (static_cast<int64_t>(kp.B) * kp.Hq > 65000) return kErrUnsupported;
+    if (static_cast<int64_t>(kp.B) * (kp.Hq + (BwdElem<T>::kScaled ? kp.Hkv : 0)) > 65000) return kErrUnsupported;
   } else {
     // Nothing attends to anything: the items write zeros and read no map.
     qa = ga = ka = va = qb = gb = kb = vb = CUtensorMap{};
@@ -334,8 +339,14 @@ int fab_attention_bwd(const fab_attention_bwd_params* p, void* stream) {
   kp.dv_sh = p->dv_stride_h;
   kp.dv_ss = p->dv_stride_s;
   kp.stats = reinterpret_cast<float*>(ws);
-  kp.row_exp = reinterpret_cast<float*>(ws + w.row_exp);
+  kp.row_norm = reinterpret_cast<float*>(ws + w.row_norm);
   kp.tile_max = reinterpret_cast<float*>(ws + w.tile_max);
+  kp.key_max = reinterpret_cast<float*>(ws + w.key_max);
+  kp.key_tiles = static_cast<int>(w.key_tiles);
+  kp.v = p->v;
+  kp.v_sb = p->v_stride_b;
+  kp.v_sh = p->v_stride_h;
+  kp.v_ss = p->v_stride_s;
   kp.stat_tiles = static_cast<int>(w.stat_tiles);
   kp.B = p->batch;
   kp.Hq = p->heads_q;

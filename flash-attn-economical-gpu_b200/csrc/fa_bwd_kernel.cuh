@@ -91,8 +91,11 @@ struct BwdElem<__half> {
   // dS = P * (dP - delta) is rounded to fp16 as an operand, and P is about
   // 1/keys: with the small dO of real training it would fall below fp16's
   // normal range although dQ and dK do not.  dS is therefore formed times a
-  // power of two that brings the largest |dO| of its row (dQ) or of the item's
-  // rows (dK) to [1, 2); the epilogue divides it out.
+  // power of two that brings the bound 2 |dO_m| |V_n| (Euclidean norms, the
+  // largest of the row or of the item's rows, and of the sequence's keys) to
+  // [2^14, 2^15); the epilogue divides it out.  (With the largest element of dO
+  // brought to [1, 2) instead, 8092 keys and rows of different size took the
+  // error against 64 bits to 1.6 times the rounding's; now 1.4.)
   static constexpr bool kScaled = true;
   // P itself is an operand of dV: as P * 2^12 it keeps its precision down to
   // 2^-26, and its largest value, 1, stays far below fp16's 65504.
@@ -158,6 +161,18 @@ __device__ __forceinline__ int64_t bwd_stat_tile0(const FaBwdParams& p, int b, i
                            : (static_cast<int64_t>(b) * p.Hq + h) * p.stat_tiles;
 }
 
+// The same for keys' tiles of kBS rows, in which V's norms are taken (fp16).
+__device__ __forceinline__ int64_t bwd_key_tile0(const FaBwdParams& p, int b, int h, int k_row0, int bs) {
+  return p.cu_k != nullptr ? static_cast<int64_t>(h) * p.key_tiles + k_row0 / bs + b
+                           : (static_cast<int64_t>(b) * p.Hkv + h) * p.key_tiles;
+}
+
+// The exponent of dS's scale where dO's and V's norms are the roots of g2, v2.
+__device__ __forceinline__ float bwd_scale_exp(float g2, float v2) {
+  const float b = 0.5f * (log2f(g2) + log2f(v2));
+  return g2 > 0.f && g2 < INFINITY && v2 > 0.f && v2 < INFINITY ? fminf(13.f - floorf(b), 60.f) : 0.f;
+}
+
 // First row and length of batch entry b.  Packed offsets are clamped to the
 // tensor and to the declared longest length, so that no offset makes the
 // kernels touch memory outside it.
@@ -200,8 +215,9 @@ __global__ void __launch_bounds__(256) fa_bwd_zero_rest_kernel(const FaBwdParams
 
 // Per query row: -lse * log2(e), plus kPExp, (-inf for rows that saw no key and for the
 // padding rows of the last tile, so that P is 0 there) and -delta, as
-// [tile][2][kBS]; for fp16 also the row's scale exponent and the tile's
-// largest |dO|.  One CTA per kBS-row tile; kLanes lanes share a row, eight
+// [tile][2][kBS]; for fp16 also the row's squared norm of dO and the tile's
+// largest, and from further CTAs those of V's rows, the tiles' largest
+// only.  One CTA per kBS-row tile; kLanes lanes share a row, eight
 // columns each, so a warp reads whole 128-byte lines.  Measured: 4 x 32 heads,
 // S 1024, 67 MB, 15 us (18 with 256 threads, 22 with 1024); 2 x 16 heads, S
 // 8192, 134 MB, 25.5 us, 5.3 TB/s.
@@ -210,20 +226,31 @@ template <typename T, int kBS, int kLanes>
 __global__ void __launch_bounds__(kStatThreads, 2) fa_bwd_stats_kernel(const FaBwdParams p) {
   // The main kernel may be set up meanwhile; it waits before it reads.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int bh = blockIdx.y;
-  if (bh >= p.B * p.Hq) {  // three more rows of CTAs, for packed batches
-    bwd_zero_rest<T>(p, bh - p.B * p.Hq);
+  // Rows of CTAs: query heads, for fp16 key/value heads, and three more for
+  // packed batches.
+  int bh = blockIdx.y;
+  const bool keys = BwdElem<T>::kScaled && bh >= p.B * p.Hq && bh < p.B * (p.Hq + p.Hkv);
+  if (bh >= p.B * p.Hq && !keys) {
+    bwd_zero_rest<T>(p, bh - p.B * (p.Hq + (BwdElem<T>::kScaled ? p.Hkv : 0)));
     return;
   }
-  const int b = bh / p.Hq, h = bh % p.Hq;
+  if (keys) bh -= p.B * p.Hq;
+  const int heads = keys ? p.Hkv : p.Hq;
+  const int b = bh / heads, h = bh % heads;
   int q0, M;
-  bwd_seq(p.cu_q, b, p.total_q, p.M, q0, M);
+  if (keys)
+    bwd_seq(p.cu_k, b, p.total_k, p.N, q0, M);
+  else
+    bwd_seq(p.cu_q, b, p.total_q, p.M, q0, M);
   const int m0 = blockIdx.x * kBS;
   if (m0 >= M) return;
-  const T* o = reinterpret_cast<const T*>(p.o) + (p.cu_q ? q0 * p.o_ss : b * p.o_sb) + h * p.o_sh;
-  const T* g = reinterpret_cast<const T*>(p.dout) + (p.cu_q ? q0 * p.g_ss : b * p.g_sb) + h * p.g_sh;
+  // For keys both operands are V.
+  const int64_t o_ss = keys ? p.v_ss : p.o_ss, g_ss = keys ? p.v_ss : p.g_ss;
+  const T* v = reinterpret_cast<const T*>(p.v) + (p.cu_k ? q0 * p.v_ss : b * p.v_sb) + h * p.v_sh;
+  const T* o = keys ? v : reinterpret_cast<const T*>(p.o) + (p.cu_q ? q0 * p.o_ss : b * p.o_sb) + h * p.o_sh;
+  const T* g = keys ? v : reinterpret_cast<const T*>(p.dout) + (p.cu_q ? q0 * p.g_ss : b * p.g_sb) + h * p.g_sh;
   const float* lse = p.lse + (p.cu_q ? q0 * p.l_ss : b * p.l_sb) + h * p.l_sh;
-  const int64_t tile = bwd_stat_tile0(p, b, h, q0, kBS) + blockIdx.x;
+  const int64_t tile = (keys ? bwd_key_tile0(p, b, h, q0, kBS) : bwd_stat_tile0(p, b, h, q0, kBS)) + blockIdx.x;
   float* st = p.stats + tile * (2 * kBS);
   constexpr int kRows = kStatThreads / kLanes;  // rows of one pass over the CTA
   const int sub = threadIdx.x % kLanes, r0 = threadIdx.x / kLanes;
@@ -240,8 +267,8 @@ __global__ void __launch_bounds__(kStatThreads, 2) fa_bwd_stats_kernel(const FaB
     ow[i] = gw[i] = make_uint4(0, 0, 0, 0);
     l[i] = -INFINITY;
     if (m < M) {
-      const T* orow = o + m * p.o_ss + col;
-      const T* grow = g + m * p.g_ss + col;
+      const T* orow = o + m * o_ss + col;
+      const T* grow = g + m * g_ss + col;
       if (col + 8 <= p.D) {
         ow[i] = *reinterpret_cast<const uint4*>(orow);
         gw[i] = *reinterpret_cast<const uint4*>(grow);
@@ -253,13 +280,13 @@ __global__ void __launch_bounds__(kStatThreads, 2) fa_bwd_stats_kernel(const FaB
         ow[i] = *reinterpret_cast<const uint4*>(part[0]);
         gw[i] = *reinterpret_cast<const uint4*>(part[1]);
       }
-      if (sub == 0) l[i] = lse[m * p.l_ss];
+      if (sub == 0 && !keys) l[i] = lse[m * p.l_ss];
     }
   }
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) {
     const int r = r0 + i * kRows;
-    float dot = 0.f, big = 0.f;
+    float dot = 0.f, norm = 0.f;
     const uint32_t* ov = reinterpret_cast<const uint32_t*>(&ow[i]);
     const uint32_t* gv = reinterpret_cast<const uint32_t*>(&gw[i]);
 #pragma unroll
@@ -267,22 +294,22 @@ __global__ void __launch_bounds__(kStatThreads, 2) fa_bwd_stats_kernel(const FaB
       const float2 of = BwdElem<T>::unpack2(ov[e]), gf = BwdElem<T>::unpack2(gv[e]);
       dot = fmaf(of.x, gf.x, dot);
       dot = fmaf(of.y, gf.y, dot);
-      big = fmaxf(big, fmaxf(fabsf(gf.x), fabsf(gf.y)));
+      if constexpr (BwdElem<T>::kScaled) norm = fmaf(gf.x, gf.x, fmaf(gf.y, gf.y, norm));
     }
 #pragma unroll
     for (int off = kLanes / 2; off > 0; off >>= 1) {
       dot += __shfl_xor_sync(0xffffffffu, dot, off);
-      if constexpr (BwdElem<T>::kScaled) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
+      if constexpr (BwdElem<T>::kScaled) norm += __shfl_xor_sync(0xffffffffu, norm, off);
     }
     if (sub == 0) {
-      const bool none = l[i] == -INFINITY;
-      st[r] = none ? -INFINITY : fmaf(-l[i], 1.4426950408889634f, BwdElem<T>::kPExp);
-      st[kBS + r] = none ? 0.f : -dot;
+      if (!keys) {
+        const bool none = l[i] == -INFINITY;
+        st[r] = none ? -INFINITY : fmaf(-l[i], 1.4426950408889634f, BwdElem<T>::kPExp);
+        st[kBS + r] = none ? 0.f : -dot;
+      }
       if constexpr (BwdElem<T>::kScaled) {
-        // 2^e * big in [1, 2); rows of zeros (and of infinities) keep their scale.
-        const float e = big > 0.f && big < INFINITY ? -floorf(log2f(big)) : 0.f;
-        p.row_exp[tile * kBS + r] = e;
-        if (big < INFINITY) amax = fmaxf(amax, big);
+        if (!keys) p.row_norm[tile * kBS + r] = norm;
+        if (norm < INFINITY) amax = fmaxf(amax, norm);
       }
     }
   }
@@ -294,7 +321,7 @@ __global__ void __launch_bounds__(kStatThreads, 2) fa_bwd_stats_kernel(const FaB
     __syncthreads();
     if (threadIdx.x == 0) {
       for (int w = 1; w < kStatThreads / 32; ++w) amax = fmaxf(amax, red[w]);
-      p.tile_max[tile] = amax;
+      (keys ? p.key_max : p.tile_max)[tile] = amax;
     }
   }
 }
@@ -972,6 +999,20 @@ __device__ __forceinline__ bool bwd_tiles(const FaBwdParams& p, const BwdCta<kDP
   return true;
 }
 
+__device__ __forceinline__ float bwd_warp_max(float x) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
+  return x;
+}
+// The largest squared norm of the sequence's V rows.
+template <int kBS>
+__device__ __forceinline__ float bwd_key_norm(const FaBwdParams& p, const BwdItem& w, int h) {
+  const float* at = p.key_max + bwd_key_tile0(p, w.b, h, w.k_row0, kBS);
+  float big = 0.f;
+  for (int x = threadIdx.x & 31; x * kBS < w.N; x += 32) big = fmaxf(big, at[x]);
+  return bwd_warp_max(big);
+}
+
 template <typename T, int kDP, bool kTwo>
 __device__ __forceinline__ bool bwd_softmax(const FaBwdParams& p, const BwdCta<kDP>& c, uint32_t tmem, const BwdItem& w,
                                             BwdSoftmax& n) {
@@ -989,29 +1030,29 @@ __device__ __forceinline__ bool bwd_softmax(const FaBwdParams& p, const BwdCta<k
     if (dkv) {
       float cta_scale = 1.f;
       if constexpr (BwdElem<T>::kScaled) {
-        // Largest |dO| over every row this item sums.
+        // The largest |dO| over every row that this item sums.
         float big = 0.f;
         for (int x = lane; x < w.nt; x += 32) {
           const int j = w.begin + x;
           big = fmaxf(big, p.tile_max[bwd_stat_tile0(p, w.b, w.h * p.group + j / w.per_head, w.q_row0, kBS) + w.first +
                                       j % w.per_head]);
         }
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
-        const float e = big > 0.f ? floorf(log2f(big)) : 0.f;
-        cta_scale = exp2f(-e - BwdElem<T>::kPExp);
-        unscale = exp2f(e);
+        const float e = bwd_scale_exp(bwd_warp_max(big), bwd_key_norm<kBS>(p, w, w.h));
+        cta_scale = exp2f(e - BwdElem<T>::kPExp);
+        unscale = exp2f(-e);
       }
       if (!bwd_tiles<T, kDP, kTwo, true>(p, c, tS, tP, half, r, 0.f, 0.f, cta_scale, w, n)) return false;
     } else {
       float row_nl = 0.f, row_nd = 0.f;
       const int my = w.row0 + r;
+      [[maybe_unused]] float v2 = 0.f;
+      if constexpr (BwdElem<T>::kScaled) v2 = bwd_key_norm<kBS>(p, w, w.h / p.group);
       if (my < w.M) {
         const int64_t st_tile = bwd_stat_tile0(p, w.b, w.h, w.q_row0, kBS) + my / kBS;
         row_nl = p.stats[st_tile * (2 * kBS) + my % kBS];
         row_nd = p.stats[st_tile * (2 * kBS) + kBS + my % kBS];
         if constexpr (BwdElem<T>::kScaled) {
-          const float e = p.row_exp[st_tile * kBS + my % kBS];
+          const float e = bwd_scale_exp(p.row_norm[st_tile * kBS + my % kBS], v2);
           row_nl += e - BwdElem<T>::kPExp;  // P, hence dS, times 2^e
           unscale = exp2f(-e);
         }

@@ -103,15 +103,19 @@ struct FaBwdParams {
   int64_t o_sb, o_sh, o_ss;
   int64_t g_sb, g_sh, g_ss;  // dout
   int64_t l_sb, l_sh, l_ss;
+  const void* v;
+  int64_t v_sb, v_sh, v_ss;
   int64_t dq_sb, dq_sh, dq_ss;
   int64_t dk_sb, dk_sh, dk_ss;
   int64_t dv_sb, dv_sh, dv_ss;
   // Workspace.  Per streamed-tile-sized tile of query rows, [2][rows]:
-  // -lse * log2(e) and -delta; for fp16 each row's scale exponent and each
-  // tile's largest |dout| too.
+  // -lse * log2(e) and -delta; for fp16 each row's squared norm of dout, each
+  // tile's largest, and the largest of V's rows for each tile of keys.
   float* stats;
-  float* row_exp;
+  float* row_norm;
   float* tile_max;
+  float* key_max;
+  int key_tiles;   // of one head, numbered like stat_tiles
   int stat_tiles;  // tiles of one head (dense: of one batch entry's head)
   int B, Hq, Hkv, M, N, D;  // M, N: longest lengths of a packed batch
   int group;

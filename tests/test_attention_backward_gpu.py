@@ -219,6 +219,20 @@ def test_fp16_gradients_keep_their_precision_at_any_size(exp, cuda_device):
     _assert_within(got, *_reference(small, q, k, v, o, lse, False, D ** -0.5))
 
 
+@pytest.mark.parametrize("vexp, dexp", [(9, 0), (9, 5), (-12, -8), (3, -12)])
+def test_fp16_values_of_any_size(vexp, dexp, cuda_device):
+    """Values and gradients times powers of two, among them one key 2^4 larger: nothing overflows inside, and small
+    ones keep their precision."""
+    dout, q, k, v = _inputs(1, 2, 1, 300, 900, 128, torch.float16, cuda_device, 14, 2.0 ** dexp)
+    v = (v.double() * 2.0 ** vexp).half()
+    v[:, :, 77] *= 16
+    q, k = q * 0.125, k * 0.125  # flat rows, and gradients that stay in range
+    o, lse = attention_forward(q, k, v, return_lse=True)
+    got = attention_backward(dout, q, k, v, o, lse)
+    assert torch.isfinite(torch.cat([t.flatten() for t in got])).all()
+    _assert_within(got, *_reference(dout, q, k, v, o, lse, False, 128 ** -0.5))
+
+
 def test_rows_of_very_different_gradients(cuda_device):
     """Single query rows whose dout is 2^-10 of the others' keep their dq in fp16."""
     dout, q, k, v = _inputs(1, 1, 1, 256, 2048, 64, torch.float16, cuda_device, 12)
