@@ -665,7 +665,7 @@ struct LayerNormBwdParams {
 // reduction that every row has in its middle; the weight waits in registers.
 // Wider than 1024 vectors, a row is shared by a cluster (kWide), and rows off
 // the 16-byte grid are taken in whole pieces (kOdd), as in the forward kernel.
-// Measured: 8192 x 3584 bf16 with dres 235 MB in 50 us, 4.7 TB/s, a third of
+// Measured: 8192 x 3584 bf16 with dres 235 MB in 50 us, 4.7 TB/s, two fifths of
 // the issue slots: what bounds it is the latency of a row's two passes over
 // shared memory with the sum in between, at the 16 warps that the sums leave
 // registers for.  Three stages (one CTA less), 16 warps in one CTA, and dy and

@@ -161,12 +161,14 @@ int fab_attention_fwd_varlen(const fab_attention_varlen_params* params, void* st
  *   dq = sm_scale dS k, dk = sm_scale sum dS^T q, dv = sum P^T dout,
  * the sums over the query heads that share a key/value head.  The
  * probabilities are recomputed; P and dS are rounded to the input type as
- * tensor-core operands, all sums are fp32 in a fixed order (the same bits on
- * every call).  fp16 operands are scaled by powers of two inside, so small
- * gradients do not underflow.  Masks as in the forward.  Query rows that see no key (lse -inf; their o
- * is ignored) get dq 0, keys that no query sees dk = dv = 0, and rows of a
- * packed tensor outside [cu[0], cu[batch]) zero gradients.  No counterpart in
- * the reference, which has no backward pass.
+ * tensor-core operands (in two parts where a sequence or the call is short),
+ * all sums are fp32 in a fixed order (the same bits on every call).  fp16
+ * operands are scaled by powers of two inside, from the norms of dout's and v's
+ * rows: small gradients do not underflow, large values do not overflow.  Masks
+ * as in the forward.  Query rows that see no key (lse -inf; their o is ignored)
+ * get dq 0, keys that no query sees dk = dv = 0, and rows of a packed tensor
+ * outside [cu[0], cu[batch]) zero gradients.  No counterpart in the reference,
+ * which has no backward pass.
  *
  * f16 or bf16 (FAB_ERR_UNSUPPORTED for f32: the forward's f32 runs as tf32),
  * head_dim <= 256, any finite sm_scale.  Tensors as in the forward: element
