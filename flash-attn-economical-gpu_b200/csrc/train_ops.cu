@@ -195,8 +195,16 @@ int run_bwd(LayerNormBwdParams p, int* lines, cudaStream_t st) {
   constexpr int kStages = 2;
   size_t smem = size_t(kStages) * NV * 3 * threads * 16;
   const int vectors = threads * NV;  // of one row, or of all the warps' rows
-  const int64_t most = std::min(resident(std::max(1, kResidentVectors / vectors), row.ctas), max_lines(p.rows, p.cols));
-  *lines = static_cast<int>(like_workers(most, kWarpRow ? ceil_div(p.rows, threads / 32) : p.rows, kOdd && !kWarpRow));
+  const int64_t rows = kWarpRow ? ceil_div(p.rows, threads / 32) : p.rows;  // one after another, if by one CTA
+  // Every CTA leaves a line of sums, as many bytes as two fp32 rows, which the
+  // finish kernel reads: with few rows in all, fewer CTAs of several rows each,
+  // but one per SM.  Measured, against a row each: 4096 x 1024 bf16 (four) 19.4
+  // and 25.6 us, 600 x 3584 (two; four 21.5) 19.4 and 21.1, 4096 x 256 (two;
+  // four 13.3) 11.4 and 15.3.
+  constexpr int kLineRows = !kWarpRow && NV == 2 ? 4 : 2;
+  const int64_t most = std::min({resident(std::max(1, kResidentVectors / vectors), row.ctas), max_lines(p.rows, p.cols),
+                                 std::max<int64_t>(kSms / row.ctas, ceil_div(rows, kLineRows))});
+  *lines = static_cast<int>(like_workers(most, rows, kOdd && !kWarpRow));
   if (kWarpRow) smem = std::max(smem, size_t(threads / 32) * p.cols * sizeof(float));
   return launch_rows(layernorm_bwd_kernel<T, W, NV, kMaxThreads, kMinCtas, kWarpRow, kWide, kOdd, kStages>, p, *lines,
                      row.ctas, threads, smem, st);
