@@ -530,6 +530,12 @@ def _conform_operand(t: torch.Tensor) -> torch.Tensor:
     return _conform(t)
 
 
+def _empty_gradient(t: torch.Tensor) -> torch.Tensor:
+    """Uninitialised gradient of `t`, in its layout where that has unit stride along head_dim, else contiguous."""
+    g = torch.empty_like(t)
+    return g if g.stride(-1) == 1 else t.new_empty(t.shape)
+
+
 # fab_attention_bwd_params as one packed record: filling its fifty-odd fields one by one costs more than the launches
 # of a short call.
 _BWD_RECORD = struct.Struct("9P27q2P9ifiPN")
@@ -579,7 +585,7 @@ def _launch_attention_backward(what, dout, q, k, v, out, lse, causal, sm_scale, 
     if padded:
         outs = tuple(_padded_like(t) for t in (q, k, v))
     else:
-        outs = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+        outs = _empty_gradient(q), _empty_gradient(k), _empty_gradient(v)
     if B == 0 or (M == 0 and N == 0):
         return tuple(t.contiguous() for t in outs) if padded else outs
     ins = [_conform_operand(t) if t.numel() else t for t in (q, k, v, out, dout)]
