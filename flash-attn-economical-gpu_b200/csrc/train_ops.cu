@@ -219,10 +219,11 @@ int bwd(const LayerNormBwdParams& p, void* dw, void* db, cudaStream_t st) {
   int rc, lines = 0;
   if (kind == Rows::kAny || places > kMaxCluster * 1024 * V) {
     lines = static_cast<int>(max_lines(p.rows, p.cols));
-    layernorm_bwd_long_kernel<T, W><<<static_cast<unsigned>(p.rows), long_threads(p.cols), 0, st>>>(p);
+    // The column sums first: dx may lie over dy.
     if (p.part != nullptr)
       layernorm_bwd_long_cols_kernel<T>
           <<<dim3(static_cast<unsigned>(ceil_div(p.cols, 1024)), static_cast<unsigned>(lines)), long_threads(p.cols), 0, st>>>(p);
+    layernorm_bwd_long_kernel<T, W><<<static_cast<unsigned>(p.rows), long_threads(p.cols), 0, st>>>(p);
     rc = launched();
   } else if (kind == Rows::kOdd) {
     if (places <= 64 * V)

@@ -890,7 +890,8 @@ __global__ void __launch_bounds__(kMaxThreads, kMinCtas) layernorm_bwd_kernel(co
 }
 
 // Rows too long for a cluster, or of unlike places: dx only, two reads of the
-// row; the column sums are left to the next kernel, which reads it again.
+// row.  The column sums are another kernel's, which reads dy and x again and
+// runs before this one, whose dx may lie over dy.
 template <typename T, typename W>
 __global__ void __launch_bounds__(1024) layernorm_bwd_long_kernel(const LayerNormBwdParams p) {
   __shared__ float red[64];
@@ -915,7 +916,7 @@ __global__ void __launch_bounds__(1024) layernorm_bwd_long_kernel(const LayerNor
   }
 }
 
-// The column sums those rows leave: CTA (x, y) sums rows y, y + gridDim.y, ...
+// The column sums of those rows: CTA (x, y) sums rows y, y + gridDim.y, ...
 // of 1024 columns into its line of `part`.
 template <typename T>
 __global__ void __launch_bounds__(1024) layernorm_bwd_long_cols_kernel(const LayerNormBwdParams p) {
