@@ -45,6 +45,8 @@ struct BwdPlan {
   int dkv_slice_len, dkv_slices, dq_slice_len, dq_slices;
   int64_t part_k_tiles, part_q_tiles;
   int64_t key_tiles;
+  int64_t dkv_tiles, dq_tiles;  // stationary tiles of all heads, a half-head's each where a tile takes two items
+  int64_t stat_q, stat_k;       // tiles of the longest sequence that the statistics kernel visits
   size_t row_norm, tile_max, key_max, dkv_part, dq_part, bytes;
 };
 
@@ -112,6 +114,10 @@ BwdPlan make_plan(const fab_attention_bwd_params* p) {
   w.key_max = at;
   w.key_tiles = packed ? p->total_k / bs + int64_t(p->batch) + 1 : ceil_div(N, bs);
   if (p->dtype == kDtypeF16) at += round256(size_t(w.key_tiles) * per_kv * sizeof(float));
+  w.dkv_tiles = int64_t(p->batch) * p->heads_kv * w.k_tiles * dsplit;
+  w.dq_tiles = int64_t(p->batch) * p->heads_q * w.q_tiles;
+  w.stat_q = ceil_div(M, bs);
+  w.stat_k = ceil_div(N, bs);
   const int dp = padded_head_dim(p->head_dim);
   w.dkv_part = at;
   if (w.dkv_slices > 1) at += size_t(w.part_k_tiles) * per_kv * w.dkv_slices * 2 * dp * 128 * sizeof(float);
@@ -119,6 +125,18 @@ BwdPlan make_plan(const fab_attention_bwd_params* p) {
   if (w.dq_slices > 1) at += size_t(w.part_q_tiles) * per_q * w.dq_slices * dp * 128 * sizeof(float);
   w.bytes = at;
   return w;
+}
+
+// CTAs of the statistics kernel, and whether it, the items and the statistics'
+// lines can be numbered in 31 bits.
+int64_t stat_ctas(const fab_attention_bwd_params* p, const BwdPlan& w) {
+  return int64_t(p->batch) * (w.stat_q * p->heads_q + (p->dtype == kDtypeF16 ? w.stat_k * p->heads_kv : 0)) +
+         (p->cu_seqlens_q != nullptr ? 3 * std::max(w.stat_q, w.stat_k) : 0);
+}
+bool numbered(const fab_attention_bwd_params* p, const BwdPlan& w) {
+  constexpr double kMost = 0x7fffffff;
+  return double(w.dkv_tiles) * w.dkv_slices + double(w.dq_tiles) * w.dq_slices <= kMost && stat_ctas(p, w) <= kMost &&
+         w.stat_tiles <= kMost && w.key_tiles <= kMost && w.part_q_tiles <= kMost && w.part_k_tiles <= kMost;
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -146,6 +164,7 @@ int validate(const fab_attention_bwd_params* p, bool* empty) {
     return kOk;
   }
   if (p->heads_kv == 0 ? p->heads_q != 0 : p->heads_q % p->heads_kv != 0) return kErrInvalidArg;
+  if (int64_t(p->batch) * p->heads_q > 0x7fffffff) return kErrUnsupported;
   const int64_t q_rows = packed ? p->total_q : p->seqlen_q, k_rows = packed ? p->total_k : p->seqlen_k;
   const int64_t nb = packed ? 1 : p->batch;
   const bool has_q = q_rows > 0 && p->heads_q > 0, has_k = k_rows > 0 && p->heads_kv > 0;
@@ -175,10 +194,8 @@ int validate(const fab_attention_bwd_params* p, bool* empty) {
 }
 
 template <typename T, int kBS>
-void launch_stats(const FaBwdParams& kp, cudaStream_t stream) {
-  constexpr bool kKeys = BwdElem<T>::kScaled;
-  const dim3 grid(static_cast<unsigned>(ceil_div(kKeys ? std::max(kp.M, kp.N) : kp.M, kBS)),
-                  static_cast<unsigned>(kp.B * (kp.Hq + (kKeys ? kp.Hkv : 0)) + (kp.cu_q != nullptr ? 3 : 0)));
+void launch_stats(const FaBwdParams& kp, int64_t ctas, cudaStream_t stream) {
+  const unsigned grid = static_cast<unsigned>(ctas);
   // Lanes per row: eight columns each.
   if constexpr (kBS == 64) {
     fa_bwd_stats_kernel<T, 64, 32><<<grid, kStatThreads, 0, stream>>>(kp);
@@ -191,7 +208,7 @@ void launch_stats(const FaBwdParams& kp, cudaStream_t stream) {
 }
 
 template <typename T, int kDP, bool kTwo>
-int launch(const fab_attention_bwd_params* p, FaBwdParams& kp, cudaStream_t stream) {
+int launch(const fab_attention_bwd_params* p, const BwdPlan& w, FaBwdParams& kp, cudaStream_t stream) {
   using C = BwdCfg<kDP>;
   auto kern = fa_bwd_kernel<T, kDP, kTwo>;
   int rc = ensure_smem_attr(reinterpret_cast<const void*>(kern), C::kSmemBytes);
@@ -227,19 +244,15 @@ int launch(const fab_attention_bwd_params* p, FaBwdParams& kp, cudaStream_t stre
       if ((rc = map(&kb, p->k, k_rows, kp.Hkv, p->k_stride_s, p->k_stride_h, p->k_stride_b, C::kBS))) return rc;
       if ((rc = map(&vb, p->v, k_rows, kp.Hkv, p->v_stride_s, p->v_stride_h, p->v_stride_b, C::kBS))) return rc;
     }
-    if (static_cast<int64_t>(kp.B) * (kp.Hq + (BwdElem<T>::kScaled ? kp.Hkv : 0)) > 65000) return kErrUnsupported;
   } else {
     // Nothing attends to anything: the items write zeros and read no map.
     qa = ga = ka = va = qb = gb = kb = vb = CUtensorMap{};
   }
-  const int64_t dkv_tiles = static_cast<int64_t>(kp.B) * kp.Hkv * kp.k_tiles * C::kDSplit;
-  const int64_t dq_tiles = static_cast<int64_t>(kp.B) * kp.Hq * kp.q_tiles;
-  const int64_t dkv = dkv_tiles * kp.dkv_slices, grid = dkv + dq_tiles * kp.dq_slices;
-  if (grid > 0x7fffffffLL) return kErrUnsupported;
+  const int64_t dkv = w.dkv_tiles * kp.dkv_slices, grid = dkv + w.dq_tiles * kp.dq_slices;
   kp.num_dkv = static_cast<int>(dkv);
   const bool stats = q_rows > 0 && k_rows > 0 && kp.M > 0;
   if (stats)
-    launch_stats<T, C::kBS>(kp, stream);
+    launch_stats<T, C::kBS>(kp, stat_ctas(p, w), stream);
   else if (packed)
     fa_bwd_zero_rest_kernel<T><<<dim3(8, 3), 256, 0, stream>>>(kp);
   if (grid > 0) {
@@ -260,29 +273,29 @@ int launch(const fab_attention_bwd_params* p, FaBwdParams& kp, cudaStream_t stre
     }
     if (kp.dkv_slices > 1)
       fa_bwd_join_kernel<T, kDP, true>
-          <<<dim3(static_cast<unsigned>(dkv_tiles), C::kOutDkv / 32), 256, 0, stream>>>(kp);
+          <<<dim3(static_cast<unsigned>(w.dkv_tiles), C::kOutDkv / 32), 256, 0, stream>>>(kp);
     if (kp.dq_slices > 1)
       fa_bwd_join_kernel<T, kDP, false>
-          <<<dim3(static_cast<unsigned>(dq_tiles), kDP / 64), 256, 0, stream>>>(kp);
+          <<<dim3(static_cast<unsigned>(w.dq_tiles), kDP / 64), 256, 0, stream>>>(kp);
   }
   return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
 }
 
 template <typename T, int kDP>
-int launch_parts(const fab_attention_bwd_params* p, FaBwdParams& kp, cudaStream_t stream) {
+int launch_parts(const fab_attention_bwd_params* p, const BwdPlan& w, FaBwdParams& kp, cudaStream_t stream) {
   const bool two = kp.few_rows || kp.cu_q != nullptr || std::min(kp.M, kp.N) <= kTwoPartLength;
-  return two ? launch<T, kDP, true>(p, kp, stream) : launch<T, kDP, false>(p, kp, stream);
+  return two ? launch<T, kDP, true>(p, w, kp, stream) : launch<T, kDP, false>(p, w, kp, stream);
 }
 
 template <typename T>
-int launch_dim(const fab_attention_bwd_params* p, FaBwdParams& kp, cudaStream_t stream) {
+int launch_dim(const fab_attention_bwd_params* p, const BwdPlan& w, FaBwdParams& kp, cudaStream_t stream) {
   switch (padded_head_dim(kp.D)) {
     case 64:
-      return launch_parts<T, 64>(p, kp, stream);
+      return launch_parts<T, 64>(p, w, kp, stream);
     case 128:
-      return launch_parts<T, 128>(p, kp, stream);
+      return launch_parts<T, 128>(p, w, kp, stream);
     default:
-      return launch_parts<T, 256>(p, kp, stream);
+      return launch_parts<T, 256>(p, w, kp, stream);
   }
 }
 
@@ -299,7 +312,9 @@ int fab_attention_bwd_workspace(const fab_attention_bwd_params* p, size_t* bytes
   bool empty = false;
   const int rc = validate(p, &empty);
   if (rc || empty) return rc;
-  *bytes = make_plan(p).bytes;
+  const BwdPlan w = make_plan(p);
+  if (!numbered(p, w)) return kErrUnsupported;
+  *bytes = w.bytes;
   return kOk;
 }
 
@@ -308,10 +323,10 @@ int fab_attention_bwd(const fab_attention_bwd_params* p, void* stream) {
   const int rc = validate(p, &empty);
   if (rc || empty) return rc;
   const BwdPlan w = make_plan(p);
+  if (!numbered(p, w)) return kErrUnsupported;
   if (w.bytes > 0 && (p->workspace == nullptr || (reinterpret_cast<uintptr_t>(p->workspace) & 255u) != 0 ||
                       p->workspace_bytes < w.bytes))
     return kErrWorkspace;
-  if (w.stat_tiles > 0x7fffffffLL) return kErrUnsupported;
   uint8_t* ws = static_cast<uint8_t*>(p->workspace);
   FaBwdParams kp{};
   kp.o = p->o;
@@ -342,6 +357,8 @@ int fab_attention_bwd(const fab_attention_bwd_params* p, void* stream) {
   kp.row_norm = reinterpret_cast<float*>(ws + w.row_norm);
   kp.tile_max = reinterpret_cast<float*>(ws + w.tile_max);
   kp.key_max = reinterpret_cast<float*>(ws + w.key_max);
+  kp.stat_q = static_cast<int>(w.stat_q);
+  kp.stat_k = static_cast<int>(w.stat_k);
   kp.key_tiles = static_cast<int>(w.key_tiles);
   kp.v = p->v;
   kp.v_sb = p->v_stride_b;
@@ -380,7 +397,7 @@ int fab_attention_bwd(const fab_attention_bwd_params* p, void* stream) {
   kp.dkv_part = reinterpret_cast<float*>(ws + w.dkv_part);
   kp.dq_part = reinterpret_cast<float*>(ws + w.dq_part);
   auto st = static_cast<cudaStream_t>(stream);
-  return p->dtype == kDtypeBF16 ? launch_dim<__nv_bfloat16>(p, kp, st) : launch_dim<__half>(p, kp, st);
+  return p->dtype == kDtypeBF16 ? launch_dim<__nv_bfloat16>(p, w, kp, st) : launch_dim<__half>(p, w, kp, st);
 }
 
 }  // extern "C"
