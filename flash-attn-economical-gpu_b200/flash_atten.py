@@ -536,6 +536,14 @@ def _empty_gradient(t: torch.Tensor) -> torch.Tensor:
     return g if g.stride(-1) == 1 else t.new_empty(t.shape)
 
 
+def _check_offsets(what: str, cu_q: torch.Tensor, cu_k: torch.Tensor, device: torch.device) -> None:
+    """Refuse cu_seqlens that the kernels could not read on `device`."""
+    for name, t in (("cu_seqlens_q", cu_q), ("cu_seqlens_k", cu_k)):
+        _require_cuda_tensor(name, t)
+        if t.device != device:
+            raise ValueError(f"{what}: {name} must be on {device} like q, got {t.device}")
+
+
 # fab_attention_bwd_params as one packed record: filling its fifty-odd fields one by one costs more than the launches
 # of a short call.
 _BWD_RECORD = struct.Struct("9P27q2P9ifiPN")
@@ -580,6 +588,10 @@ def _launch_attention_backward(what, dout, q, k, v, out, lse, causal, sm_scale, 
         raise ValueError(f"{what}: lse must be float32, one value per query row and head")
     if D < 1 or D > 256:
         raise ValueError(f"{what}: head_dim must be between 1 and 256, got {D}")
+    if workspace is not None:
+        _require_cuda_tensor("workspace", workspace)
+        if workspace.device != dev or not workspace.is_contiguous():
+            raise ValueError(f"{what}: workspace must be a contiguous tensor on {dev}")
     # Head dims off the 16-byte grid are written to padded rows first.
     padded = D % 8 != 0
     if padded:
@@ -604,7 +616,6 @@ def _launch_attention_backward(what, dout, q, k, v, out, lse, causal, sm_scale, 
             ws = torch.empty(need, device=dev, dtype=torch.uint8)
             have = need
         elif ws is not None:
-            _require_cuda_tensor("workspace", ws)
             have = ws.numel() * ws.element_size()
         strides = [s for t in ins for s in t.stride()[:3]] + list(lse.stride()) + [s for t in outs for s in t.stride()[:3]]
         p = _native.FabAttentionBwdParams.from_buffer_copy(_BWD_RECORD.pack(
@@ -634,8 +645,8 @@ def attention_backward(
     from q, k and lse.  float16 or bfloat16; grouped-query gradients are summed
     over each group's query heads in fp32 inside the kernel, and the same
     inputs give the same bits on every call.  `workspace` (CUDA, at least
-    attention_backward_workspace_bytes bytes, 256-byte aligned) must not be
-    used by another call until this one has completed; by default one is
+    attention_backward_workspace_bytes bytes, contiguous, 256-byte aligned) must
+    not be used by another call until this one has completed; by default one is
     allocated.  No counterpart in the reference (forward only).
     """
     for name, t in (("dout", dout), ("q", q), ("k", k), ("v", v), ("out", out)):
@@ -673,8 +684,7 @@ def attention_backward_varlen(
     for name, t in (("dout", dout), ("q", q), ("k", k), ("v", v), ("out", out)):
         if not isinstance(t, torch.Tensor) or t.ndim != 3:
             raise ValueError(f"{what} expects {name} with shape [total_tokens, heads, head_dim]")
-    for name, t in (("cu_seqlens_q", cu_seqlens_q), ("cu_seqlens_k", cu_seqlens_k)):
-        _require_cuda_tensor(name, t)
+    _check_offsets(what, cu_seqlens_q, cu_seqlens_k, q.device)
     if cu_seqlens_q.dtype != torch.int32 or cu_seqlens_k.dtype != torch.int32:
         raise ValueError(f"{what}: cu_seqlens_q / cu_seqlens_k must be int32")
     if cu_seqlens_q.ndim != 1 or cu_seqlens_q.shape != cu_seqlens_k.shape or cu_seqlens_q.numel() < 1:

@@ -16,6 +16,7 @@ import torch
 
 import _native
 from flash_atten import (
+    _check_offsets,
     _require_cuda_tensor,
     attention_backward,
     attention_backward_varlen,
@@ -300,6 +301,7 @@ def attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
                      sm_scale: float | None = None) -> torch.Tensor:
     """Differentiable flash_atten.attention_forward_varlen (float16 or bfloat16)."""
     _check_trainable("attention_varlen", q)
+    _check_offsets("attention_varlen", cu_seqlens_q, cu_seqlens_k, q.device)
     return _AttentionVarlen.apply(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, causal, sm_scale)
 
 
