@@ -76,6 +76,21 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_tiled_fn() {
   return fn;
 }
 
+// Encodes a map.  The driver call needs a current context, which a thread has
+// only after its first runtime call that does work on the device: autograd's
+// threads, say, can come here before that.  Such a call is made once more after
+// the runtime has made the device's context current.
+template <typename F>
+static int encode_map(F encode) {
+  CUresult r = encode();
+  if (r != CUDA_SUCCESS) {
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || cudaSetDevice(device) != cudaSuccess) return kErrCuda;
+    r = encode();
+  }
+  return r == CUDA_SUCCESS ? kOk : kErrInvalidArg;
+}
+
 static bool stride_ok(int64_t stride_bytes) {
   return stride_bytes > 0 && (stride_bytes % 16) == 0 && stride_bytes < (int64_t(1) << 40);
 }
@@ -97,9 +112,10 @@ int make_bhsd_map(CUtensorMap* map, const void* base, CUtensorMapDataType dt, in
   cuuint64_t strides[3] = {cuuint64_t(bs), cuuint64_t(bh), cuuint64_t(bb)};
   cuuint32_t box[4] = {cuuint32_t(box_inner), cuuint32_t(box_rows), 1, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
-  CUresult r = enc(map, dt, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? kOk : kErrInvalidArg;
+  return encode_map([&] {
+    return enc(map, dt, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  });
 }
 
 int make_2d_map(CUtensorMap* map, const void* base, CUtensorMapDataType dt, int elt, int cols, int rows, int64_t ld,
@@ -114,9 +130,10 @@ int make_2d_map(CUtensorMap* map, const void* base, CUtensorMapDataType dt, int 
   cuuint64_t strides[1] = {cuuint64_t(bs)};
   cuuint32_t box[2] = {cuuint32_t(box_inner), cuuint32_t(box_rows)};
   cuuint32_t estr[2] = {1, 1};
-  CUresult r = enc(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? kOk : kErrInvalidArg;
+  return encode_map([&] {
+    return enc(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  });
 }
 
 static int elt_size(int dtype) { return dtype == kDtypeF32 ? 4 : 2; }
