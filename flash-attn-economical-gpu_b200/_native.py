@@ -167,6 +167,7 @@ PROTOTYPES = {
     "fab_attention_fwd_plan": (_i32, [ctypes.POINTER(FabAttentionParams), _i32, ctypes.POINTER(FabFaPlan)]),
     "fab_debug_set_wait_limit_ns": (_i32, [ctypes.c_ulonglong]),
     "fab_debug_starve_kv_load": (_i32, [_i32]),
+    "fab_debug_starve_row_sums": (_i32, [_i32]),
     "fab_attention_fwd_splitkv_workspace": (
         _i32, [ctypes.POINTER(FabAttentionParams), _i32, ctypes.POINTER(ctypes.c_size_t), ctypes.POINTER(_i32)]),
     "fab_attention_fwd_splitkv": (_i32, [ctypes.POINTER(FabAttentionParams), _i32, _vp, ctypes.c_size_t, _vp]),
@@ -253,7 +254,7 @@ def device_error() -> int:
 DEVICE_WAITS = {1: "a Q tile's load", 2: "a K/V tile's load", 3: "an S product", 4: "a softmax's P",
                 5: "O's last product", 6: "a free K/V or stage slot", 7: "a GEMM accumulator",
                 8: "the drain at teardown", 9: "a peer rank's partial tile", 10: "a peer owner's reduced tile",
-                11: "a stream-K piece from another CTA pair", 12: "the CTA-pair GEMM's next tile from its scheduler",
+                11: "a stream-K piece from another CTA pair", 12: "the next tile from the cluster scheduler",
                 13: "the split-KV merge's copies", 14: "the layer norm's row sums"}
 
 
@@ -296,13 +297,19 @@ def fa_config_variant(dtype: int, head_dim: int, variant: int) -> FabFaConfig | 
 
 
 def set_wait_limit_ns(ns: int) -> None:
-    """Time limit of one bounded wait in the attention kernels of the current device (0: the 2 s default)."""
+    """Time limit of one bounded wait in the kernels of the current device (0: the default)."""
     check(lib.fab_debug_set_wait_limit_ns(int(ns)), "fab_debug_set_wait_limit_ns")
 
 
 def starve_kv_load(ring_tile: int) -> None:
-    """Test hook: every attention CTA skips K/V ring load `ring_tile` (-1: none), so its wait runs out."""
+    """Test hook: every attention CTA skips K/V ring load `ring_tile`, and in the backward awaits more of its streamed tiles
+    than comes (-1: neither), so the wait for it runs out."""
     check(lib.fab_debug_starve_kv_load(int(ring_tile)), "fab_debug_starve_kv_load")
+
+
+def starve_row_sums(row: int) -> None:
+    """Test hook: one CTA of a layer norm's clusters withholds its sums of `row` (-1: none), so the wait for them runs out."""
+    check(lib.fab_debug_starve_row_sums(int(row)), "fab_debug_starve_row_sums")
 
 
 def kernel_attrs(which: int, dtype: int, head_dim: int = 0) -> FabKernelAttrs:

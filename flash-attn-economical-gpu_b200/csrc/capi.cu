@@ -422,12 +422,21 @@ int fab_attention_fwd_plan(const fab_attention_params* p, int variant, fab_fa_pl
 
 int fab_debug_set_wait_limit_ns(unsigned long long ns) {
   const uint64_t v = ns == 0 ? kWaitLimitNs : static_cast<uint64_t>(ns);
-  return cudaMemcpyToSymbol(g_fab_wait_limit_ns, &v, sizeof(v)) == cudaSuccess ? kOk : kErrCuda;
+  if (cudaMemcpyToSymbol(g_fab_wait_limit_ns, &v, sizeof(v)) != cudaSuccess) return kErrCuda;
+  fa_bwd_set_wait_limit(ns);
+  if (int rc = gemm_set_wait_limit(v)) return rc;
+  return train_ops_set_wait_limit(v);
 }
 
 int fab_debug_starve_kv_load(int ring_tile) {
   const int v = ring_tile < 0 ? -1 : ring_tile;
+  fa_bwd_starve_loads(v >= 0);
   return cudaMemcpyToSymbol(g_fab_starve_kv_load, &v, sizeof(v)) == cudaSuccess ? kOk : kErrCuda;
+}
+
+int fab_debug_starve_row_sums(int row) {
+  train_ops_starve_row_sums(row < 0 ? -1 : row);
+  return kOk;
 }
 
 int fab_flash_attn_config_variant(int dtype, int head_dim, int variant, fab_fa_config* out) {

@@ -5,6 +5,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 
@@ -24,6 +25,13 @@ int fa_bwd_take_device_error(int* code) {
   *code = v;
   return kOk;
 }
+
+// Read by every later launch.
+static std::atomic<int> g_spared_tries{0}, g_starve_bytes{0};
+void fa_bwd_set_wait_limit(uint64_t ns) {
+  g_spared_tries = ns == 0 || ns / 1000 >= kWaitTries ? 0 : kWaitTries - std::max(static_cast<int>(ns / 1000), 1);
+}
+void fa_bwd_starve_loads(bool starve) { g_starve_bytes = starve ? 16 : 0; }
 
 namespace {
 
@@ -386,6 +394,8 @@ int fab_attention_bwd(const fab_attention_bwd_params* p, void* stream) {
     kp.M = kp.M < kp.total_q ? kp.M : kp.total_q;
     kp.N = kp.N < kp.total_k ? kp.N : kp.total_k;
   }
+  kp.spared_tries = g_spared_tries;
+  kp.starve_bytes = g_starve_bytes;
   kp.q_tiles = w.q_tiles;
   kp.k_tiles = w.k_tiles;
   kp.dkv_slice_len = w.dkv_slice_len;

@@ -136,7 +136,7 @@ struct BwdCfg {
   // S, P x 2, dP, dS x 2; issue order x 2; accumulators final x 2 and read; ragged tile x 2; next item
   // full/empty x 2; its request; teardown x 2.
   static constexpr int kNumBars = 2 * (kRing0 + kRing1) + 4 + 4 + 6 + 3 + 2 + 4 + 3 + 2;
-  static constexpr int kTailBytes = 304;  // TMEM address, abort flag, a zero word, two items, the scheduler's response
+  static constexpr int kTailBytes = 304;  // TMEM address, two abort flags with a word each, two items, the scheduler's response
   static constexpr int kSmemBytes =
       2 * kABytes + (kRing0 + kRing1) * kBBytes + 2 * kStatBytes + kNumBars * 8 + kTailBytes;
   // P and dS are handed to the tensor core in two halves where a warp works
@@ -384,21 +384,22 @@ __device__ __forceinline__ void bwd_store_chunk(int64_t row, int64_t stride, int
 // hold some sixty waits, and with the general one (ptx.cuh) inlined at each
 // they outgrew the instruction cache.  Each try suspends for a microsecond at
 // most; after kWaitTries, or once another warp of the CTA has given up, the
-// warp leaves its code in the abort flag and unwinds.
-constexpr uint32_t kWaitTries = 4000000;
+// warp leaves its code in the abort flag and unwinds.  The word after the flag,
+// read with it, is the number of tries not to make: 0 but in tests.
+constexpr int kWaitTries = 4000000;
 __device__ __forceinline__ bool bwd_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int code) {
   // Usually complete already: one test, no loop.
   if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
   uint32_t ok;
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\t.reg .u32 n, a;\n\t"
+      "{\n\t.reg .pred p, q;\n\t.reg .u32 n, a, m;\n\t"
       "mov.u32 n, %4;\n\t"
       "WAIT:\n\t"
       "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\t"
       "@p bra DONE;\n\t"
-      "ld.volatile.shared.u32 a, [%3];\n\t"
+      "ld.volatile.shared.v2.u32 {a, m}, [%3];\n\t"
       "sub.u32 n, n, 1;\n\t"
-      "setp.eq.u32 q, n, 0;\n\t"
+      "setp.le.u32 q, n, m;\n\t"
       "setp.ne.or.u32 q, a, 0, q;\n\t"
       "@!q bra WAIT;\n\t"
       "DONE:\n\t"
@@ -598,8 +599,8 @@ struct BwdCta {
     clc = sched_empty + 2;
     drained = clc + 1;
     tmem_slot = reinterpret_cast<uint32_t*>(drained + 2);
-    abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    clc_resp = (smem_u32(tmem_slot + 3) + 15u) & ~15u;
+    abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 2);
+    clc_resp = (smem_u32(tmem_slot + 6) + 15u) & ~15u;  // 16 bytes
     item = reinterpret_cast<BwdItem*>(tmem_slot + 12);
     static_assert(48 + 2 * sizeof(BwdItem) <= C::kTailBytes, "two items in the tail");
   }
@@ -681,7 +682,7 @@ __device__ __forceinline__ bool bwd_produce(const FaBwdParams& p, const BwdCta<k
     const bool fix = ti == ragged;
     if (lane == 0) {
       uint64_t* bar = fix ? c.fix + role : landed;
-      mbar_arrive_expect_tx(bar, C::kBBytes);
+      mbar_arrive_expect_tx(bar, C::kBBytes + p.starve_bytes);
 #pragma unroll
       for (int a = 0; a < C::kAtoms; ++a)
         tma_load_4d(dst + a * C::kBAtomBytes, map_s, bar, a * 64, row_first + ti * kBS, head, map_b);
@@ -1142,7 +1143,8 @@ __global__ void __launch_bounds__(384, 1)
     mbar_init(c.acc_free, 8);
     mbar_init(c.clc, 1);
     *c.abort_flag = *reinterpret_cast<volatile int*>(&g_fab_device_error) != 0 ? -1 : 0;
-    c.abort_flag[1] = 0;
+    c.abort_flag[2] = 0;
+    c.abort_flag[1] = c.abort_flag[3] = p.spared_tries;
     // The swizzled tiles need the base that the alignment above asks for.
     if (smem_u32(smem_raw) & 1023u) {
       record_device_error(kDevTimeoutTeardown);
@@ -1183,9 +1185,9 @@ __global__ void __launch_bounds__(384, 1)
           mbar_arrive_expect_tx(c.clc, 16);
           clc_try_cancel(c.clc_resp, c.clc);
         }
-        // The answer must have landed before this CTA may leave: the word
-        // after the abort flag stays zero, so only the tries bound this wait.
-        const bool ok = bwd_wait(c.clc, answer.phase, c.abort_flag + 1, kDevTimeoutSched);
+        // The answer must have landed before this CTA may leave: the second
+        // abort flag stays zero till then, so only the tries bound this wait.
+        const bool ok = bwd_wait(c.clc, answer.phase, c.abort_flag + 2, kDevTimeoutSched);
         answer.next(1);
         return ok ? clc_first_cta_x(c.clc_resp) : -1;
       };
@@ -1224,7 +1226,7 @@ __global__ void __launch_bounds__(384, 1)
       }
       // No copy may still be landing when a producer leaves: the last one
       // into every buffer, whether or not its tile was handed on.
-      if (n.any) bwd_wait(c.a_full + role, n.a.phase ^ 1, c.abort_flag + 1, kDevTimeoutTeardown);
+      if (n.any) bwd_wait(c.a_full + role, n.a.phase ^ 1, c.abort_flag + 2, kDevTimeoutTeardown);
       uint64_t* const full = role == 0 ? c.full0 : c.full1;
       const int size = role == 0 ? C::kRing0 : C::kRing1;
       BwdPos last = n.ring;  // the oldest of the last `size` loads, if there were as many
@@ -1232,7 +1234,7 @@ __global__ void __launch_bounds__(384, 1)
       else last.phase ^= 1;
 #pragma unroll 1
       for (int x = min(n.tiles, size); x > 0; --x) {
-        bwd_wait(full + last.slot, last.phase, c.abort_flag + 1, kDevTimeoutTeardown);
+        bwd_wait(full + last.slot, last.phase, c.abort_flag + 2, kDevTimeoutTeardown);
         last.next(size);
       }
       BwdPos stat = n.stat;
@@ -1240,7 +1242,7 @@ __global__ void __launch_bounds__(384, 1)
       else stat.phase ^= 1;
 #pragma unroll 1
       for (int x = min(n.stats, 2); x > 0; --x) {
-        bwd_wait(c.st_full + stat.slot, stat.phase, c.abort_flag + 1, kDevTimeoutTeardown);
+        bwd_wait(c.st_full + stat.slot, stat.phase, c.abort_flag + 2, kDevTimeoutTeardown);
         stat.next(2);
       }
     } else if (!skip) {
@@ -1255,7 +1257,7 @@ __global__ void __launch_bounds__(384, 1)
       }
       // Drain the tensor pipe before TMEM is released.
       if (leader) mma_commit(c.drained + role);
-      bwd_wait(c.drained + role, 0, c.abort_flag + 1, kDevTimeoutTeardown);
+      bwd_wait(c.drained + role, 0, c.abort_flag + 2, kDevTimeoutTeardown);
     }
   } else {
     setmaxnreg_inc<C::kSoftmaxRegs>();
@@ -1274,7 +1276,7 @@ __global__ void __launch_bounds__(384, 1)
   // A warp that gave up left its code.
   __syncthreads();
   if (threadIdx.x == 0 && c.abort_flag[0] > 0) record_device_error(c.abort_flag[0]);
-  if (threadIdx.x == 0 && c.abort_flag[1] > 0) record_device_error(c.abort_flag[1]);
+  if (threadIdx.x == 0 && c.abort_flag[2] > 0) record_device_error(c.abort_flag[2]);
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {

@@ -137,6 +137,8 @@ struct FaBwdParams {
   const int* cu_k;
   int total_q;
   int total_k;
+  int spared_tries;  // of kWaitTries, for tests that make a wait run out: the ones not to make
+  int starve_bytes;  // and what a streamed tile's barrier awaits beyond the tile
 };
 
 // Plan of a split-KV launch: the tile config it runs and the workspace it needs.
@@ -276,6 +278,15 @@ int gemm_take_device_error(int* code);
 int fa_bwd_take_device_error(int* code);
 // And for the training operators' unit.
 int train_ops_take_device_error(int* code);
+
+// Test hooks of the other units' bounded waits, behind fab_debug_*: the limit
+// of one wait (0 the default), and what is withheld so that one runs out:
+// part of every streamed tile, a row's sums (-1 none).
+int gemm_set_wait_limit(uint64_t ns);
+int train_ops_set_wait_limit(uint64_t ns);
+void fa_bwd_set_wait_limit(uint64_t ns);
+void fa_bwd_starve_loads(bool starve);
+void train_ops_starve_row_sums(int row);
 
 // Helpers implemented in capi.cu.
 int ensure_smem_attr(const void* kernel, int bytes);

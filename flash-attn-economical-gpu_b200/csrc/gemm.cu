@@ -4,7 +4,7 @@
 // one unit with them, the CTA-pair kernel's instantiation changed the
 // attention kernels' register allocation (a small spill; measured on B200,
 // 2.5 % of attention throughput).  Each unit has its own copy of the device
-// status word; fab_get_device_error reads both.
+// status word; fab_get_device_error reads them all.
 #include <cudaTypedefs.h>
 
 #include <cstdint>
@@ -25,6 +25,10 @@ int gemm_take_device_error(int* code) {
   }
   *code = v;
   return kOk;
+}
+
+int gemm_set_wait_limit(uint64_t ns) {
+  return cudaMemcpyToSymbol(g_fab_wait_limit_ns, &ns, sizeof(ns)) == cudaSuccess ? kOk : kErrCuda;
 }
 
 }  // namespace fab

@@ -33,15 +33,15 @@ enum DeviceError : int {
 };
 
 // Device-global status word of the kernels of one translation unit (internal
-// linkage: capi.cu and gemm.cu each have one; fab_get_device_error reads
-// both).  A kernel that starts after a failed wait of its unit skips its work.
+// linkage: each unit has one; fab_get_device_error reads them all).  A kernel that starts after a failed wait of its unit skips its work.
 static __device__ int g_fab_device_error = 0;
 
 // A single wait may take at most this long before the kernel gives up.
 constexpr uint64_t kWaitLimitNs = 2000000000ull;  // 2 s
 
 // The limit the waits of this unit apply: kWaitLimitNs unless a test has set
-// a shorter one through fab_debug_set_wait_limit_ns (attention unit only).
+// a shorter one through fab_debug_set_wait_limit_ns.  (The attention backward
+// counts tries instead.)
 static __device__ uint64_t g_fab_wait_limit_ns = kWaitLimitNs;
 
 __device__ __forceinline__ uint64_t globaltimer_ns() {

@@ -2,6 +2,7 @@
 // norm and multi-axis rotary embedding (train_ops.cuh), with their C entry
 // points.  The unit has its own copy of the device status word.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 
@@ -21,6 +22,14 @@ int train_ops_take_device_error(int* code) {
   *code = v;
   return kOk;
 }
+
+int train_ops_set_wait_limit(uint64_t ns) {
+  return cudaMemcpyToSymbol(g_fab_wait_limit_ns, &ns, sizeof(ns)) == cudaSuccess ? kOk : kErrCuda;
+}
+
+// Read by every later launch.
+static std::atomic<int> g_starve_row{-1};
+void train_ops_starve_row_sums(int row) { g_starve_row = row; }
 
 namespace {
 
@@ -316,7 +325,7 @@ int fab_layernorm(const void* x, const void* residual, const void* w, const void
   if (!aligned(x, e) || !aligned(residual, e) || !aligned(y, e) || !aligned(x_out, e) || !aligned(w, we) ||
       !aligned(bias, we) || !aligned(mean, 4) || !aligned(rstd, 4))
     return kErrInvalidArg;
-  LayerNormParams p{x, residual, w, bias, y, x_out, mean, rstd, ld_x, ld_res, ld_y, ld_xo, rows, cols, eps, 0};
+  LayerNormParams p{x, residual, w, bias, y, x_out, mean, rstd, ld_x, ld_res, ld_y, ld_xo, rows, cols, eps, 0, g_starve_row};
   auto st = static_cast<cudaStream_t>(stream);
   return by_types(dtype, w_dtype, [&](auto t, auto wt) { return fwd<decltype(t), decltype(wt)>(p, st); });
 }
@@ -350,7 +359,7 @@ int fab_layernorm_bwd(const void* dy, const void* x, const void* w, const float*
                workspace_bytes < size_t(max_lines(rows, cols)) * 2 * size_t(cols) * sizeof(float)))
     return kErrWorkspace;
   LayerNormBwdParams p{dy, x, w, mean, rstd, dresidual, dx, sums ? static_cast<float*>(workspace) : nullptr,
-                       ld_dy, ld_x, ld_dres, ld_dx, rows, cols, 0};
+                       ld_dy, ld_x, ld_dres, ld_dx, rows, cols, 0, g_starve_row};
   return by_types(dtype, w_dtype,
                   [&](auto t, auto wt) { return bwd<decltype(t), decltype(wt)>(p, dw, db, st); });
 }

@@ -250,14 +250,15 @@ __device__ __forceinline__ void init_sums(float (&red)[2][kFloats], RowBars& bar
     __syncthreads();
   }
 }
-// K sums over the cluster; false when a peer's never came.
+// K sums over the cluster; false when a peer's never came.  `withheld`: this
+// CTA sends none.
 template <int K>
 __device__ __forceinline__ bool cluster_sum(float (&v)[K], float* red, uint64_t* bar, uint32_t parity, RowBars& bars,
-                                            const RowShare& r) {
+                                            const RowShare& r, bool withheld) {
   const int lane = threadIdx.x & 31;
   warp_sum<K>(v);
   if (threadIdx.x == 0) mbar_arrive_expect_tx(bar, K * 4 * (blockDim.x >> 5) * r.ctas);
-  if (lane < r.ctas) {
+  if (lane < r.ctas && !withheld) {
 #pragma unroll
     for (int k = 0; k < K; ++k)
       asm volatile(
@@ -343,6 +344,7 @@ struct LayerNormParams {
   int cols;
   float eps;
   int span;  // columns of a CTA where a cluster shares a row
+  int starve_row;  // test hook: the row whose sums the cluster's last CTA withholds, or -1
 };
 
 // y = (x' - mean) * rsqrt(var + eps) * w + b per row, x' = x or round(x + residual).
@@ -466,6 +468,7 @@ __global__ void __launch_bounds__(kMaxThreads, kMinCtas) layernorm_fwd_stream_ke
   const int c0 = threadIdx.x * V, step = threads * V;  // first column, columns between vectors
   init_sums<kWide>(red, bars);
   [[maybe_unused]] uint32_t parity = 0;
+  [[maybe_unused]] const int starve_row = share.rank == share.ctas - 1 ? p.starve_row : -1;
   float2 w[NV][N], b[NV][N];
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
@@ -553,7 +556,7 @@ __global__ void __launch_bounds__(kMaxThreads, kMinCtas) layernorm_fwd_stream_ke
     if ((from += stage_size) == end) from = mine;
     float sum[1] = {sum2.x + sum2.y};
     if constexpr (kWide) {
-      if (!cluster_sum<1>(sum, red[0], bars.bar, parity, bars, share)) break;
+      if (!cluster_sum<1>(sum, red[0], bars.bar, parity, bars, share, row == starve_row)) break;
     } else {
       few_warps_sum<1>(sum, red[0]);
     }
@@ -571,7 +574,7 @@ __global__ void __launch_bounds__(kMaxThreads, kMinCtas) layernorm_fwd_stream_ke
     float sq[1] = {sq2.x + sq2.y};
     // Each of the two sums also frees the other's buffer.
     if constexpr (kWide) {
-      if (!cluster_sum<1>(sq, red[1], bars.bar + 1, parity, bars, share)) break;
+      if (!cluster_sum<1>(sq, red[1], bars.bar + 1, parity, bars, share, false)) break;
       parity ^= 1u;
     } else {
       few_warps_sum<1>(sq, red[1]);
@@ -651,6 +654,7 @@ struct LayerNormBwdParams {
   int64_t rows;
   int cols;
   int span;  // columns of a CTA where a cluster shares a row
+  int starve_row;  // test hook: the row whose sums the cluster's last CTA withholds, or -1
 };
 
 // With xhat = (x - mean) * rstd and g = dy * w:
@@ -691,6 +695,7 @@ __global__ void __launch_bounds__(kMaxThreads, kMinCtas) layernorm_bwd_kernel(co
   const bool summed = p.dres != nullptr;
   init_sums<kWide>(red, bars);
   [[maybe_unused]] uint32_t parity = 0;
+  [[maybe_unused]] const int starve_row = share.rank == share.ctas - 1 ? p.starve_row : -1;
   float2 w[NV][N], dw[NV][N], db[NV][N];
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
@@ -798,7 +803,7 @@ __global__ void __launch_bounds__(kMaxThreads, kMinCtas) layernorm_bwd_kernel(co
     if constexpr (kWarpRow) {
       warp_sum<2>(s);
     } else if constexpr (kWide) {
-      if (!cluster_sum<2>(s, red[turn], bars.bar + turn, parity, bars, share)) break;
+      if (!cluster_sum<2>(s, red[turn], bars.bar + turn, parity, bars, share, row == starve_row)) break;
       parity ^= static_cast<uint32_t>(turn);
     } else {
       few_warps_sum<2>(s, red[turn]);  // the other buffer is free again: every thread has passed this row's barrier

@@ -617,25 +617,32 @@ int fab_device_limits_query(int device, fab_device_limits* out);
  *    4 a softmax's P              5 O's last product        6 a free K/V or stage slot
  *    7 a GEMM accumulator         8 the drain at teardown   9 a peer rank's partial tile
  *   10 a peer owner's reduced tile                          11 a stream-K piece from another pair
- *   12 the CTA-pair GEMM's next tile from its scheduler     13 the split-KV merge's copies
+ *   12 the next tile from the cluster scheduler (CTA-pair GEMM, attention backward)
+ *   13 the split-KV merge's copies                          14 a row's sums from another CTA (layer norm)
  * Synchronises with the device (call it between launches).
  */
 int fab_get_device_error(int* code);
 
 /*
- * Test hooks for the bounded waits of the attention kernels (no counterpart
- * in the reference, which has no device-side waits).  They change device
- * state of the current device and synchronise with it; call them only
- * between launches.
+ * Test hooks for the bounded waits of the kernels (no counterpart in the
+ * reference, which has no device-side waits).  They change state of the
+ * current device and of the process and synchronise with the device; call
+ * them only between launches.
  * fab_debug_set_wait_limit_ns: the time one wait may take before the kernel
  *   records its code in the device error word and unwinds (0 restores the
- *   default of 2 s).
+ *   default of 2 s; the attention backward counts tries of a microsecond at
+ *   most, 4 million by default).
  * fab_debug_starve_kv_load: the producer of every attention CTA skips the
  *   K/V ring load with this index (ring order: K_0, V_0, K_1, V_1, ... with
- *   one S buffer), so the wait for it runs out; -1 restores normal loading.
+ *   one S buffer), and the barriers of the attention backward's streamed tiles
+ *   await 16 bytes more than a tile has, so the wait for it runs out; -1
+ *   restores normal loading.
+ * fab_debug_starve_row_sums: where a cluster of CTAs shares a layer norm's
+ *   rows, its last one withholds its sums of this row; -1 restores sending.
  */
 int fab_debug_set_wait_limit_ns(unsigned long long ns);
 int fab_debug_starve_kv_load(int ring_tile);
+int fab_debug_starve_row_sums(int row);
 
 /* Human-readable text for a FAB_* return code. */
 const char* fab_error_string(int rc);
