@@ -54,7 +54,6 @@ struct BwdPlan {
   int64_t part_k_tiles, part_q_tiles;
   int64_t key_tiles;
   int64_t dkv_tiles, dq_tiles;  // stationary tiles of all heads, a half-head's each where a tile takes two items
-  int64_t stat_q, stat_k;       // tiles of the longest sequence that the statistics kernel visits
   size_t row_norm, tile_max, key_max, dkv_part, dq_part, bytes;
 };
 
@@ -124,8 +123,6 @@ BwdPlan make_plan(const fab_attention_bwd_params* p) {
   if (p->dtype == kDtypeF16) at += round256(size_t(w.key_tiles) * per_kv * sizeof(float));
   w.dkv_tiles = int64_t(p->batch) * p->heads_kv * w.k_tiles * dsplit;
   w.dq_tiles = int64_t(p->batch) * p->heads_q * w.q_tiles;
-  w.stat_q = ceil_div(M, bs);
-  w.stat_k = ceil_div(N, bs);
   const int dp = padded_head_dim(p->head_dim);
   w.dkv_part = at;
   if (w.dkv_slices > 1) at += size_t(w.part_k_tiles) * per_kv * w.dkv_slices * 2 * dp * 128 * sizeof(float);
@@ -135,16 +132,13 @@ BwdPlan make_plan(const fab_attention_bwd_params* p) {
   return w;
 }
 
-// CTAs of the statistics kernel, and whether it, the items and the statistics'
-// lines can be numbered in 31 bits.
-int64_t stat_ctas(const fab_attention_bwd_params* p, const BwdPlan& w) {
-  return int64_t(p->batch) * (w.stat_q * p->heads_q + (p->dtype == kDtypeF16 ? w.stat_k * p->heads_kv : 0)) +
-         (p->cu_seqlens_q != nullptr ? 3 * std::max(w.stat_q, w.stat_k) : 0);
-}
+// Can the items, the heads of both kinds and the tiles of one head be numbered
+// in 31 bits?
 bool numbered(const fab_attention_bwd_params* p, const BwdPlan& w) {
   constexpr double kMost = 0x7fffffff;
-  return double(w.dkv_tiles) * w.dkv_slices + double(w.dq_tiles) * w.dq_slices <= kMost && stat_ctas(p, w) <= kMost &&
-         w.stat_tiles <= kMost && w.key_tiles <= kMost && w.part_q_tiles <= kMost && w.part_k_tiles <= kMost;
+  return double(w.dkv_tiles) * w.dkv_slices + double(w.dq_tiles) * w.dq_slices <= kMost &&
+         double(p->batch) * (double(p->heads_q) + p->heads_kv) + 65538 <= kMost && w.stat_tiles <= kMost &&
+         w.key_tiles <= kMost && w.part_q_tiles <= kMost && w.part_k_tiles <= kMost;
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -202,8 +196,12 @@ int validate(const fab_attention_bwd_params* p, bool* empty) {
 }
 
 template <typename T, int kBS>
-void launch_stats(const FaBwdParams& kp, int64_t ctas, cudaStream_t stream) {
-  const unsigned grid = static_cast<unsigned>(ctas);
+void launch_stats(const FaBwdParams& kp, cudaStream_t stream) {
+  constexpr bool kKeys = BwdElem<T>::kScaled;
+  const int64_t rows = int64_t(kp.B) * (kp.Hq + (kKeys ? kp.Hkv : 0)) + (kp.cu_q != nullptr ? 3 : 0);
+  const int64_t y = std::min<int64_t>(rows, 65535);
+  const dim3 grid(static_cast<unsigned>(ceil_div(kKeys ? std::max(kp.M, kp.N) : kp.M, kBS)), static_cast<unsigned>(y),
+                  static_cast<unsigned>(ceil_div(rows, y)));
   // Lanes per row: eight columns each.
   if constexpr (kBS == 64) {
     fa_bwd_stats_kernel<T, 64, 32><<<grid, kStatThreads, 0, stream>>>(kp);
@@ -260,7 +258,7 @@ int launch(const fab_attention_bwd_params* p, const BwdPlan& w, FaBwdParams& kp,
   kp.num_dkv = static_cast<int>(dkv);
   const bool stats = q_rows > 0 && k_rows > 0 && kp.M > 0;
   if (stats)
-    launch_stats<T, C::kBS>(kp, stat_ctas(p, w), stream);
+    launch_stats<T, C::kBS>(kp, stream);
   else if (packed)
     fa_bwd_zero_rest_kernel<T><<<dim3(8, 3), 256, 0, stream>>>(kp);
   if (grid > 0) {
@@ -365,8 +363,6 @@ int fab_attention_bwd(const fab_attention_bwd_params* p, void* stream) {
   kp.row_norm = reinterpret_cast<float*>(ws + w.row_norm);
   kp.tile_max = reinterpret_cast<float*>(ws + w.tile_max);
   kp.key_max = reinterpret_cast<float*>(ws + w.key_max);
-  kp.stat_q = static_cast<int>(w.stat_q);
-  kp.stat_k = static_cast<int>(w.stat_k);
   kp.key_tiles = static_cast<int>(w.key_tiles);
   kp.v = p->v;
   kp.v_sb = p->v_stride_b;

@@ -187,10 +187,9 @@ __device__ __forceinline__ void bwd_seq(const int* cu, int b, int total, int lon
 }
 
 // Rows of a packed tensor that belong to no sequence (before cu[0], after
-// cu[B]) get zero gradients.  which: 0 dq, 1 dk, 2 dv; this is CTA `cta` of
-// `ctas` that clear them.
+// cu[B]) get zero gradients, from CTAs along x.  which: 0 dq, 1 dk, 2 dv.
 template <typename T>
-__device__ __forceinline__ void bwd_zero_rest(const FaBwdParams& p, int which, int cta, int ctas) {
+__device__ __forceinline__ void bwd_zero_rest(const FaBwdParams& p, int which) {
   const bool is_q = which == 0;
   const int* cu = is_q ? p.cu_q : p.cu_k;
   const int total = is_q ? p.total_q : p.total_k, heads = is_q ? p.Hq : p.Hkv;
@@ -200,7 +199,7 @@ __device__ __forceinline__ void bwd_zero_rest(const FaBwdParams& p, int which, i
   const int64_t ss = is_q ? p.dq_ss : which == 1 ? p.dk_ss : p.dv_ss;
   const int64_t sh = is_q ? p.dq_sh : which == 1 ? p.dk_sh : p.dv_sh;
   const int rest = head + total - tail;
-  for (int64_t i = cta * int64_t(blockDim.x) + threadIdx.x; i < static_cast<int64_t>(rest) * heads * p.D; i += ctas * int64_t(blockDim.x)) {
+  for (int64_t i = blockIdx.x * int64_t(blockDim.x) + threadIdx.x; i < static_cast<int64_t>(rest) * heads * p.D; i += gridDim.x * int64_t(blockDim.x)) {
     const int d = static_cast<int>(i % p.D);
     const int h = static_cast<int>(i / p.D % heads);
     int row = static_cast<int>(i / p.D / heads);
@@ -211,7 +210,7 @@ __device__ __forceinline__ void bwd_zero_rest(const FaBwdParams& p, int which, i
 
 template <typename T>
 __global__ void __launch_bounds__(256) fa_bwd_zero_rest_kernel(const FaBwdParams p) {
-  bwd_zero_rest<T>(p, blockIdx.y, blockIdx.x, gridDim.x);
+  bwd_zero_rest<T>(p, blockIdx.y);
 }
 
 // Per query row: -lse * log2(e), plus kPExp, (-inf for rows that saw no key and for the
@@ -227,27 +226,24 @@ template <typename T, int kBS, int kLanes>
 __global__ void __launch_bounds__(kStatThreads, 2) fa_bwd_stats_kernel(const FaBwdParams p) {
   // The main kernel may be set up meanwhile; it waits before it reads.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  // One row of CTAs: the tiles of every (batch entry, query head), for fp16 of
-  // every key/value head, and for packed batches those that clear the rest.
-  // (As a grid of (tile, head) it could not hold more than 65535 heads.)
-  int index = blockIdx.x;
-  const int q_ctas = p.stat_q * p.B * p.Hq, k_ctas = BwdElem<T>::kScaled ? p.stat_k * p.B * p.Hkv : 0;
-  if (index >= q_ctas + k_ctas) {
-    index -= q_ctas + k_ctas;
-    bwd_zero_rest<T>(p, index % 3, index / 3, max(p.stat_q, p.stat_k));
+  // Rows of CTAs, in y and past its 65535 in z: query heads, for fp16
+  // key/value heads, and three more for packed batches.
+  int bh = blockIdx.z * gridDim.y + blockIdx.y;
+  const int q_heads = p.B * p.Hq, all_heads = q_heads + (BwdElem<T>::kScaled ? p.B * p.Hkv : 0);
+  if (bh >= all_heads) {
+    if (p.cu_q != nullptr && bh < all_heads + 3) bwd_zero_rest<T>(p, bh - all_heads);
     return;
   }
-  const bool keys = index >= q_ctas;
-  if (keys) index -= q_ctas;
-  const int tiles = keys ? p.stat_k : p.stat_q, heads = keys ? p.Hkv : p.Hq;
-  const int bh = index / tiles, own_tile = index - bh * tiles;
-  const int b = bh / heads, h = bh - b * heads;
+  const bool keys = BwdElem<T>::kScaled && bh >= q_heads;
+  if (keys) bh -= q_heads;
+  const int heads = keys ? p.Hkv : p.Hq;
+  const int b = bh / heads, h = bh % heads;
   int q0, M;
   if (keys)
     bwd_seq(p.cu_k, b, p.total_k, p.N, q0, M);
   else
     bwd_seq(p.cu_q, b, p.total_q, p.M, q0, M);
-  const int m0 = own_tile * kBS;
+  const int m0 = blockIdx.x * kBS;
   if (m0 >= M) return;
   // For keys both operands are V.
   const int64_t o_ss = keys ? p.v_ss : p.o_ss, g_ss = keys ? p.v_ss : p.g_ss;
@@ -255,7 +251,7 @@ __global__ void __launch_bounds__(kStatThreads, 2) fa_bwd_stats_kernel(const FaB
   const T* o = keys ? v : reinterpret_cast<const T*>(p.o) + (p.cu_q ? q0 * p.o_ss : b * p.o_sb) + h * p.o_sh;
   const T* g = keys ? v : reinterpret_cast<const T*>(p.dout) + (p.cu_q ? q0 * p.g_ss : b * p.g_sb) + h * p.g_sh;
   const float* lse = p.lse + (p.cu_q ? q0 * p.l_ss : b * p.l_sb) + h * p.l_sh;
-  const int64_t tile = (keys ? bwd_key_tile0(p, b, h, q0, kBS) : bwd_stat_tile0(p, b, h, q0, kBS)) + own_tile;
+  const int64_t tile = (keys ? bwd_key_tile0(p, b, h, q0, kBS) : bwd_stat_tile0(p, b, h, q0, kBS)) + blockIdx.x;
   float* st = p.stats + tile * (2 * kBS);
   constexpr int kRows = kStatThreads / kLanes;  // rows of one pass over the CTA
   const int sub = threadIdx.x % kLanes, r0 = threadIdx.x / kLanes;

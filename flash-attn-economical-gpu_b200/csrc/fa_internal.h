@@ -115,7 +115,6 @@ struct FaBwdParams {
   float* row_norm;
   float* tile_max;
   float* key_max;
-  int stat_q, stat_k;  // tiles of the longest sequence that the statistics kernel visits: queries', keys' (fp16)
   int key_tiles;   // of one head, numbered like stat_tiles
   int stat_tiles;  // tiles of one head (dense: of one batch entry's head)
   int B, Hq, Hkv, M, N, D;  // M, N: longest lengths of a packed batch

@@ -530,12 +530,6 @@ def _conform_operand(t: torch.Tensor) -> torch.Tensor:
     return _conform(t)
 
 
-def _empty_gradient(t: torch.Tensor) -> torch.Tensor:
-    """Uninitialised gradient of `t`, in its layout where that has unit stride along head_dim, else contiguous."""
-    g = torch.empty_like(t)
-    return g if g.stride(-1) == 1 else t.new_empty(t.shape)
-
-
 def _check_offsets(what: str, cu_q: torch.Tensor, cu_k: torch.Tensor, device: torch.device) -> None:
     """Refuse cu_seqlens that the kernels could not read on `device`."""
     for name, t in (("cu_seqlens_q", cu_q), ("cu_seqlens_k", cu_k)):
@@ -597,10 +591,15 @@ def _launch_attention_backward(what, dout, q, k, v, out, lse, causal, sm_scale, 
     if padded:
         outs = tuple(_padded_like(t) for t in (q, k, v))
     else:
-        outs = _empty_gradient(q), _empty_gradient(k), _empty_gradient(v)
+        outs = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
     if B == 0 or (M == 0 and N == 0):
         return tuple(t.contiguous() for t in outs) if padded else outs
     ins = [_conform_operand(t) if t.numel() else t for t in (q, k, v, out, dout)]
+    sq, sk, sv = [t.stride() for t in outs]
+    if not sq[3] == sk[3] == sv[3] == 1:
+        # An operand without head_dim innermost has a contiguous gradient.
+        outs = tuple(t if t.stride(3) == 1 else t.new_empty(t.shape) for t in outs)
+        sq, sk, sv = [t.stride() for t in outs]
     code = _native.FAB_DTYPE_BF16 if dtype is torch.bfloat16 else _native.FAB_DTYPE_F16
     causal = 1 if causal else 0
     if cu_q is None:
@@ -617,9 +616,10 @@ def _launch_attention_backward(what, dout, q, k, v, out, lse, causal, sm_scale, 
             have = need
         elif ws is not None:
             have = ws.numel() * ws.element_size()
-        strides = [s for t in ins for s in t.stride()[:3]] + list(lse.stride()) + [s for t in outs for s in t.stride()[:3]]
+        strides = [s for t in ins for s in t.stride()[:3]] + list(lse.stride())
         p = _native.FabAttentionBwdParams.from_buffer_copy(_BWD_RECORD.pack(
-            *[t.data_ptr() for t in ins], lse.data_ptr(), *[t.data_ptr() for t in outs], *strides, *cu, *sizes,
+            *[t.data_ptr() for t in ins], lse.data_ptr(), *[t.data_ptr() for t in outs], *strides, *sq[:3], *sk[:3],
+            *sv[:3], *cu, *sizes,
             float(sm_scale), causal, ws.data_ptr() if ws is not None else 0, have))
         rc = _native.lib.fab_attention_bwd(ctypes.byref(p), _native.current_stream_handle(dev))
     _native.check(rc, what)

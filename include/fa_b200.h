@@ -180,7 +180,7 @@ int fab_attention_fwd_varlen(const fab_attention_varlen_params* params, void* st
  * The workspace (fab_attention_bwd_workspace bytes, 256-byte aligned, not
  * initialised) belongs to the call until it completes on its stream.  Both
  * entries return FAB_ERR_UNSUPPORTED for more than 2^31 - 1 pieces of work
- * (batch x heads x 128-row tiles, 64-row ones past head_dim 128).
+ * (batch x heads x 128-row tiles, of queries and of keys).
  */
 typedef struct fab_attention_bwd_params {
   const void* q;
