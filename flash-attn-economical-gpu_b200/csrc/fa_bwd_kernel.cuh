@@ -83,7 +83,6 @@ struct BwdElem<__nv_bfloat16> {
     return *reinterpret_cast<uint32_t*>(&h);
   }
   __device__ static float2 unpack2(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
-  __device__ static float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
 };
 template <>
 struct BwdElem<__half> {
@@ -105,7 +104,6 @@ struct BwdElem<__half> {
     return *reinterpret_cast<uint32_t*>(&h);
   }
   __device__ static float2 unpack2(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
-  __device__ static float to_f(__half x) { return __half2float(x); }
 };
 
 // Tile shapes by padded head dim.  Streamed tiles have 128 rows up to head
