@@ -110,8 +110,10 @@ BwdPlan make_plan(const fab_attention_bwd_params* p) {
   if (w.k_tiles > 0) dkv = double(streamed_tiles(w.k_tiles, M, bs, causal, true)) / w.k_tiles * group * dsplit * per_kv * w.part_k_tiles;
   if (w.q_tiles > 0) dq = double(streamed_tiles(w.q_tiles, N, bs, causal, false)) / w.q_tiles * per_q * w.part_q_tiles;
   const double share = (4 * dkv + 3 * dq) / kSms;
-  choose_slices(ceil_div(M, bs) * group, share / 4, &w.dkv_slice_len, &w.dkv_slices);
-  choose_slices(ceil_div(N, bs), share / 3, &w.dq_slice_len, &w.dq_slices);
+  // (Where there is no tile, a long sum of nothing is not cut: no item would
+  // write its slices, and there is nothing to join.)
+  choose_slices(w.k_tiles > 0 ? ceil_div(M, bs) * group : 0, share / 4, &w.dkv_slice_len, &w.dkv_slices);
+  choose_slices(w.q_tiles > 0 ? ceil_div(N, bs) : 0, share / 3, &w.dq_slice_len, &w.dq_slices);
   const int64_t tiles = w.stat_tiles * per_q;
   size_t at = round256(size_t(tiles) * 2 * bs * sizeof(float));
   w.row_norm = at;
