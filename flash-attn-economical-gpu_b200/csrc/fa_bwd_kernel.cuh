@@ -17,7 +17,8 @@
 //     shared memory.
 //   * dQ items: Q and dO tiles stationary, K and V tiles streamed,
 //     S = Q K^T, dP = dO V^T, dQ += dS K.
-// S and dP are formed twice (7 products instead of 5), and in return every
+// S and dP are formed twice (7 products instead of 5; at head dims past 128
+// three times, 9 products, see BwdCfg), and in return every
 // output element is summed in one accumulator in a fixed order: no fp32 dQ
 // traffic through L2, no atomics, the same bits from call to call, and shared
 // heads need no second reduction.
@@ -40,19 +41,25 @@
 // dS it runs dV(i) and S(i+1).  P overwrites its own half of S, dS its own
 // half of dP, so no warp writes columns another still has to read.
 //
-// What bounds it.  B1 H16 S4096 D128 (bf16, all pairs) takes 353 us, 973 TF/s
-// of the five products that the formula needs and 1360 TF/s of the seven that
-// run: the rate a plain GEMM sustains here under the power limit.  A tile of a
-// dK/dV item is 2048 tensor-core cycles against some 2400 of the softmax warps'
-// chain (S's wait, 64 exponentials a lane, P's store, dP's wait, dS's store).
-// Causal 4 x 32 heads of S 1024 (184 us, 467 TF/s) spends a further 15 % on the
-// accumulators' read-out and stores, which nothing overlaps (the stores alone
-// 3 %), and 15 us on the statistics.  At head dim 64 the same exponentials stand
-// against half the products: 32 heads S 4096 566 us, 607 TF/s.  At 256, 2 x 16
-// heads S 4096 causal 1170 us, 590 TF/s: products of 64 streamed rows read each
-// stationary operand from shared memory for half the work, some 2250 cycles of
-// its bandwidth against 1536 of the tensor core's; a second half-tile slot for
-// dO in place of its single one changed nothing.
+// What bounds it (times: ten calls back to back, the best of several such
+// groups; in a long run the power limit lowers the clock).  B1 H16 S4096 D128
+// (bf16, all pairs) takes 353 us, 973 TF/s of the five products that the
+// formula needs and 1362 of the seven that run, against 1633 of a plain GEMM in
+// a run as short; over two seconds 398 us, 1209 against the GEMM's 1360.  The
+// tensor pipe is active 69 % of the time: a tile of a dK/dV item is 2048
+// tensor-core cycles against some 2400 of the softmax warps' chain (S's wait,
+// 64 exponentials a lane, P's store, dP's wait, dS's store).
+// Causal 4 x 32 heads of S 1024 (173 us, 497 TF/s; 132 us of this kernel and 18
+// of the statistics at the full clock) works through 62 such tiles per SM, 58 %
+// of this kernel's cycles; the rest lies around its 14 items: the accumulators'
+// read-out and stores, which nothing overlaps, were 15 % of the time (the
+// stores alone 3 %), what starts and ends the pipeline was not taken apart.
+// At head dim 64 the same exponentials stand against half the products: 32
+// heads S 4096 516 us, 666 TF/s (645 us on a GPU already at its power limit).
+// At 256, 2 x 16 heads S 4096 causal 1176 us, 585 TF/s: products of 64 streamed
+// rows read each stationary operand from shared memory for half the work, some
+// 2250 cycles of its bandwidth against 1536 of the tensor core's; a second
+// half-tile slot for dO in place of its single one changed nothing.
 //
 // P and dS are handed on in halves (kHalves): B1 H16 S4096 353 us against 365
 // in one piece.  16 softmax warps (32 columns each) and exponentials by
@@ -94,7 +101,9 @@ struct BwdElem<__half> {
   // largest of the row or of the item's rows, and of the sequence's keys) to
   // [2^14, 2^15); the epilogue divides it out.  (With the largest element of dO
   // brought to [1, 2) instead, 8092 keys and rows of different size took the
-  // error against 64 bits to 1.6 times the rounding's; now 1.4.)
+  // error against 64 bits to 1.6 times the rounding's; now 1.4.)  What that
+  // leaves: dS is subnormal below 2^-29 of the bound and 0 below 2^-39, so dk
+  // of a key whose every probability is that small has an absolute precision.
   static constexpr bool kScaled = true;
   // P itself is an operand of dV: as P * 2^12 it keeps its precision down to
   // 2^-26, and its largest value, 1, stays far below fp16's 65504.
@@ -110,7 +119,10 @@ struct BwdElem<__half> {
 // dim 128; at 256 shared memory holds the two stationary tiles (128 KB) and
 // three 64-row ones.  dK and dV together exceed TMEM at 256, so there a dK/dV
 // item forms S and dP over the whole head dim but 128 columns of each output,
-// and two items cover a key tile.
+// and two items cover a key tile: with dQ's, S and dP are formed three times,
+// nine products instead of the formula's five.  Head dims 129 to 255 run as 256
+// (2 x 16 heads S 2048 causal: D 160, 192 and 256 all 345 us), 65 to 127 as 128
+// (D 72, 80, 96 and 128: 124 to 134 us).
 //
 // The two streamed operands have a ring each.  The first (Q, or K) is read by
 // S(i) and again by dK(i) or dQ(i), a whole tile's time later, and its next

@@ -1007,7 +1007,8 @@ __device__ __forceinline__ int rope_row(const RopeParams& p, int axis, int64_t t
 // k in and out once; the table rows stay in L1 and L2.  A position outside the
 // table makes its pairs NaN; nothing is read out of bounds.  Measured: a call of
 // 16384 tokens, 28 + 4 heads of 128, bf16, 268 MB, takes 53 us with a cold L2
-// (5.1 TB/s); two heads per thread 59, one 69, six 67, eight 55.
+// (5.0 TB/s), 50 among other calls; with a cold L2 two heads per thread 59, one
+// 69, six 67, eight 55.  fp32, 537 MB: 90 us (6.0 TB/s), 87.
 constexpr int kRopeHeads = 4;
 template <typename T, int V>
 __global__ void __launch_bounds__(256, 3) rope_axes_kernel(const RopeParams p) {

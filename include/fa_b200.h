@@ -167,15 +167,18 @@ int fab_attention_fwd_varlen(const fab_attention_varlen_params* params, void* st
  * rows: small gradients do not underflow, large values do not overflow.  Masks
  * as in the forward.  Query rows that see no key (lse -inf; their o is ignored)
  * get dq 0, keys that no query sees dk = dv = 0, and rows of a packed tensor
- * outside [cu[0], cu[batch]) zero gradients.  No counterpart in the reference,
- * which has no backward pass.
+ * outside [cu[0], cu[batch]) zero gradients.  As in the forward, an infinite or
+ * NaN row reaches masked pairs of its own sequence within a 128-row tile (0
+ * times it is NaN), and never another sequence.  No counterpart in the
+ * reference, which has no backward pass.
  *
  * f16 or bf16 (FAB_ERR_UNSUPPORTED for f32: the forward's f32 runs as tf32),
  * head_dim <= 256, any finite sm_scale.  Tensors as in the forward: element
  * strides, stride 1 along head_dim, 16-byte aligned bases and outer strides;
  * packed tensors use stride_s / stride_h (stride_b is ignored) and lse
  * [head, token] through lse_stride_h / lse_stride_s.  seqlen_q / seqlen_k are
- * the longest lengths of a packed batch.  Gradients may not alias inputs.
+ * the longest lengths of a packed batch; rows of a sequence past them are left
+ * out, their gradients unwritten.  Gradients may not alias inputs.
  *
  * The workspace (fab_attention_bwd_workspace bytes, 256-byte aligned, not
  * initialised) belongs to the call until it completes on its stream.  Both
