@@ -47,6 +47,11 @@ def _tma_ready(t: torch.Tensor, strides: tuple[int, ...]) -> bool:
     return all((s * es) % 16 == 0 for s, n in zip(strides[:-1], t.shape[:-1]) if n > 1)
 
 
+def _store_ready(t: torch.Tensor) -> bool:
+    """_tma_ready for an output, whose strides the library also checks where their dim has one element."""
+    return _tma_ready(t, t.stride()) and all(s * t.element_size() % 16 == 0 for s in t.stride()[:-1])
+
+
 def _padded_like(t: torch.Tensor) -> torch.Tensor:
     """Uninitialised tensor shaped like `t` whose rows start on 16-byte boundaries."""
     per16 = 16 // t.element_size()
@@ -144,7 +149,7 @@ def _launch_attention(
         # Uniform weights over the visible keys; a vanishing positive scale gives the same weights.
         sm_scale = 1e-30
     qc, kc, vc = _conform(q), _conform(k), _conform(v)
-    oc = o if _tma_ready(o, tuple(o.stride())) else _padded_like(o)
+    oc = o if _store_ready(o) else _padded_like(o)
     lc = lse
     if lse is not None and lse.data_ptr() % 4:
         lc = torch.empty_like(lse, memory_format=torch.contiguous_format)
@@ -491,7 +496,7 @@ def attention_forward_varlen(
     # [total, heads, D] viewed as [1, total, heads, D] -> conform as [1, heads, total, D] views.
     qc, kc, vc = (_conform(t.unsqueeze(0).transpose(1, 2)).transpose(1, 2).squeeze(0) for t in (q, k, v))
     o4 = o.unsqueeze(0).transpose(1, 2)
-    oc = o if _tma_ready(o4, tuple(o4.stride())) else _padded_like(o4).transpose(1, 2).squeeze(0)
+    oc = o if _store_ready(o4) else _padded_like(o4).transpose(1, 2).squeeze(0)
     cq, ck = cu_seqlens_q.contiguous(), cu_seqlens_k.contiguous()
     p = _native.FabAttentionVarlenParams()
     p.q, p.k, p.v, p.o = qc.data_ptr(), kc.data_ptr(), vc.data_ptr(), oc.data_ptr()
