@@ -83,7 +83,7 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_tiled_fn() {
 template <typename F>
 static int encode_map(F encode) {
   CUresult r = encode();
-  if (r != CUDA_SUCCESS) {
+  if (r == CUDA_ERROR_INVALID_CONTEXT || r == CUDA_ERROR_NOT_INITIALIZED) {
     int device = 0;
     if (cudaGetDevice(&device) != cudaSuccess || cudaSetDevice(device) != cudaSuccess) return kErrCuda;
     r = encode();
